@@ -18,6 +18,7 @@ HOST_LIB_PATH = os.path.join(LIBDIR, "libgotensor_host.so")
 MAX_DIMS = 8
 FLOAT32, FLOAT64 = 0, 1
 ACT_NONE, ACT_RELU, ACT_TANH, ACT_SIGMOID = 0, 1, 2, 3
+STATE_NATIVE, STATE_E4M3 = 0, 1
 
 
 class GtView(ctypes.Structure):
@@ -36,6 +37,12 @@ class SgdCfg(ctypes.Structure):
 class AdamCfg(ctypes.Structure):
     _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
                 ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double)]
+
+
+class AdamwTensor(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_void_p), ("g", ctypes.c_void_p), ("m", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("m_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("n", ctypes.c_int64),
+                ("lr_mul", ctypes.c_double), ("wd_mul", ctypes.c_double)]
 
 
 class Layer(ctypes.Structure):
@@ -114,6 +121,14 @@ CUDA_API = {
     "gt_sgd_step": ("err", [_P, _INT, _P, _P, _P, _I64, ctypes.POINTER(SgdCfg), _INT]),
     "gt_adam_step": ("err", [_P, _INT, _P, _P, _P, _P, _I64, ctypes.POINTER(AdamCfg), _I64]),
     "gt_adam_step_dev": ("err", [_P, _INT, _P, _P, _P, _P, _I64, ctypes.POINTER(AdamCfg), _P]),
+    "gt_linear_xent_fwd_bwd": ("err", [_P, _INT, _P, _P, _P, _P, _I64, _I64, _I64, ctypes.c_int32, _I64, _P, _P, _P,
+                                       _P, _P, _P]),
+    "gt_adamw_new": ("err", [_P, _INT, _INT, ctypes.POINTER(AdamwTensor), _I64, _P, ctypes.c_uint64,
+                             ctypes.POINTER(_P)]),
+    "gt_adamw_free": ("err", [_P]),
+    "gt_adamw_set_grads": ("err", [_P, ctypes.POINTER(_P), _I64]),
+    "gt_adamw_clip": ("err", [_P, _D, _P]),
+    "gt_adamw_step": ("err", [_P, ctypes.POINTER(AdamCfg), _P, _P]),
     "gt_comm_unique_id": ("err", [ctypes.c_char_p]),
     "gt_comm_init": ("err", [_P, _INT, _INT, ctypes.c_char_p, _INT]),
     "gt_allreduce_avg": ("err", [_P, _INT, _P, _I64]),

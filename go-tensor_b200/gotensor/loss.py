@@ -1,0 +1,39 @@
+"""The loss of a classifier head over a large vocabulary.
+
+``linear_cross_entropy`` is ``gt_linear_xent_fwd_bwd`` (include/gt_cuda.h): a
+Linear, its softmax cross-entropy and every gradient, without keeping the
+logits. Buffers are device addresses, or storages of ``gotensor.backend``
+(whose lengths and dtypes are then checked). The call is queued on the
+context's stream and does not wait.
+"""
+from __future__ import annotations
+
+from . import _lib
+from ._lib import FLOAT32, check
+from .backend import Context, CudaStorage
+
+
+def address(buf, n=None, dt=None, what="buffer"):
+    """The device address of a storage (checked for length and dtype) or of an address, None for None."""
+    if buf is None:
+        return None
+    if isinstance(buf, CudaStorage):
+        if n is not None and buf.n < n:
+            raise ValueError(f"{what}: {n} elements wanted, the storage has {buf.n}")
+        if dt is not None and buf.dt != dt:
+            raise TypeError(f"{what}: mixed dtypes")
+        return buf.ptr
+    return int(buf)
+
+
+def linear_cross_entropy(x, w, bias, labels, M, K, V, *, loss, rows=None, dx=None, dw=None, db=None, bad_label=None,
+                         ignore_label=-100, workspace_bytes=0, dtype=FLOAT32, device=0):
+    """loss = mean over the rows that count of -log softmax(x w^T + bias)[label], each row's own loss in ``rows`` and
+    the gradients in ``dx`` (M, K), ``dw`` (V, K) and ``db`` (V); each of the four may be None. ``labels`` and
+    ``bad_label`` are addresses of int32 on the device. Rows labelled ``ignore_label`` take no part."""
+    ctx = Context.get(device)
+    check(ctx.lib.gt_linear_xent_fwd_bwd(
+        ctx.ptr, dtype, address(x, M * K, dtype, "x"), address(w, V * K, dtype, "w"), address(bias, V, dtype, "bias"),
+        address(labels), M, K, V, ignore_label, workspace_bytes, address(loss, 1, dtype, "loss"),
+        address(rows, M, dtype, "rows"), address(dx, M * K, dtype, "dx"), address(dw, V * K, dtype, "dw"),
+        address(db, V, dtype, "db"), address(bad_label)))

@@ -1,0 +1,95 @@
+"""AdamW over many tensors in one launch (``gt_adamw_*``, include/gt_cuda.h)."""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Any
+
+from . import _lib
+from ._lib import FLOAT32, STATE_E4M3, STATE_NATIVE, AdamCfg, AdamwTensor, check
+from .backend import Context
+from .loss import address
+
+BLOCK = 256  # values that share a scale of an 8-bit state
+
+
+@dataclass
+class Tensor:
+    """One parameter tensor of ``n`` values: device addresses or storages of the parameters, gradients and states
+    (codes and scales for 8-bit states), and its factors on the learning rate and the weight decay."""
+    p: Any
+    g: Any
+    m: Any
+    v: Any
+    n: int
+    m_scale: Any = None
+    v_scale: Any = None
+    lr_mul: float = 1.0
+    wd_mul: float = 1.0
+
+
+class AdamW:
+    """``step`` is the address of the device's int64 step counter; ``state`` STATE_NATIVE or STATE_E4M3 (8 bits, with
+    stochastic rounding from ``seed``). The buffers stay the caller's and have to outlive the optimizer's use."""
+
+    def __init__(self, tensors, *, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,
+                 state=STATE_NATIVE, seed=0, dtype=FLOAT32, device=0):
+        self.ctx = Context.get(device)
+        self.lib = self.ctx.lib
+        self.cfg = AdamCfg(lr, beta1, beta2, eps, weight_decay)
+        held = None if state == STATE_E4M3 else dtype
+        self.tensors = list(tensors)  # keeps the storages alive
+        arr = (AdamwTensor * max(1, len(self.tensors)))()
+        for a, t in zip(arr, self.tensors):
+            a.p, a.g = address(t.p, t.n, dtype, "p"), address(t.g, t.n, dtype, "g")
+            a.m = address(t.m, t.n if held is not None else None, held, "m")
+            a.v = address(t.v, t.n if held is not None else None, held, "v")
+            a.m_scale = address(t.m_scale, -(-t.n // BLOCK), FLOAT32, "m_scale")
+            a.v_scale = address(t.v_scale, -(-t.n // BLOCK), FLOAT32, "v_scale")
+            a.n, a.lr_mul, a.wd_mul = t.n, t.lr_mul, t.wd_mul
+        self._step = step
+        self.dtype = dtype
+        self._clip = None
+        self.ptr = None
+        p = ctypes.c_void_p()
+        check(self.lib.gt_adamw_new(self.ctx.ptr, dtype, state, arr, len(self.tensors), address(step), seed,
+                                    ctypes.byref(p)))
+        self.ptr = p
+
+    def close(self):
+        """Frees the handle (not while the stream is captured)."""
+        p, self.ptr = self.ptr, None
+        if p:
+            check(self.lib.gt_adamw_free(p))
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # interpreter shutdown
+            pass
+
+    def set_grads(self, grads):
+        """New gradient buffers, one per tensor, for every later call."""
+        grads = list(grads)
+        if len(grads) != len(self.tensors):
+            raise ValueError(f"{len(grads)} gradients for {len(self.tensors)} tensors")
+        arr = (ctypes.c_void_p * max(1, len(grads)))(
+            *[address(g, t.n, self.dtype, "g") for g, t in zip(grads, self.tensors)])
+        check(self.lib.gt_adamw_set_grads(self.ptr, arr, len(grads)))
+        for t, g in zip(self.tensors, grads):
+            t.g = g
+
+    def clip_grad_norm(self, max_norm, out):
+        """Writes the gradients' global norm and the coefficient min(1, max_norm / norm) to the two doubles at the
+        device address ``out``; the next ``step`` multiplies the gradients by it."""
+        out = address(out)
+        check(self.lib.gt_adamw_clip(self.ptr, max_norm, out))
+        self._clip = out
+
+    def step(self, lr=None, lr_device=None):
+        """One update; ``lr`` replaces the learning rate from here on, ``lr_device`` is a device double that
+        replaces it for this call (and for the replays of a graph that captured it)."""
+        if lr is not None:
+            self.cfg.lr = lr
+        clip, self._clip = self._clip, None
+        check(self.lib.gt_adamw_step(self.ptr, ctypes.byref(self.cfg), clip, address(lr_device)))

@@ -332,6 +332,38 @@ GT_API char* gt_xent_fwd_bwd_db(gt_ctx* ctx, int dtype, const void* logits, cons
 GT_API char* gt_xent_fwd_bwd_noalloc(gt_ctx* ctx, int dtype, const void* logits, const int32_t* labels, int64_t B,
                                      int64_t C, void* loss, void* dlogits, int32_t* bad_label);
 
+/* Softmax cross-entropy of a Linear over a large vocabulary, with all
+ * gradients, without keeping the logits: for x (M, K), w (V, K), bias (V)
+ * (NULL: none) and int32 labels (M) on the device,
+ *   z = x @ w^T + bias,  lse_i = log sum_v exp(z_iv),
+ *   row_loss_i = lse_i - z_i,label(i),  loss = sum_i row_loss_i / n,
+ *   g_iv = (exp(z_iv - lse_i) - [v == label(i)]) / n,
+ *   dx (M, K) = g @ w,  dw (V, K) = g^T @ x,  db (V) = the column sums of g.
+ * row_loss (M), dx, dw and db may each be NULL; with the last three NULL the
+ * call is a forward pass. Every output is overwritten.
+ * Rows whose label is ignore_label (any value; one outside [0, V) to pass
+ * over no class) take no part: n counts the others, row_loss and the rows of
+ * dx are 0, and their x may hold anything, NaN included. With every row
+ * ignored the loss is NaN, as the mean of nothing is, and the gradients are
+ * 0. A label that is neither in [0, V) nor ignore_label sets *bad_label
+ * (device int32, may be NULL) to 1 and makes its row_loss and the loss NaN.
+ * bias may mask classes with -infinity (probability and gradient 0). A row
+ * whose every class is masked has no distribution: its row_loss, its row of
+ * dx, and the loss, dw and db of the call are NaN. Infinities and NaN in a row
+ * of x that counts, or in w, may turn any output that depends on them into
+ * NaN.
+ * The logits exist only in pieces of rows whose workspace stays within
+ * workspace_bytes (0: 1 GiB; at least one piece of 128 rows is used whatever
+ * it says). No output may overlap an input or another output. The result does
+ * not depend on timing: the same call gives the same bits. Replaces Linear
+ * followed by CrossEntropyLoss (nn/module.go:51-53, nn/loss.go:12-14) and
+ * their backward for vocabularies whose logits are too large to keep; there
+ * is no counterpart of the ignored label in the reference. */
+GT_API char* gt_linear_xent_fwd_bwd(gt_ctx* ctx, int dtype, const void* x, const void* w, const void* bias,
+                                    const int32_t* labels, int64_t M, int64_t K, int64_t V, int32_t ignore_label,
+                                    int64_t workspace_bytes, void* loss, void* row_loss, void* dx, void* dw, void* db,
+                                    int32_t* bad_label);
+
 /* Optimizer hyperparameters (optim.SGDConfig / optim.AdamConfig,
  * optim/optim.go:22-27, 74-80). */
 typedef struct {
@@ -356,6 +388,57 @@ GT_API char* gt_adam_step(gt_ctx* ctx, int dtype, void* p, const void* g, void* 
  * the update. No counterpart in the reference (graph capture). */
 GT_API char* gt_adam_step_dev(gt_ctx* ctx, int dtype, void* p, const void* g, void* m, void* v, int64_t n,
                        const gt_adam_cfg* cfg, int64_t* step_dev);
+
+/* AdamW (decoupled weight decay) over many tensors in one launch. A handle
+ * keeps the tensors' addresses and a table of their pieces; the step is
+ *   g' = g * clip coefficient (1 without one)
+ *   m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2
+ *   p = p (1 - lr wd) - m lr / (1 - beta1^t) / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * with lr = cfg->lr * lr_mul, wd = cfg->weight_decay * wd_mul of the tensor
+ * and every operation rounded to the dtype (bias corrections in float64).
+ * State formats: GT_STATE_NATIVE keeps m and v in the dtype. GT_STATE_E4M3
+ * (float32 parameters) keeps m and sqrt(v) as one e4m3 code per value (sign,
+ * 4 bits of exponent, 3 of mantissa; value = code value * scale) and a
+ * float32 scale per 256 values of a tensor, rounded up or down at random with
+ * the probability of the distance by a hash of (seed, step, place): the same
+ * seed and step give the same bits. All-zero codes and scales are the initial
+ * state. A value that is not finite is kept as the NaN code.
+ * No counterpart in the reference (whose Adam, optim/optim.go:110-132, updates
+ * one tensor at a time and adds the decay to the gradient). */
+enum { GT_STATE_NATIVE = 0, GT_STATE_E4M3 = 1 };
+typedef struct {
+  void* p;        /* parameters, n elements of the dtype */
+  const void* g;  /* gradients */
+  void* m;        /* first moment: n elements, or n codes */
+  void* v;        /* second moment: n elements, or n codes of its square root */
+  float* m_scale; /* GT_STATE_E4M3: ceil(n / 256) scales (else unused) */
+  float* v_scale;
+  int64_t n;
+  double lr_mul;  /* factor on cfg->lr (1: none) */
+  double wd_mul;  /* factor on cfg->weight_decay (1: none, 0: no decay) */
+} gt_adamw_tensor;
+typedef struct gt_adamw gt_adamw;
+/* Makes a handle for `count` tensors (copied; their buffers stay the
+ * caller's) and the device step counter (int64, the steps taken so far, the
+ * caller's; 0 at the start of training). Any alignment of the elements works;
+ * 16-byte aligned (native: equally misaligned) arrays are fastest. Nothing
+ * that the step writes may overlap anything else it touches. Not during
+ * capture. Free the handle before its context. */
+GT_API char* gt_adamw_new(gt_ctx* ctx, int dtype, int state, const gt_adamw_tensor* tensors, int64_t count,
+                          int64_t* step_dev, uint64_t seed, gt_adamw** out);
+GT_API char* gt_adamw_free(gt_adamw* opt);
+/* New gradient addresses, one per tensor, for every later call (not during capture). */
+GT_API char* gt_adamw_set_grads(gt_adamw* opt, const void* const* grads, int64_t count);
+/* clip (device, 2 doubles) = the Euclidean norm of all gradients, and the
+ * coefficient min(1, max_norm / norm), NaN when the norm is not finite. */
+GT_API char* gt_adamw_clip(gt_adamw* opt, double max_norm, double* clip);
+/* One step, advancing the step counter. clip: NULL, or the device pair of
+ * gt_adamw_clip, whose coefficient multiplies the gradients; with a NaN
+ * coefficient the step changes nothing and the counter stays. lr_dev: NULL,
+ * or a device double that replaces cfg->lr (a schedule under a captured
+ * graph). cfg's fields are taken as they are (0 is 0). Captured into a graph,
+ * a replay is a further step. */
+GT_API char* gt_adamw_step(gt_adamw* opt, const gt_adam_cfg* cfg, const double* clip, const double* lr_dev);
 
 /* ---- data parallelism (no counterpart in the reference) ------------------ */
 
