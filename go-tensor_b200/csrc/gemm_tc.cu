@@ -64,10 +64,10 @@
 #include <type_traits>
 
 #include "gemm.cuh"
+#include "split_gemm.cuh"
+#include "tc_pipe.cuh"
 
 namespace gt {
-
-__device__ int g_tc_error = 0;
 
 namespace tc {
 
@@ -162,7 +162,6 @@ constexpr uint32_t BUF_COLS = 256;
 // the split keeps the block's total: 256 * 64 + 256 * 192 = 256 * 128 * 2.
 constexpr int REGS_LOW = 64, REGS_HIGH = 192;
 static_assert(256 * REGS_LOW + 256 * REGS_HIGH <= THREADS * 128, "register split exceeds the launch's registers");
-constexpr uint64_t kTimeoutNs = 2000000000ull;  // default limit, 2 s; a healthy wait takes microseconds
 
 // Where an operand comes from. A: TMA, or gathered by the splitter warps as
 // im2col values with positions on the rows (A_IM2COL_POS) or patch entries
@@ -217,112 +216,6 @@ struct Gather {
   int b_lo_row = 0;         // B_SPLIT2: first row of the lo plane
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-
-__device__ __forceinline__ uint32_t cluster_id() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
-  return r;
-}
-
-__device__ __forceinline__ uint32_t num_clusters() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%nclusterid.x;" : "=r"(r));
-  return r;
-}
-
-// The shared::cluster address of a local shared-memory object in CTA `rank`.
-__device__ __forceinline__ uint32_t map_to_rank(uint32_t local, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
-  return r;
-}
-
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-
-// Arrival on the barrier at the same offset in CTA `rank` of the cluster.
-__device__ __forceinline__ void mbar_arrive_rank(uint64_t* bar, uint32_t rank) {
-  uint32_t remote = map_to_rank(smem_u32(bar), rank);
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-__device__ __forceinline__ uint64_t globaltimer() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-
-// Waits for the phase of `bar` with the given parity; false (and the error
-// word set to `site`) once `limit_ns` has passed.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int site, uint64_t limit_ns) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer();
-  while (!mbar_try_wait(bar, parity)) {
-    if (globaltimer() - t0 > limit_ns) {
-      atomicCAS(&g_tc_error, 0, site);
-      return false;
-    }
-  }
-  return true;
-}
-
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-          smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
-      : "memory");
-}
-
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::
-          "r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
-
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
-                                            int c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
-          "r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
-}
-
-__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
 // Shared-memory matrix descriptor (tcgen05 "version 1").
 //   K-major operands: 64-byte rows (16 fp32 of K) with the 64-byte swizzle;
 //     8-row groups 512 B apart (SBO); one K step (8 tf32) is +32 bytes.
@@ -332,16 +225,6 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 //     step (8 rows) is +1024 bytes.
 constexpr uint32_t kLayoutSw64 = 4, kLayoutSw128Atom32 = 1;
 constexpr uint32_t kLboMN = BK * 128;
-
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo, uint32_t layout) {
-  uint64_t d = 0;
-  d |= (uint64_t)((addr >> 4) & 0x3FFF);
-  d |= (uint64_t)((lbo >> 4) & 0x3FFF) << 16;
-  d |= (uint64_t)((sbo >> 4) & 0x3FFF) << 32;
-  d |= (uint64_t)1 << 46;  // descriptor version for tcgen05
-  d |= (uint64_t)layout << 61;
-  return d;
-}
 
 template <bool MN>
 __device__ __forceinline__ uint64_t operand_desc(uint32_t base, int kk) {
@@ -387,41 +270,6 @@ __device__ __forceinline__ void mma_tf32_pair_tmem_a(uint32_t tmem_d, uint32_t t
 }
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// One lane of the converged warp (elect.sync): the producer and MMA warps run
-// their loops warp-wide, so addresses and descriptors stay warp-uniform, and
-// only the elected lane issues the copies, MMAs and commits.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t e;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
-  return e != 0;
-}
-
-// Arrives on `bar` in both CTAs of the pair once the MMAs issued so far complete.
-__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          smem_u32(bar)),
-      "h"((uint16_t)3)
-      : "memory");
-}
-
-__device__ __forceinline__ void tmem_load32(uint32_t taddr, float* v) {
-  uint32_t r[32];
-  // Load and wait in one asm block: the registers are valid only after the wait.
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
-}
 
 __device__ __forceinline__ void tmem_store32(uint32_t taddr, const float* v) {
   asm volatile(
@@ -1432,10 +1280,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TL::TMEM_COLS));
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 // 2-D fp32 tensor map over `outer` rows of `inner` contiguous elements with a
 // pitch of `ld` elements; zero fill outside. K-major operands: box 16 x
 // box_rows with the 64-byte swizzle; M/N-major: box 32 x 16 with the
@@ -1938,6 +1782,12 @@ static bool fits32(const gt_geom& g, int64_t chans_out) {
 void set_gemm_splits(int splits) { tc::g_force_splits = splits; }
 void set_tc_wait_limit_us(int64_t us) { tc::g_wait_limit_ns = us > 0 ? (uint64_t)us * 1000ull : tc::kTimeoutNs; }
 void tc_withhold_next_arrive() { tc::g_withhold_next = 1; }
+uint64_t tc_wait_limit_ns() { return tc::g_wait_limit_ns; }
+int tc_take_withhold() {
+  const int w = tc::g_withhold_next;
+  tc::g_withhold_next = 0;
+  return w;
+}
 
 // Reports (and clears) a timed-out pipeline wait of an earlier tcgen05 GEMM.
 char* tc_check_errors() {
@@ -1948,7 +1798,7 @@ char* tc_check_errors() {
     cudaMemcpyToSymbol(g_tc_error, &zero, sizeof zero);
     return errorf("tcgen05 GEMM: a pipeline wait timed out (site %d); results are invalid", e);
   }
-  return nullptr;
+  return split_gemm_check_errors();
 }
 
 bool tc_writes_colsums(const Epi<float>& epi, int64_t n_cols) {

@@ -9,19 +9,29 @@
 //   dx = G w,  dw = G^T x,  db_v = sum_i G_iv
 //
 // The rows are taken in pieces: the logits of one piece live in workspace,
-// become the gradient in place and are overwritten by the next piece, so
-// memory does not grow with the number of rows.
+// become the gradient and are overwritten by the next piece, so memory does
+// not grow with the number of rows. float32 runs on the tensor cores
+// (split_gemm.cu):
+//
+//   operand_top_kernel   largest magnitudes of x and w, the rows that count
+//   operand_split_kernel x and w as two float16 planes each
+//   per piece of rows:
+//     split_gemm         z, and per strip of 128 classes of a row its maximum
+//                        and sum of exponentials, from the registers of the
+//                        product; a forward pass alone never writes z
+//     strip_join_kernel  the strips' pairs joined: lse, the rows' losses
+//     grad_planes_kernel z -> n G as two float16 planes, its column sums
+//     split_gemm         dx = G w, dw (+)= G^T x
+//   mean_rows_kernel     the loss
+//
+// float64 runs the same pieces over the FP64 GEMM.
 #include <algorithm>
 #include <cmath>
 
 #include "gemm.cuh"
+#include "split_gemm.cuh"
 
 namespace gt {
-
-__device__ __forceinline__ float exp_t(float x) { return expf(x); }
-__device__ __forceinline__ double exp_t(double x) { return exp(x); }
-__device__ __forceinline__ float log_t(float x) { return logf(x); }
-__device__ __forceinline__ double log_t(double x) { return log(x); }
 
 // counts[0] = rows that count (label != ignore); a label outside [0, V) sets *bad.
 __global__ void __launch_bounds__(1024) label_count_kernel(const int32_t* __restrict__ labels, int64_t M, int64_t V,
@@ -49,52 +59,49 @@ __global__ void __launch_bounds__(1024) label_count_kernel(const int32_t* __rest
 }
 
 // out = x with the ignored rows zeroed (padding may hold anything).
-template <typename T>
-__global__ void keep_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ labels, int64_t rows, int64_t K,
-                                 int32_t ignore, T* __restrict__ out) {
+__global__ void keep_rows_kernel(const double* __restrict__ x, const int32_t* __restrict__ labels, int64_t rows, int64_t K,
+                                 int32_t ignore, double* __restrict__ out) {
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < rows * K; i += (int64_t)gridDim.x * blockDim.x)
-    out[i] = labels[i / K] == ignore ? (T)0 : x[i];
+    out[i] = labels[i / K] == ignore ? 0.0 : x[i];
 }
 
 // Joins two running (maximum, sum of exp(z - maximum)) pairs.
-template <typename T>
-__device__ __forceinline__ void join(T& m, T& s, T m2, T s2) {
-  const T top = go_max(m, m2);
-  s = (m == top ? s : s * exp_t(m - top)) + (m2 == top ? s2 : s2 * exp_t(m2 - top));
+__device__ __forceinline__ void join(double& m, double& s, double m2, double s2) {
+  const double top = go_max(m, m2);
+  s = (m == top ? s : s * exp(m - top)) + (m2 == top ? s2 : s2 * exp(m2 - top));
   m = top;
 }
 
 // A block per row: the running maximum and sum in one pass over the row, then
 // the gradient in place.
-template <typename T>
-__global__ void __launch_bounds__(256) xent_piece_kernel(T* __restrict__ z, const int32_t* __restrict__ labels,
+__global__ void __launch_bounds__(256) xent_piece_f64_kernel(double* __restrict__ z, const int32_t* __restrict__ labels,
                                                          int64_t rows, int64_t V, int32_t ignore,
-                                                         const int64_t* __restrict__ counts, T* __restrict__ row_loss,
+                                                         const int64_t* __restrict__ counts, double* __restrict__ row_loss,
                                                          bool grad) {
-  __shared__ T wm[8], wsum[8];
-  const T inv = (T)(1.0 / (double)counts[0]);
+  __shared__ double wm[8], wsum[8];
+  const double inv = 1.0 / (double)counts[0];
   for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
-    T* zr = z + i * V;
+    double* zr = z + i * V;
     const int32_t y = labels[i];
     if (y == ignore) {
-      if (threadIdx.x == 0) row_loss[i] = (T)0;
+      if (threadIdx.x == 0) row_loss[i] = 0.0;
       if (grad)
-        for (int64_t j = threadIdx.x; j < V; j += blockDim.x) zr[j] = (T)0;
+        for (int64_t j = threadIdx.x; j < V; j += blockDim.x) zr[j] = 0.0;
       continue;
     }
-    T m = (T)(-INFINITY), s = (T)0;
+    double m = -INFINITY, s = 0.0;
     for (int64_t j = threadIdx.x; j < V; j += blockDim.x) {
-      const T v = zr[j];
+      const double v = zr[j];
       if (v > m) {
-        s = s * exp_t(m - v) + (T)1;
+        s = s * exp(m - v) + 1.0;
         m = v;
-      } else if (v != (T)(-INFINITY)) {  // (a NaN comes here too)
-        s += exp_t(v - m);
+      } else if (v != -INFINITY) {  // (a NaN comes here too)
+        s += exp(v - m);
       }
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
-      const T m2 = __shfl_xor_sync(0xffffffffu, m, off), s2 = __shfl_xor_sync(0xffffffffu, s, off);
+      const double m2 = __shfl_xor_sync(0xffffffffu, m, off), s2 = __shfl_xor_sync(0xffffffffu, s, off);
       join(m, s, m2, s2);
     }
     if ((threadIdx.x & 31) == 0) wm[threadIdx.x >> 5] = m, wsum[threadIdx.x >> 5] = s;
@@ -102,13 +109,13 @@ __global__ void __launch_bounds__(256) xent_piece_kernel(T* __restrict__ z, cons
     m = wm[0], s = wsum[0];
     for (int w = 1; w < 8; w++) join(m, s, wm[w], wsum[w]);
     const bool bad = y < 0 || y >= V;
-    if (threadIdx.x == 0) row_loss[i] = bad ? (T)NAN : log_t(s) + (m - zr[y]);
+    if (threadIdx.x == 0) row_loss[i] = bad ? (double)NAN : log(s) + (m - zr[y]);
     __syncthreads();  // the label's logit is read, and wm / wsum are free
     if (grad)
       // (not exp(z - lse): the logarithm would vanish beside a maximum that is
       // a mask's lowest value)
       for (int64_t j = threadIdx.x; j < V; j += blockDim.x) {
-        const T e = exp_t(zr[j] - m) / s * inv;
+        const double e = exp(zr[j] - m) / s * inv;
         zr[j] = j == y ? e - inv : e;
       }
   }
@@ -133,17 +140,16 @@ __global__ void __launch_bounds__(1024) mean_rows_kernel(const T* __restrict__ r
 }
 
 // db (+)= column sums of a piece's gradient, rows in order.
-template <typename T>
-__global__ void piece_columns_kernel(const T* __restrict__ g, int64_t rows, int64_t V, bool first, T* __restrict__ db) {
+__global__ void piece_columns_kernel(const double* __restrict__ g, int64_t rows, int64_t V, bool first,
+                                     double* __restrict__ db) {
   for (int64_t j = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; j < V; j += (int64_t)gridDim.x * blockDim.x) {
-    double acc = first ? 0.0 : (double)db[j];
-    for (int64_t i = 0; i < rows; i++) acc += (double)g[i * V + j];
-    db[j] = (T)acc;
+    double acc = first ? 0.0 : db[j];
+    for (int64_t i = 0; i < rows; i++) acc += g[i * V + j];
+    db[j] = acc;
   }
 }
 
-template <typename T>
-__global__ void add_kernel(T* __restrict__ out, const T* __restrict__ x, int64_t n) {
+__global__ void add_kernel(double* __restrict__ out, const double* __restrict__ x, int64_t n) {
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
     out[i] = out[i] + x[i];
 }
@@ -159,68 +165,361 @@ struct XentCall {
   int32_t* bad;
 };
 
-// float32 products on the FP32 pipe: the 3xTF32 path loses subnormal operands.
-static char* product(gt_ctx* ctx, const GemmShape& s, const float* A, const float* B, const Epi<float>& e) {
-  return gemm_simt<float>(ctx, s, A, B, e);
-}
-static char* product(gt_ctx* ctx, const GemmShape& s, const double* A, const double* B, const Epi<double>& e) {
-  return gemm<double>(ctx, s, A, B, e);
+// What the kernels of one float32 call share: the operands' largest finite
+// magnitudes (as ordered words), the rows that count, and the products' factors.
+struct XentMeta {
+  uint32_t x_top, w_top;
+  int64_t count;
+  SplitScale logits, dx, dw;
+};
+
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
 }
 
-// Pieces of rows over the GEMM entry points: one piece's logits in workspace.
-template <typename T>
-static char* linear_xent_pieces(gt_ctx* ctx, const XentCall<T>& c, void** held) {
+// The largest magnitudes of w (blocks 0 .. w_blocks - 1) and of the rows of x
+// that count (the other blocks, a warp per row), and those rows' number; a
+// label outside [0, V) sets *bad.
+__global__ void __launch_bounds__(256) operand_top_kernel(const float* __restrict__ x, const float* __restrict__ w,
+                                                          const int32_t* __restrict__ labels, int64_t M, int64_t K,
+                                                          int64_t V, int32_t ignore, int w_blocks, XentMeta* meta,
+                                                          int32_t* bad) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t top = 0;
+  if ((int)blockIdx.x < w_blocks) {
+    const int64_t n = V * K, n4 = ((uintptr_t)w & 15) == 0 ? n / 4 : 0, stride = (int64_t)w_blocks * 256;
+#pragma unroll 4
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += stride) {
+      const float4 v = reinterpret_cast<const float4*>(w)[i];
+      top = max(max(top, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
+    }
+#pragma unroll 4
+    for (int64_t i = n4 * 4 + (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride)
+      top = max(top, finite_bits(w[i]));
+  } else {
+    int64_t kept = 0;
+    for (int64_t m = (int64_t)(blockIdx.x - w_blocks) * 8 + warp; m < M; m += (int64_t)(gridDim.x - w_blocks) * 8) {
+      const int32_t y = labels[m];
+      if (y == ignore) continue;
+      kept++;
+      if (lane == 0 && bad && (y < 0 || y >= V)) *bad = 1;
+      const float* r = x + m * K;
+#pragma unroll 4
+      for (int64_t k = lane; k < K; k += 32) top = max(top, finite_bits(r[k]));
+    }
+    if (lane == 0 && kept) atomicAdd((unsigned long long*)&meta->count, (unsigned long long)kept);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0 && top) atomicMax((int)blockIdx.x < w_blocks ? &meta->w_top : &meta->x_top, top);
+}
+
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// The exponent e that puts a largest magnitude at 2^14 .. 2^15 when
+// multiplied by 2^e: -113 .. 163.
+__device__ __forceinline__ int plane_exponent(uint32_t top) {
+  if (top == 0) return 0;
+  return 14 - (top < 0x800000u ? 31 - __clz((int)top) - 149 : (int)(top >> 23) - 127);
+}
+
+// 2^-e and a factor f, the power in two halves (beyond 2^-252 nothing is left
+// of an accumulator anyway).
+__device__ __forceinline__ SplitScale undo(int e, float f) {
+  e = min(e, 252);
+  return {exp2_int(-e / 2), exp2_int(-e - (-e / 2)), f};
+}
+
+__device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
+  hi = __float2half_rn(v);
+  const float back = __half2float(hi);
+  lo = __float2half_rn(isfinite(back) ? __fsub_rn(v, back) : 0.0f);  // an infinity stays one
+}
+
+constexpr int kGradExponent = 15;  // n G lies in [-1, 1]
+
+// x (ignored rows as zeros) and w as planes of pitch Kp, a warp per row.
+__global__ void __launch_bounds__(256) operand_split_kernel(const float* __restrict__ x, const float* __restrict__ w,
+                                                            const int32_t* __restrict__ labels, int64_t M, int64_t K,
+                                                            int64_t V, int64_t Kp, int32_t ignore, XentMeta* meta,
+                                                            __half* __restrict__ xp, __half* __restrict__ wp) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int ex = plane_exponent(meta->x_top), ew = plane_exponent(meta->w_top);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    const float inv = (float)(1.0 / (double)meta->count);
+    meta->logits = undo(ex + ew, 1.0f);
+    meta->dx = undo(ew + kGradExponent, inv);
+    meta->dw = undo(ex + kGradExponent, inv);
+    if (meta->count == 0) meta->dx.f = meta->dw.f = 0.0f;  // no row counts: the gradients are 0
+  }
+  for (int64_t i = (int64_t)blockIdx.x * 8 + warp; i < M + V; i += (int64_t)gridDim.x * 8) {
+    const bool is_x = i >= V;
+    const int64_t row = is_x ? i - V : i;
+    const float* src = (is_x ? x : w) + row * K;
+    __half* hi = (is_x ? xp : wp) + row * Kp;
+    __half* lo = hi + (is_x ? M : V) * Kp;
+    const int e = is_x ? ex : ew;
+    const float f1 = exp2_int(e / 2), f2 = exp2_int(e - e / 2);
+    const bool keep = !is_x || labels[row] != ignore;
+    if ((K & 7) == 0 && ((uintptr_t)src & 15) == 0) {
+      for (int64_t k = lane; k < K / 8; k += 32) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+        if (keep) a = reinterpret_cast<const float4*>(src)[2 * k], b = reinterpret_cast<const float4*>(src)[2 * k + 1];
+        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        __align__(16) __half h[8], l[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) split_half(__fmul_rn(__fmul_rn(v[j], f1), f2), h[j], l[j]);
+        reinterpret_cast<uint4*>(hi)[k] = *reinterpret_cast<uint4*>(h);
+        reinterpret_cast<uint4*>(lo)[k] = *reinterpret_cast<uint4*>(l);
+      }
+    } else {
+#pragma unroll 4
+      for (int64_t k = lane; k < K; k += 32) split_half(__fmul_rn(__fmul_rn(keep ? src[k] : 0.0f, f1), f2), hi[k], lo[k]);
+    }
+  }
+}
+
+// Joins two (maximum, sum of exponentials) pairs; one without a finite or
+// infinite value has the maximum -infinity and the sum 0.
+__device__ __forceinline__ void join(float2& a, const float2 b) {
+  const float top = fmaxf(a.x, b.x), from = top == -INFINITY ? 0.0f : top;
+  a.y = a.y * expf(a.x - from) + b.y * expf(b.x - from);
+  a.x = top;
+}
+
+// Per row: the strips' pairs joined (32 rows per block; a warp takes every
+// 32nd strip, then the warps' pairs are joined in order), the row's loss, and
+// (maximum, 1 / sum) for the gradient; 1 / sum is 0 for an ignored row.
+__global__ void __launch_bounds__(1024) strip_join_kernel(const float2* __restrict__ strips, int64_t strip_rows, int n,
+                                                          const int32_t* __restrict__ labels, int64_t rows, int64_t V,
+                                                          int32_t ignore, const float* __restrict__ picked,
+                                                          float2* __restrict__ stat, float* __restrict__ row_loss) {
+  __shared__ float2 ws[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t m = (int64_t)blockIdx.x * 32 + lane;
+  float2 a = make_float2(-INFINITY, 0.0f);
+  if (m < rows) {
+#pragma unroll 4
+    for (int i = warp; i < n; i += 32) join(a, strips[(int64_t)i * strip_rows + m]);
+  }
+  ws[warp][lane] = a;
+  __syncthreads();
+  if (warp == 0 && m < rows) {
+    for (int i = 1; i < 32; i++) join(a, ws[i][lane]);
+    const int32_t y = labels[m];
+    const bool kept = y != ignore;
+    stat[m] = kept ? make_float2(a.x, __fdiv_rn(1.0f, a.y)) : make_float2(0.0f, 0.0f);
+    row_loss[m] = !kept ? 0.0f : y < 0 || y >= V ? NAN : logf(a.y) + (a.x - picked[m]);
+  }
+}
+
+// n G = exp(z - maximum) / sum - [label] for 32 rows of 1024 columns (4 per
+// thread), as two float16 planes of n G 2^15 and, for db, summed over the rows.
+constexpr int kGradCols = 1024;
+template <bool DB>
+__global__ void __launch_bounds__(256) grad_planes_kernel(const float* __restrict__ z, const float2* __restrict__ stat,
+                                                          const int32_t* __restrict__ labels, int64_t rows, int64_t V,
+                                                          int64_t Vp, int across, __half* __restrict__ g,
+                                                          int64_t plane, float* __restrict__ part) {
+  __shared__ float2 st[32];
+  __shared__ int32_t ys[32];
+  const int64_t rb = blockIdx.x / across, cb = blockIdx.x - rb * across;
+  const int64_t m0 = rb * 32, c = cb * kGradCols + 4 * threadIdx.x;
+  const int n = (int)min((int64_t)32, rows - m0);
+  if (threadIdx.x < n) st[threadIdx.x] = stat[m0 + threadIdx.x], ys[threadIdx.x] = labels[m0 + threadIdx.x];
+  __syncthreads();
+  if (c >= V) return;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = 0; i < n; i++) {
+    const float4 v = *reinterpret_cast<const float4*>(z + (m0 + i) * Vp + c);
+    const float2 s = st[i];
+    const int64_t at = (int64_t)ys[i] - c;
+    float p[4] = {v.x, v.y, v.z, v.w};
+    __align__(8) __half hi[4], lo[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      p[j] = s.y == 0.0f ? 0.0f : expf(p[j] - s.x) * s.y - (at == j ? 1.0f : 0.0f);
+      if (DB) sum[j] += p[j];
+      split_half(p[j] * (float)(1 << kGradExponent), hi[j], lo[j]);
+    }
+    __half* o = g + (m0 + i) * Vp + c;
+    *reinterpret_cast<uint2*>(o) = *reinterpret_cast<uint2*>(hi);
+    *reinterpret_cast<uint2*>(o + plane) = *reinterpret_cast<uint2*>(lo);
+  }
+  if (DB) {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (c + j < V) part[rb * V + c + j] = sum[j];
+  }
+}
+
+// db (+)= the column sums of the blocks of 32 rows, in order, / n.
+__global__ void __launch_bounds__(64) db_kernel(const float* __restrict__ part, int64_t blocks, int64_t V,
+                                                const XentMeta* __restrict__ meta, bool first, float* __restrict__ db) {
+  const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x;
+  if (c >= V) return;
+  double acc = 0.0;
+#pragma unroll 8
+  for (int64_t i = 0; i < blocks; i++) acc += (double)part[i * V + c];
+  const float d = (float)(meta->count ? acc / (double)meta->count : 0.0);
+  db[c] = first ? d : db[c] + d;
+}
+
+// The pointers of one workspace block.
+struct Carver {
+  char* base;
+  int64_t used = 0;
+  template <typename U>
+  U* take(int64_t n) {
+    U* p = base ? (U*)(base + used) : nullptr;
+    used += ceil_div(n * (int64_t)sizeof(U), 256) * 256;
+    return p;
+  }
+};
+
+// float32: see the top of the file.
+static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
   const bool grad = c.dx || c.dw || c.db;
-  int64_t R = std::max<int64_t>(1, c.workspace / (int64_t)(c.V * sizeof(T)));
+  const int64_t Kp = ceil_div(c.K, 8) * 8, Vp = ceil_div(c.V, 8) * 8, strips = ceil_div(c.V, kStripCols);
+  // Rows per piece: as many as the workspace holds (z and the two planes of G
+  // take 8 bytes per logit, the strips 8 per 128), in multiples of the tiles'
+  // 256 rows, and the pieces of equal size.
+  const int64_t per_row = (grad ? 8 * Vp : 0) + 8 * strips;
+  int64_t R = std::max<int64_t>(1, c.workspace / per_row / 256) * 256;
+  R = std::min(c.M, ceil_div(ceil_div(c.M, ceil_div(c.M, R)), 256) * 256);
+  const int64_t blocks32 = ceil_div(R, 32);
+  struct {
+    XentMeta* meta;
+    __half *x, *w, *g;
+    float *z, *rows, *picked, *part;
+    float2 *strips, *stat;
+  } ws;
+  auto carve = [&](Carver& k) {
+    ws.meta = k.take<XentMeta>(1);
+    ws.x = k.take<__half>(2 * c.M * Kp);
+    ws.w = k.take<__half>(2 * c.V * Kp);
+    ws.g = k.take<__half>(grad ? 2 * R * Vp : 0);
+    ws.z = k.take<float>(grad ? R * Vp : 0);
+    ws.rows = k.take<float>(c.rows ? 0 : c.M);
+    ws.picked = k.take<float>(R);
+    ws.part = k.take<float>(c.db ? blocks32 * c.V : 0);
+    ws.strips = k.take<float2>(strips * R);
+    ws.stat = k.take<float2>(R);
+  };
+  Carver size{nullptr};
+  carve(size);
+  GT_TRY(scratch(ctx, (size_t)size.used, &held[0]));
+  Carver at{(char*)held[0]};
+  carve(at);
+  float* rows = c.rows ? c.rows : ws.rows;
+
+  GT_CUDA(cudaMemsetAsync(ws.meta, 0, sizeof(XentMeta), ctx->stream));
+  const int wb = grid_for(ctx, c.V * c.K, 256, 16), xb = grid_for(ctx, c.M * c.K, 256, 16);
+  operand_top_kernel<<<wb + xb, 256, 0, ctx->stream>>>(c.x, c.w, c.labels, c.M, c.K, c.V, c.ignore, wb, ws.meta,
+                                                        c.bad);
+  GT_LAUNCH_CHECK();
+  const int sb = (int)std::min<int64_t>(ceil_div(c.M + c.V, 8), (int64_t)ctx->sm_count * 32);
+  operand_split_kernel<<<sb, 256, 0, ctx->stream>>>(c.x, c.w, c.labels, c.M, c.K, c.V, Kp, c.ignore, ws.meta, ws.x,
+                                                     ws.w);
+  GT_LAUNCH_CHECK();
+  const HalfPlanes w{ws.w, c.V, c.K, Kp, c.V * Kp};
+  for (int64_t r0 = 0; r0 < c.M; r0 += R) {
+    const int64_t r = std::min(R, c.M - r0);
+    const HalfPlanes x{ws.x + r0 * Kp, r, c.K, Kp, c.M * Kp}, g{ws.g, r, c.V, Vp, R * Vp};
+    SplitGemm f;
+    f.M = r, f.N = c.V, f.K = c.K, f.a = x, f.b = w, f.scale = &ws.meta->logits;
+    f.out = grad ? ws.z : nullptr, f.ldc = Vp, f.bias = c.bias, f.labels = c.labels + r0;
+    f.strips = ws.strips, f.strip_rows = R, f.picked = ws.picked;
+    GT_TRY(split_gemm(ctx, f));
+    strip_join_kernel<<<(unsigned)ceil_div(r, 32), 1024, 0, ctx->stream>>>(
+        ws.strips, R, (int)strips, c.labels + r0, r, c.V, c.ignore, ws.picked, ws.stat, rows + r0);
+    GT_LAUNCH_CHECK();
+    if (!grad) continue;
+    const int64_t across = ceil_div(c.V, kGradCols), down = ceil_div(r, 32);
+    if (c.db)
+      grad_planes_kernel<true><<<(unsigned)(across * down), 256, 0, ctx->stream>>>(
+          ws.z, ws.stat, c.labels + r0, r, c.V, Vp, (int)across, ws.g, R * Vp, ws.part);
+    else
+      grad_planes_kernel<false><<<(unsigned)(across * down), 256, 0, ctx->stream>>>(
+          ws.z, ws.stat, c.labels + r0, r, c.V, Vp, (int)across, ws.g, R * Vp, nullptr);
+    GT_LAUNCH_CHECK();
+    if (c.dx) {
+      SplitGemm d;
+      d.M = r, d.N = c.K, d.K = c.V, d.a = g, d.b = w, d.b_mn = true, d.scale = &ws.meta->dx;
+      d.out = c.dx + r0 * c.K, d.ldc = c.K;
+      GT_TRY(split_gemm(ctx, d));
+    }
+    if (c.dw) {
+      SplitGemm d;
+      d.M = c.V, d.N = c.K, d.K = r, d.a = g, d.a_mn = true, d.b = x, d.b_mn = true, d.scale = &ws.meta->dw;
+      d.out = c.dw, d.ldc = c.K, d.accumulate = r0 > 0;
+      GT_TRY(split_gemm(ctx, d));
+    }
+    if (c.db) {
+      db_kernel<<<(unsigned)ceil_div(c.V, 64), 64, 0, ctx->stream>>>(ws.part, ceil_div(r, 32), c.V, ws.meta, r0 == 0,
+                                                                      c.db);
+      GT_LAUNCH_CHECK();
+    }
+  }
+  mean_rows_kernel<float><<<1, 1024, 0, ctx->stream>>>(rows, c.M, &ws.meta->count, c.loss);
+  GT_LAUNCH_CHECK();
+  return nullptr;
+}
+
+// float64: pieces of rows over the FP64 GEMM, one piece's logits in workspace.
+static char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
+  const bool grad = c.dx || c.dw || c.db;
+  int64_t R = std::max<int64_t>(1, c.workspace / (int64_t)(c.V * sizeof(double)));
   R = std::min(c.M, R >= 128 ? R / 128 * 128 : 128);
   const int64_t pieces = ceil_div(c.M, R);
-  T *z, *xk, *more = nullptr, *rows = c.rows;
+  double *z, *xk, *more = nullptr, *rows = c.rows;
   int64_t* counts;
-  GT_TRY(scratch(ctx, (size_t)R * c.V * sizeof(T), &held[0]));
-  GT_TRY(scratch(ctx, (size_t)R * c.K * sizeof(T), &held[1]));
+  GT_TRY(scratch(ctx, (size_t)R * c.V * sizeof(double), &held[0]));
+  GT_TRY(scratch(ctx, (size_t)R * c.K * sizeof(double), &held[1]));
   GT_TRY(scratch(ctx, 64, &held[2]));
   if (!rows) {
-    GT_TRY(scratch(ctx, (size_t)c.M * sizeof(T), &held[3]));
-    rows = (T*)held[3];
+    GT_TRY(scratch(ctx, (size_t)c.M * sizeof(double), &held[3]));
+    rows = (double*)held[3];
   }
   if (c.dw && pieces > 1) {
-    GT_TRY(scratch(ctx, (size_t)c.V * c.K * sizeof(T), &held[4]));
-    more = (T*)held[4];
+    GT_TRY(scratch(ctx, (size_t)c.V * c.K * sizeof(double), &held[4]));
+    more = (double*)held[4];
   }
-  z = (T*)held[0], xk = (T*)held[1], counts = (int64_t*)held[2];
+  z = (double*)held[0], xk = (double*)held[1], counts = (int64_t*)held[2];
   label_count_kernel<<<1, 1024, 0, ctx->stream>>>(c.labels, c.M, c.V, c.ignore, counts, c.bad);
   GT_LAUNCH_CHECK();
   for (int64_t r0 = 0; r0 < c.M; r0 += R) {
     const int64_t r = std::min(R, c.M - r0);
-    keep_rows_kernel<T><<<grid_for(ctx, r * c.K, 256), 256, 0, ctx->stream>>>(c.x + r0 * c.K, c.labels + r0, r, c.K,
+    keep_rows_kernel<<<grid_for(ctx, r * c.K, 256), 256, 0, ctx->stream>>>(c.x + r0 * c.K, c.labels + r0, r, c.K,
                                                                                c.ignore, xk);
     GT_LAUNCH_CHECK();
-    Epi<T> e;
+    Epi<double> e;
     e.out = z, e.ldc = c.V, e.bias = c.bias;
-    GT_TRY(product(ctx, GemmShape{r, c.V, c.K, false, true, c.K, c.K}, xk, c.w, e));
-    xent_piece_kernel<T><<<(unsigned)std::min<int64_t>(r, (int64_t)ctx->sm_count * 8), 256, 0, ctx->stream>>>(
+    GT_TRY(gemm<double>(ctx, GemmShape{r, c.V, c.K, false, true, c.K, c.K}, xk, c.w, e));
+    xent_piece_f64_kernel<<<(unsigned)std::min<int64_t>(r, (int64_t)ctx->sm_count * 8), 256, 0, ctx->stream>>>(
         z, c.labels + r0, r, c.V, c.ignore, counts, rows + r0, grad);
     GT_LAUNCH_CHECK();
     if (c.dx) {
-      Epi<T> d;
+      Epi<double> d;
       d.out = c.dx + r0 * c.K, d.ldc = c.K;
-      GT_TRY(product(ctx, GemmShape{r, c.K, c.V, false, false, c.V, c.K}, z, c.w, d));
+      GT_TRY(gemm<double>(ctx, GemmShape{r, c.K, c.V, false, false, c.V, c.K}, z, c.w, d));
     }
     if (c.dw) {
-      Epi<T> d;
+      Epi<double> d;
       d.out = r0 ? more : c.dw, d.ldc = c.K;
-      GT_TRY(product(ctx, GemmShape{c.V, c.K, r, true, false, c.V, c.K}, z, xk, d));
+      GT_TRY(gemm<double>(ctx, GemmShape{c.V, c.K, r, true, false, c.V, c.K}, z, xk, d));
       if (r0) {
-        add_kernel<T><<<grid_for(ctx, c.V * c.K, 256), 256, 0, ctx->stream>>>(c.dw, more, c.V * c.K);
+        add_kernel<<<grid_for(ctx, c.V * c.K, 256), 256, 0, ctx->stream>>>(c.dw, more, c.V * c.K);
         GT_LAUNCH_CHECK();
       }
     }
     if (c.db) {
-      piece_columns_kernel<T><<<grid_for(ctx, c.V, 64), 64, 0, ctx->stream>>>(z, r, c.V, r0 == 0, c.db);
+      piece_columns_kernel<<<grid_for(ctx, c.V, 64), 64, 0, ctx->stream>>>(z, r, c.V, r0 == 0, c.db);
       GT_LAUNCH_CHECK();
     }
   }
-  mean_rows_kernel<T><<<1, 1024, 0, ctx->stream>>>(rows, c.M, counts, c.loss);
+  mean_rows_kernel<double><<<1, 1024, 0, ctx->stream>>>(rows, c.M, counts, c.loss);
   GT_LAUNCH_CHECK();
   return nullptr;
 }
@@ -268,7 +567,7 @@ extern "C" char* gt_linear_xent_fwd_bwd(gt_ctx* ctx, int dtype, const void* x, c
   GT_DISPATCH(dtype, {
     const XentCall<T> c{(const T*)x, (const T*)w, (const T*)bias, labels, M, K, V, ignore_label, workspace_bytes,
                         (T*)loss, (T*)row_loss, (T*)dx, (T*)dw, (T*)db, bad_label};
-    err = linear_xent_pieces<T>(ctx, c, held);
+    err = linear_xent(ctx, c, held);
   });
   for (void* h : held) release(ctx, h);
   return err;

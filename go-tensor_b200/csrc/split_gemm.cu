@@ -1,0 +1,560 @@
+// tcgen05 GEMM of float32 operands held as two float16 planes, for sm_100a.
+//
+// Precision. x s = hi + lo with hi = half(x s), lo = half(x s - hi), s a power of
+// two that puts the operand's largest magnitude at 2^14: 22 bits of every
+// value down to 2^-18 of the largest, and nothing worse than 2^-40 of the
+// largest below that. A product is
+//   a b ~= hi(a) hi(b) + hi(a) lo(b) + lo(a) hi(b)          (lo lo dropped, 2^-22)
+// the same three products and the same mantissas as 3xTF32 (gemm_tc.cu), but
+// kind::f16 runs at twice the rate of kind::tf32 and a plane takes half the
+// bytes. The range that float16 lacks is in the scale, which the epilogue
+// undoes exactly. The operands arrive split (each is used by two GEMMs), so
+// no warp splits them here.
+// Tensor-core accumulation truncates, so, as there, the MMAs accumulate 256
+// values of K into one of two partial buffers in tensor memory and promoter
+// warps add each partial to a total in registers with rounded adds.
+//
+// Work split. A CTA pair (cta_group::2) computes 256 x 256 outputs: each CTA
+// stages 128 rows of A and of B, both planes, 32 values of K per stage (32
+// KB), six stages. Warp roles of the 12 warps: warp 0 TMA producer, warp 1 MMA
+// issuer (leader), warp 2 relays "my half of the stage has landed" to the
+// leader, warps 4-11 promoters and epilogue. Persistent over units (tiles, or
+// K-splits of tiles when the tiles do not fill the SM pairs).
+// The operand with more rows is walked in the outer loop, so that it is read
+// from HBM once while the other stays in L2.
+//
+// Every barrier wait is bounded, with the same exit as gemm_tc.cu's kernel.
+#include "split_gemm.cuh"
+
+#include <algorithm>
+#include <cmath>
+
+#include "tc_pipe.cuh"
+
+namespace gt {
+namespace tc {
+
+constexpr int SBM = 128;                         // rows of A and of B per CTA
+constexpr int SBK = 32;                          // K per stage
+constexpr int SSTAGES = 6;
+constexpr int SGROUP = 8;                        // stages per promotion (256 of K)
+constexpr int STHREADS = 384;
+constexpr uint32_t PLANE_BYTES = SBM * SBK * 2;  // one plane of one operand, 8 KB
+constexpr uint32_t OPER_BYTES = 2 * PLANE_BYTES;
+constexpr uint32_t SSTAGE_BYTES = 2 * OPER_BYTES;
+constexpr int SPROMOTERS = 8;                    // warps
+constexpr int STILE = 256;
+constexpr int SEPI_LD = 33;
+constexpr uint32_t SBAR_OFFSET = SSTAGES * SSTAGE_BYTES;
+constexpr uint32_t SEPI_OFFSET = SBAR_OFFSET + 512;
+constexpr uint32_t SSMEM_BYTES = SEPI_OFFSET + SPROMOTERS * 32 * SEPI_LD * 4 + 1024;
+static_assert(SSMEM_BYTES <= 232448, "shared memory budget");
+constexpr int64_t STILE_ELEMS = (int64_t)STILE * STILE;
+// The launch gives every thread 65536 / 384 = 170, rounded down to 168: 4
+// warps with 64 and 8 with 216 stay within 12 * 168.
+constexpr int SREGS_LOW = 64, SREGS_HIGH = 216;
+static_assert(128 * SREGS_LOW + 256 * SREGS_HIGH <= STHREADS * 168, "register split exceeds the launch's registers");
+
+struct SplitUnits {
+  int whole = 0, splits = 1;  // tiles computed whole; K-splits of the others
+  float* ws = nullptr;        // [splits][tiles - whole][256 * 256]
+  uint64_t wait_limit_ns = kTimeoutNs;
+  int withhold = 0;  // test hook: the peer's relay withholds its first arrival
+};
+
+struct SplitShared {
+  uint64_t full[SSTAGES];   // TMA -> local relay (and the leader's MMA)
+  uint64_t ready[SSTAGES];  // the peer's relay -> the leader's MMA
+  uint64_t empty[SSTAGES];  // MMA -> producers of both CTAs
+  uint64_t pfull[2], pempty[2];
+  uint64_t mma_done;
+  uint32_t tmem_base;
+  int failed;
+};
+
+struct SplitArgs {
+  int64_t M, N, K;
+  const SplitScale* scale;
+  float* out;
+  int64_t ldc;
+  int accumulate;
+  int m_fast;  // consecutive tiles share their columns of C, else their rows
+  const float* bias;
+  const int32_t* labels;
+  float2* strips;
+  int64_t strip_rows;
+  float* picked;
+};
+
+// Unit u: tile (mt, nt) over the stages [kb, ke); the split index or -1.
+__device__ __forceinline__ int split_unit(int u, int m_tiles, int n_tiles, int m_fast, const SplitUnits& su, int num_k,
+                                          int& t, int& mt, int& nt, int& kb, int& ke) {
+  const int tiles = m_tiles * n_tiles;
+  int sidx = -1;
+  t = u, kb = 0, ke = num_k;
+  if (u >= su.whole) {
+    const int rest = tiles - su.whole, v = u - su.whole;
+    sidx = v / rest;
+    t = su.whole + (v - sidx * rest);
+    kb = (int)((int64_t)sidx * num_k / su.splits);
+    ke = (int)((int64_t)(sidx + 1) * num_k / su.splits);
+  }
+  if (m_fast)
+    nt = t / m_tiles, mt = t - nt * m_tiles;
+  else
+    mt = t / n_tiles, nt = t - mt * n_tiles;
+  return sidx;
+}
+
+// Descriptors of an operand's first K step of 16 in stage 0's hi plane. K-major:
+// 64-byte rows, 64-byte swizzle, 8-row groups 512 bytes apart; a K step is +32
+// bytes, the lo plane + PLANE_BYTES. M/N-major: 128-byte rows of 64 values,
+// one per k, 128-byte swizzle, 8-k groups 1024 bytes apart; 64-value groups
+// (each its hi and lo planes, 4 KB both) 8 KB apart; a K step is + 2048 bytes,
+// the lo plane + 4 KB.
+template <bool MN>
+__device__ __forceinline__ uint64_t split_desc(uint32_t base) {
+  return MN ? smem_desc(base, 8192, 1024, 2) : smem_desc(base, 16, 512, 4);
+}
+template <bool MN>
+constexpr uint32_t kstep_units() { return (MN ? 2048 : 32) >> 4; }
+template <bool MN>
+constexpr uint32_t lo_units() { return (MN ? 4096 : PLANE_BYTES) >> 4; }
+
+// kind::f16, both operands float16, float32 accumulator, 256 x 256.
+template <bool A_MN, bool B_MN>
+__device__ __forceinline__ uint32_t split_idesc() {
+  return 1u << 4 | (A_MN ? 1u : 0u) << 15 | (B_MN ? 1u : 0u) << 16 | (uint32_t)(STILE >> 3) << 17 |
+         (uint32_t)(STILE >> 4) << 24;
+}
+
+__device__ __forceinline__ void mma_f16_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// One operand's stage: both planes. K-major: one box {32, 128, 2}; M/N-major:
+// a box {64, 32, 2} per 64 values.
+template <bool MN>
+__device__ __forceinline__ void split_load(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int k0) {
+  if (MN) {
+    tma_load_3d(dst, map, bar, row, k0, 0);
+    tma_load_3d(dst + PLANE_BYTES, map, bar, row + 64, k0, 0);
+  } else {
+    tma_load_3d(dst, map, bar, k0, row, 0);
+  }
+}
+
+template <int J>
+__device__ __forceinline__ void split_chunk(float* xpose, const float (&tot)[128], int lane) {
+#pragma unroll
+  for (int i = 0; i < 32; i++) xpose[lane * SEPI_LD + i] = tot[32 * J + i];
+}
+
+__device__ __forceinline__ float apply(const SplitScale& s, float v) {
+  return __fmul_rn(__fmul_rn(__fmul_rn(v, s.h1), s.h2), s.f);
+}
+
+template <bool A_MN, bool B_MN, bool LOGITS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
+    split_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const SplitArgs s,
+                      const SplitUnits su) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  SplitShared* sh = (SplitShared*)(smem + SBAR_OFFSET);
+  volatile int* failed = &sh->failed;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  const int num_k = (int)((s.K + SBK - 1) / SBK);
+  const int m_tiles = (int)((s.M + STILE - 1) / STILE), n_tiles = (int)((s.N + STILE - 1) / STILE);
+  const int tiles = m_tiles * n_tiles;
+  const int units = su.whole + (tiles - su.whole) * su.splits;
+  const int pair = (int)cluster_id(), pairs = (int)num_clusters();
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < SSTAGES; i++) {
+      mbar_init(&sh->full[i], 1);
+      mbar_init(&sh->ready[i], 1);
+      mbar_init(&sh->empty[i], 1);
+    }
+    for (int b = 0; b < 2; b++) {
+      mbar_init(&sh->pfull[b], 1);
+      mbar_init(&sh->pempty[b], 2 * SPROMOTERS);
+    }
+    mbar_init(&sh->mma_done, 1);
+    sh->failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem_base)),
+                 "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem_base;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SREGS_LOW));
+    if (warp == 0) {  // ---- TMA producer
+      const bool issuer = elect_one();
+      int it = 0, issued_to = 0;
+      for (int u = pair; u < units && !__shfl_sync(0xffffffffu, *failed, 0); u += pairs) {
+        int t, mt, nt, kb, ke;
+        split_unit(u, m_tiles, n_tiles, s.m_fast, su, num_k, t, mt, nt, kb, ke);
+        const int a_row = mt * STILE + (int)rank * SBM, b_row = nt * STILE + (int)rank * SBM;
+        for (int kt = kb; kt < ke; kt++, it++) {
+          const int st = it % SSTAGES;
+          if (!__all_sync(0xffffffffu, mbar_wait(&sh->empty[st], ((it / SSTAGES) & 1) ^ 1, 1, su.wait_limit_ns))) {
+            if (lane == 0) *failed = 1;
+            break;
+          }
+          if (issuer) {
+            uint64_t* bar = &sh->full[st];
+            uint8_t* stage = smem + st * SSTAGE_BYTES;
+            mbar_expect_tx(bar, SSTAGE_BYTES);
+            split_load<A_MN>(stage, &tmA, bar, a_row, kt * SBK);
+            split_load<B_MN>(stage + OPER_BYTES, &tmB, bar, b_row, kt * SBK);
+          }
+          __syncwarp();
+          issued_to = it + 1;
+        }
+      }
+      if (__shfl_sync(0xffffffffu, *failed, 0)) {  // let copies in flight land before the CTA tears down
+        for (int i = issued_to > SSTAGES ? issued_to - SSTAGES : 0; i < issued_to; i++)
+          mbar_wait(&sh->full[i % SSTAGES], (i / SSTAGES) & 1, 5, kTimeoutNs);
+      }
+    } else if (warp == 1) {
+      if (leader) {  // ---- MMA issuer
+        const bool issuer = elect_one();
+        const uint32_t idesc = split_idesc<A_MN, B_MN>();
+        const uint64_t adesc0 = split_desc<A_MN>(smem_u32(smem)), bdesc0 = split_desc<B_MN>(smem_u32(smem) + OPER_BYTES);
+        int it = 0, group = 0;
+        bool stop = false;
+        for (int u = pair; u < units && !stop; u += pairs) {
+          int t, mt, nt, kb, ke;
+          split_unit(u, m_tiles, n_tiles, s.m_fast, su, num_k, t, mt, nt, kb, ke);
+          for (int kt = kb; kt < ke; kt++, it++) {
+            const int st = it % SSTAGES;
+            const uint32_t phase = (it / SSTAGES) & 1;
+            const bool start = (kt - kb) % SGROUP == 0;
+            const uint32_t buf = (uint32_t)(group & 1);
+            bool ok = mbar_wait(&sh->full[st], phase, 3, su.wait_limit_ns);
+            ok = ok && mbar_wait(&sh->ready[st], phase, 4, su.wait_limit_ns);
+            if (start) ok = ok && mbar_wait(&sh->pempty[buf], ((group >> 1) & 1) ^ 1, 2, su.wait_limit_ns);
+            if (!__all_sync(0xffffffffu, ok)) {
+              stop = true;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t slot = (uint64_t)((st * SSTAGE_BYTES) >> 4);
+            const uint32_t d = tmem + buf * 256;
+            uint64_t ah[2], bh[2];
+#pragma unroll
+            for (int kk = 0; kk < 2; kk++) {
+              ah[kk] = adesc0 + slot + kk * kstep_units<A_MN>();
+              bh[kk] = bdesc0 + slot + kk * kstep_units<B_MN>();
+            }
+            if (issuer) {
+#pragma unroll
+              for (int kk = 0; kk < 2; kk++) {
+                mma_f16_pair(d, ah[kk] + lo_units<A_MN>(), bh[kk], idesc, start && kk == 0 ? 0u : 1u);
+                mma_f16_pair(d, ah[kk], bh[kk] + lo_units<B_MN>(), idesc, 1u);
+                mma_f16_pair(d, ah[kk], bh[kk], idesc, 1u);
+              }
+              mma_commit_pair(&sh->empty[st]);
+            }
+            __syncwarp();
+            if ((kt - kb) % SGROUP == SGROUP - 1 || kt == ke - 1) {
+              if (issuer) mma_commit_pair(&sh->pfull[buf]);
+              __syncwarp();
+              group++;
+            }
+          }
+        }
+        if (stop && lane == 0) *failed = 1;
+        if (issuer)
+          asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                           smem_u32(&sh->mma_done))
+                       : "memory");
+        __syncwarp();
+        mbar_wait(&sh->mma_done, 0, 6, kTimeoutNs);
+      }
+    } else if (warp == 2 && !leader) {  // ---- the peer's half of each stage has landed
+      int it = 0;
+      bool stop = false;
+      for (int u = pair; u < units && !stop; u += pairs) {
+        int t, mt, nt, kb, ke;
+        split_unit(u, m_tiles, n_tiles, s.m_fast, su, num_k, t, mt, nt, kb, ke);
+        for (int kt = kb; kt < ke; kt++, it++) {
+          const int st = it % SSTAGES;
+          if (__shfl_sync(0xffffffffu, *failed, 0) ||
+              !__all_sync(0xffffffffu, mbar_wait(&sh->full[st], (it / SSTAGES) & 1, 8, su.wait_limit_ns))) {
+            if (lane == 0) *failed = 1;
+            stop = true;
+            break;
+          }
+          if (lane == 0 && !(su.withhold && it == 0)) mbar_arrive_rank(&sh->ready[st], 0);
+          __syncwarp();
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SREGS_HIGH));
+    // ---- promoters and epilogue: warp quarter q has TMEM lanes 32 q .. (its
+    // rows), half h the columns 128 h .. 128 h + 127.
+    const int q = warp & 3, h = (warp - 4) >> 2;
+    const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16) + 128 * h;
+    float* xpose = (float*)(smem + SEPI_OFFSET) + (warp - 4) * 32 * SEPI_LD;
+    const SplitScale sc = *s.scale;
+    int group = 0;
+    for (int u = pair; u < units && !__shfl_sync(0xffffffffu, *failed, 0); u += pairs) {
+      int t, mt, nt, kb, ke;
+      const int sidx = split_unit(u, m_tiles, n_tiles, s.m_fast, su, num_k, t, mt, nt, kb, ke);
+      const int groups = (ke - kb + SGROUP - 1) / SGROUP;
+      float tot[128];
+#pragma unroll
+      for (int i = 0; i < 128; i++) tot[i] = 0.0f;
+      bool ok = true;
+      for (int g = 0; g < groups; g++, group++) {
+        const uint32_t buf = (uint32_t)(group & 1);
+        if (!__all_sync(0xffffffffu, mbar_wait(&sh->pfull[buf], (group >> 1) & 1, 7, su.wait_limit_ns))) {
+          *failed = 1;
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          float p[32];
+          tmem_load32(lane_base + buf * 256 + 32 * j, p);
+#pragma unroll
+          for (int i = 0; i < 32; i++) tot[32 * j + i] = __fadd_rn(tot[32 * j + i], p[i]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_rank(&sh->pempty[buf], 0);
+      }
+      if (!ok) break;
+      const int64_t m0 = (int64_t)mt * STILE + rank * SBM + 32 * q, n0 = (int64_t)nt * STILE + 128 * h;
+      float* part = sidx < 0 ? nullptr
+                             : su.ws + ((int64_t)sidx * (tiles - su.whole) + (t - su.whole)) * STILE_ELEMS +
+                                   (int64_t)(rank * SBM + 32 * q) * STILE + 128 * h + lane;
+      const int rows = (int)(s.M - m0 < 32 ? (s.M - m0 > 0 ? s.M - m0 : 0) : 32);
+      float top = -INFINITY, sum = 0.0f;  // LOGITS: this lane's row over the strip
+      const int32_t label = LOGITS && lane < rows ? s.labels[m0 + lane] : -1;
+      // 32 x 32 blocks through the per-warp buffer (the switch keeps the
+      // register indices static in a loop that is not unrolled).
+#pragma unroll 1
+      for (int j = 0; j < 4; j++) {
+        switch (j) {
+          case 0: split_chunk<0>(xpose, tot, lane); break;
+          case 1: split_chunk<1>(xpose, tot, lane); break;
+          case 2: split_chunk<2>(xpose, tot, lane); break;
+          default: split_chunk<3>(xpose, tot, lane); break;
+        }
+        __syncwarp();
+        const int64_t nb = n0 + 32 * j;
+        if (part) {
+#pragma unroll 4
+          for (int r = 0; r < 32; r++) part[r * STILE + 32 * j] = xpose[r * SEPI_LD + lane];
+        } else if constexpr (LOGITS) {
+          const float my_bias = s.bias && nb + lane < s.N ? __ldg(s.bias + nb + lane) : 0.0f;
+          const int cols = (int)(s.N - nb < 32 ? (s.N - nb > 0 ? s.N - nb : 0) : 32);
+          float z[32], block_top = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 32; i++) {
+            z[i] = __fadd_rn(apply(sc, xpose[lane * SEPI_LD + i]), __shfl_sync(0xffffffffu, my_bias, i));
+            xpose[lane * SEPI_LD + i] = z[i];
+            if (i >= cols) z[i] = -INFINITY;
+            block_top = fmaxf(block_top, z[i]);
+          }
+          // the running maximum and sum; a maximum of -infinity sums to 0, a
+          // NaN (which fmaxf passes over) reaches the sum
+          const float up = fmaxf(top, block_top), from = up == -INFINITY ? 0.0f : up;
+          float add = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 32; i++) add += expf(z[i] - from);
+          sum = sum * expf(top - from) + add;
+          top = up;
+          const int64_t at = (int64_t)label - nb;
+          if (at >= 0 && at < cols) s.picked[m0 + lane] = xpose[lane * SEPI_LD + at];
+          __syncwarp();
+          if (s.out && lane < cols) {
+            float* o = s.out + m0 * s.ldc + nb + lane;
+#pragma unroll 8
+            for (int r = 0; r < rows; r++) o[(int64_t)r * s.ldc] = xpose[r * SEPI_LD + lane];
+          }
+        } else if (nb + lane < s.N) {
+          float* o = s.out + m0 * s.ldc + nb + lane;
+          if (s.accumulate) {
+#pragma unroll 8
+            for (int r = 0; r < rows; r++)
+              o[(int64_t)r * s.ldc] = __fadd_rn(o[(int64_t)r * s.ldc], apply(sc, xpose[r * SEPI_LD + lane]));
+          } else {
+#pragma unroll 8
+            for (int r = 0; r < rows; r++) o[(int64_t)r * s.ldc] = apply(sc, xpose[r * SEPI_LD + lane]);
+          }
+        }
+        __syncwarp();
+      }
+      if constexpr (LOGITS) {
+        if (!part && lane < rows && n0 < s.N)
+          s.strips[(n0 / kStripCols) * s.strip_rows + m0 + lane] = make_float2(top, sum);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncwarp();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
+// The split tiles: their partials added in split order, then the epilogue.
+__global__ void split_reduce_kernel(SplitUnits su, int m_tiles, int n_tiles, SplitArgs s) {
+  const int rest = m_tiles * n_tiles - su.whole;
+  const int64_t total = (int64_t)rest * STILE_ELEMS;
+  const SplitScale sc = *s.scale;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int r = (int)(i / STILE_ELEMS), e = (int)(i - (int64_t)r * STILE_ELEMS), t = su.whole + r;
+    const int mt = s.m_fast ? t % m_tiles : t / n_tiles, nt = s.m_fast ? t / m_tiles : t % n_tiles;
+    const int64_t m = (int64_t)mt * STILE + e / STILE, n = (int64_t)nt * STILE + e % STILE;
+    if (m >= s.M || n >= s.N) continue;
+    float acc = su.ws[i];
+    for (int k = 1; k < su.splits; k++) acc = __fadd_rn(acc, su.ws[(int64_t)k * total + i]);
+    float* o = s.out + m * s.ldc + n;
+    acc = apply(sc, acc);
+    *o = s.accumulate ? __fadd_rn(*o, acc) : acc;
+  }
+}
+
+static char* split_map(gt_ctx* ctx, CUtensorMap* map, const HalfPlanes& p, bool mn) {
+  auto encode = (EncodeTiledFn)ctx->encode_tiled;
+  if (!encode) return errorf("split_gemm: cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {(cuuint64_t)p.cols, (cuuint64_t)p.rows, 2};
+  cuuint64_t strides[2] = {(cuuint64_t)p.pitch * 2, (cuuint64_t)p.plane_elems * 2};
+  cuuint32_t box[3] = {mn ? 64u : (cuuint32_t)SBK, mn ? (cuuint32_t)SBK : (cuuint32_t)SBM, 2};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (void*)p.base, dims, strides, box, estr,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, mn ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return errorf("split_gemm: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return nullptr;
+}
+
+// K-splits: whole tiles, every tile split S ways, or only the tiles of the
+// last round, whichever the cost model finds cheapest. In units of a stage on
+// a pair (768 clocks of MMA, 0.42 us): rounds of (stages + a fixed overhead per
+// unit), plus the partials' trip through memory at about 5 TB/s.
+static SplitUnits split_plan(int64_t tiles, int64_t pairs, int64_t num_k) {
+  constexpr double kOverhead = 12.0;
+  SplitUnits best;
+  best.whole = (int)tiles;
+  auto rounds = [&](int64_t units) { return std::ceil((double)units / pairs); };
+  auto traffic = [&](int64_t t, int S) { return (S + 1) * (double)t * STILE_ELEMS * 4.0 / 5e6 / 0.42; };
+  const double base = rounds(tiles) * (num_k + kOverhead);
+  double cost = base;
+  for (int S = 2; S <= 64 && num_k / S >= 2 * SGROUP; S++) {
+    const double per = std::ceil((double)num_k / S) + kOverhead;
+    if ((double)S * tiles * STILE_ELEMS * 4 <= (double)(1 << 30)) {
+      const double c = rounds(tiles * S) * per + traffic(tiles, S);
+      if (c < cost) cost = c, best.whole = 0, best.splits = S;
+    }
+    const int64_t full = tiles / pairs * pairs, rest = tiles - full;
+    if (full > 0 && rest > 0 && rest * S <= pairs) {
+      const double c = (double)(tiles / pairs) * (num_k + kOverhead) + per + traffic(rest, S);
+      if (c < cost) cost = c, best.whole = (int)full, best.splits = S;
+    }
+  }
+  if (cost > 0.95 * base) best.whole = (int)tiles, best.splits = 1;
+  return best;
+}
+
+template <bool A_MN, bool B_MN, bool LOGITS>
+static char* split_launch(gt_ctx* ctx, const SplitGemm& g) {
+  auto kern = split_gemm_kernel<A_MN, B_MN, LOGITS>;
+  static bool configured[64] = {};
+  if (ctx->device < 0 || ctx->device >= 64 || !configured[ctx->device]) {
+    GT_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SSMEM_BYTES));
+    if (ctx->device >= 0 && ctx->device < 64) configured[ctx->device] = true;
+  }
+  CUtensorMap ta, tb;
+  GT_TRY(split_map(ctx, &ta, g.a, A_MN));
+  GT_TRY(split_map(ctx, &tb, g.b, B_MN));
+  const int64_t m_tiles = ceil_div(g.M, STILE), n_tiles = ceil_div(g.N, STILE), tiles = m_tiles * n_tiles;
+  if (tiles > INT32_MAX / 64) return errorf("split_gemm: too many tiles");
+  const int64_t free_sms = (int64_t)ctx->sm_count - ctx->gemm_sm_reserve, avail = free_sms >= 2 ? free_sms / 2 : 1;
+  SplitUnits su;
+  if (LOGITS)  // its epilogue needs whole rows of a tile
+    su.whole = (int)tiles;
+  else
+    su = split_plan(tiles, avail, ceil_div(g.K, SBK));
+  su.wait_limit_ns = tc_wait_limit_ns();
+  su.withhold = tc_take_withhold();
+  SplitArgs s{g.M, g.N, g.K, g.scale, g.out, g.ldc, g.accumulate, g.N > g.M, g.bias, g.labels, g.strips, g.strip_rows,
+              g.picked};
+  void* ws = nullptr;
+  if (su.splits > 1) {
+    GT_TRY(scratch(ctx, (size_t)su.splits * (tiles - su.whole) * STILE_ELEMS * sizeof(float), &ws));
+    su.ws = (float*)ws;
+  }
+  const int64_t units = su.whole + (tiles - su.whole) * su.splits;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * std::min(units, avail)), 1, 1);
+  cfg.blockDim = dim3(STHREADS, 1, 1);
+  cfg.dynamicSmemBytes = SSMEM_BYTES;
+  cfg.stream = ctx->stream;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tb, s, su);
+  count_launch();
+  if (e == cudaSuccess && su.splits > 1) {
+    split_reduce_kernel<<<grid_for(ctx, (tiles - su.whole) * STILE_ELEMS, 256), 256, 0, ctx->stream>>>(
+        su, (int)m_tiles, (int)n_tiles, s);
+    count_launch();
+  }
+  if (e == cudaSuccess) e = cudaGetLastError();
+  release(ctx, ws);
+  if (e != cudaSuccess) return cuda_error(e, "split_gemm launch", __FILE__, __LINE__);
+  return nullptr;
+}
+
+}  // namespace tc
+
+static bool g_split_used = false;
+
+char* split_gemm(gt_ctx* ctx, const SplitGemm& g) {
+  if (ctx->sm_count < 2) return errorf("split_gemm: needs a pair of SMs");
+  g_split_used = true;
+  if (g.strips) {
+    if (g.a_mn || g.b_mn) return errorf("split_gemm: the logits' operands are K-major");
+    return tc::split_launch<false, false, true>(ctx, g);
+  }
+  if (!g.a_mn && g.b_mn) return tc::split_launch<false, true, false>(ctx, g);
+  if (g.a_mn && g.b_mn) return tc::split_launch<true, true, false>(ctx, g);
+  return errorf("split_gemm: layout not built");
+}
+
+char* split_gemm_check_errors() {
+  if (!g_split_used) return nullptr;
+  int e = 0;
+  GT_CUDA(cudaMemcpyFromSymbol(&e, g_tc_error, sizeof e));
+  if (e) {
+    int zero = 0;
+    cudaMemcpyToSymbol(g_tc_error, &zero, sizeof zero);
+    return errorf("tcgen05 split GEMM: a pipeline wait timed out (site %d); results are invalid", e);
+  }
+  return nullptr;
+}
+
+}  // namespace gt

@@ -1,0 +1,59 @@
+// float32 products of operands kept as two halves (float16 planes): the GEMMs
+// of the large-vocabulary loss (linear_xent.cu).
+#pragma once
+#include <cuda_fp16.h>
+
+#include "gt_common.cuh"
+
+namespace gt {
+
+// A float32 matrix (rows x cols) as two float16 planes, hi = half(x s) and
+// lo = half(x s - hi) with s a power of two: base[plane * plane_elems + row *
+// pitch + col]. pitch and plane_elems are multiples of 8 and the base is
+// 16-byte aligned (TMA).
+struct HalfPlanes {
+  const __half* base = nullptr;
+  int64_t rows = 0, cols = 0, pitch = 0, plane_elems = 0;
+};
+
+// Three factors that an accumulator is multiplied by, in order: a power of
+// two in two halves (so that no step overflows when the result does not) and
+// one more.
+struct SplitScale {
+  float h1, h2, f;
+};
+
+// C (M x N) = A (M x K) B (K x N). A is stored with rows M and columns K, or
+// with rows K and columns M (a_mn); B with rows N and columns K, or with rows
+// K and columns N (b_mn).
+struct SplitGemm {
+  int64_t M = 0, N = 0, K = 0;
+  HalfPlanes a, b;
+  bool a_mn = false, b_mn = false;
+  const SplitScale* scale = nullptr;  // device
+  float* out = nullptr;               // row-major, pitch ldc; logits: may be NULL
+  int64_t ldc = 0;
+  bool accumulate = false;  // out += instead of out =
+  // The logits' epilogue (strips set): out = C + bias, and for every row and
+  // strip of kStripCols columns the maximum of C + bias and the sum of exp(. -
+  // maximum), at strips[strip * strip_rows + row]; the label's logit goes to
+  // picked[row].
+  const float* bias = nullptr;
+  const int32_t* labels = nullptr;
+  float2* strips = nullptr;
+  int64_t strip_rows = 0;
+  float* picked = nullptr;
+};
+
+constexpr int kStripCols = 128;
+
+char* split_gemm(gt_ctx* ctx, const SplitGemm& g);
+
+// Reports (and clears) a pipeline wait of split_gemm's kernel that ran out.
+char* split_gemm_check_errors();
+
+// The bounded waits' limit and the test hook of gt_debug_tc_withhold_arrive (taken once), gemm_tc.cu.
+uint64_t tc_wait_limit_ns();
+int tc_take_withhold();
+
+}  // namespace gt

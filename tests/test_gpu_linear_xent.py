@@ -383,6 +383,27 @@ def test_two_calls_in_a_row_without_waiting():
             assert np.array_equal(got[k], want[k]), k
 
 
+def test_timed_out_wait_returns_an_error_and_the_context_recovers():
+    """The bounded waits of the split GEMM: with the limit at 20 ms, the peer CTA of each pair withholds one arrival, so
+    the MMA issuer's wait runs out and the kernel returns; gt_sync reports it, and the next call is right."""
+    be = cuda_backend()
+    h = Head(*inputs(300, 90, 700, 23, 0), 0)
+    want = h.call().host()
+    be.Sync()
+    be.lib.gt_debug_set_tc_wait_limit_us(20000)
+    try:
+        be.lib.gt_debug_tc_withhold_arrive()
+        h.call()
+        with pytest.raises(GTError, match=r"split GEMM: a pipeline wait timed out \(site \d\)"):
+            be.Sync()
+        be.Sync()
+    finally:
+        be.lib.gt_debug_set_tc_wait_limit_us(0)
+    got = h.call().host()
+    for k in got:
+        assert np.array_equal(got[k], want[k]), k
+
+
 def test_storages_are_checked():
     h = Head(*inputs(8, 8, 8, 25, 0), 0)
     with pytest.raises(ValueError, match="elements"):
