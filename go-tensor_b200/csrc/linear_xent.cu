@@ -178,6 +178,10 @@ __device__ __forceinline__ uint32_t finite_bits(float v) {
   return b < 0x7f800000u ? b : 0u;
 }
 
+__device__ __forceinline__ uint32_t finite_bits4(float4 v) {
+  return max(max(finite_bits(v.x), finite_bits(v.y)), max(finite_bits(v.z), finite_bits(v.w)));
+}
+
 // The largest magnitudes of w (blocks 0 .. w_blocks - 1) and of the rows of x
 // that count (the other blocks, a warp per row), and those rows' number; a
 // label outside [0, V) sets *bad.
@@ -188,15 +192,17 @@ __global__ void __launch_bounds__(256) operand_top_kernel(const float* __restric
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t top = 0;
   if ((int)blockIdx.x < w_blocks) {
-    const int64_t n = V * K, n4 = ((uintptr_t)w & 15) == 0 ? n / 4 : 0, stride = (int64_t)w_blocks * 256;
-#pragma unroll 4
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += stride) {
-      const float4 v = reinterpret_cast<const float4*>(w)[i];
-      top = max(max(top, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
+    const int64_t n = V * K, stride = (int64_t)w_blocks * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t n4 = ((uintptr_t)w & 15) == 0 ? n / 4 : 0;
+    const float4* w4 = reinterpret_cast<const float4*>(w);
+    for (int64_t i = at; i < n4; i += 4 * stride) {  // four loads in flight
+      float4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) v[u] = i + u * stride < n4 ? w4[i + u * stride] : float4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < 4; u++) top = max(top, finite_bits4(v[u]));
     }
-#pragma unroll 4
-    for (int64_t i = n4 * 4 + (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride)
-      top = max(top, finite_bits(w[i]));
+    for (int64_t i = n4 * 4 + at; i < n; i += stride) top = max(top, finite_bits(w[i]));
   } else {
     int64_t kept = 0;
     for (int64_t m = (int64_t)(blockIdx.x - w_blocks) * 8 + warp; m < M; m += (int64_t)(gridDim.x - w_blocks) * 8) {
@@ -205,8 +211,17 @@ __global__ void __launch_bounds__(256) operand_top_kernel(const float* __restric
       kept++;
       if (lane == 0 && bad && (y < 0 || y >= V)) *bad = 1;
       const float* r = x + m * K;
+      const int64_t k4 = ((K & 3) | ((uintptr_t)x & 15)) == 0 ? K / 4 : 0;
+      for (int64_t k = lane; k < k4; k += 128) {
+        float4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+          v[u] = k + 32 * u < k4 ? reinterpret_cast<const float4*>(r)[k + 32 * u] : float4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < 4; u++) top = max(top, finite_bits4(v[u]));
+      }
 #pragma unroll 4
-      for (int64_t k = lane; k < K; k += 32) top = max(top, finite_bits(r[k]));
+      for (int64_t k = 4 * k4 + lane; k < K; k += 32) top = max(top, finite_bits(r[k]));
     }
     if (lane == 0 && kept) atomicAdd((unsigned long long*)&meta->count, (unsigned long long)kept);
   }
@@ -223,11 +238,12 @@ __device__ __forceinline__ int plane_exponent(uint32_t top) {
   return 14 - (top < 0x800000u ? 31 - __clz((int)top) - 149 : (int)(top >> 23) - 127);
 }
 
-// 2^-e and a factor f, the power in two halves (beyond 2^-252 nothing is left
-// of an accumulator anyway).
+// 2^-e times f (at most 1), as one factor, or as two halves of the power where one
+// would not be a normal number (beyond 2^-252 nothing is left of an accumulator anyway).
 __device__ __forceinline__ SplitScale undo(int e, float f) {
   e = min(e, 252);
-  return {exp2_int(-e / 2), exp2_int(-e - (-e / 2)), f};
+  if (e >= -126 && e <= 64) return {__fmul_rn(exp2_int(-e), f), 1.0f};
+  return {exp2_int(-e / 2), __fmul_rn(exp2_int(-e - (-e / 2)), f)};
 }
 
 __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
@@ -250,7 +266,7 @@ __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restr
     meta->logits = undo(ex + ew, 1.0f);
     meta->dx = undo(ew + kGradExponent, inv);
     meta->dw = undo(ex + kGradExponent, inv);
-    if (meta->count == 0) meta->dx.f = meta->dw.f = 0.0f;  // no row counts: the gradients are 0
+    if (meta->count == 0) meta->dx.c1 = meta->dw.c1 = meta->dx.c2 = meta->dw.c2 = 0.0f;  // no row counts: the gradients are 0
   }
   for (int64_t i = (int64_t)blockIdx.x * 8 + warp; i < M + V; i += (int64_t)gridDim.x * 8) {
     const bool is_x = i >= V;
@@ -354,14 +370,22 @@ __global__ void __launch_bounds__(256) grad_planes_kernel(const float* __restric
   }
 }
 
-// db (+)= the column sums of the blocks of 32 rows, in order, / n.
-__global__ void __launch_bounds__(64) db_kernel(const float* __restrict__ part, int64_t blocks, int64_t V,
-                                                const XentMeta* __restrict__ meta, bool first, float* __restrict__ db) {
-  const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  if (c >= V) return;
+// db (+)= the column sums of the blocks of 32 rows, / n: 32 columns per block,
+// warp w adds the rows w, w + 8, ... in order, then the warps' sums in order.
+__global__ void __launch_bounds__(256) db_kernel(const float* __restrict__ part, int64_t blocks, int64_t V,
+                                                 const XentMeta* __restrict__ meta, bool first, float* __restrict__ db) {
+  __shared__ double ws[8][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   double acc = 0.0;
+  if (c < V) {
 #pragma unroll 8
-  for (int64_t i = 0; i < blocks; i++) acc += (double)part[i * V + c];
+    for (int64_t i = warp; i < blocks; i += 8) acc += (double)part[i * V + c];
+  }
+  ws[warp][lane] = acc;
+  __syncthreads();
+  if (warp != 0 || c >= V) return;
+  for (int i = 1; i < 8; i++) acc += ws[i][lane];
   const float d = (float)(meta->count ? acc / (double)meta->count : 0.0);
   db[c] = first ? d : db[c] + d;
 }
@@ -457,7 +481,7 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
       GT_TRY(split_gemm(ctx, d));
     }
     if (c.db) {
-      db_kernel<<<(unsigned)ceil_div(c.V, 64), 64, 0, ctx->stream>>>(ws.part, ceil_div(r, 32), c.V, ws.meta, r0 == 0,
+      db_kernel<<<(unsigned)ceil_div(c.V, 32), 256, 0, ctx->stream>>>(ws.part, ceil_div(r, 32), c.V, ws.meta, r0 == 0,
                                                                       c.db);
       GT_LAUNCH_CHECK();
     }

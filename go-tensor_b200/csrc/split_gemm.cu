@@ -11,7 +11,7 @@
 // undoes exactly. The operands arrive split (each is used by two GEMMs), so
 // no warp splits them here.
 // Tensor-core accumulation truncates, so, as there, the MMAs accumulate 256
-// values of K into one of two partial buffers in tensor memory and promoter
+// (or 128) values of K into one of two partial buffers in tensor memory and promoter
 // warps add each partial to a total in registers with rounded adds.
 //
 // Work split. A CTA pair (cta_group::2) computes 256 x 256 outputs: each CTA
@@ -37,17 +37,25 @@ namespace tc {
 constexpr int SBM = 128;                         // rows of A and of B per CTA
 constexpr int SBK = 32;                          // K per stage
 constexpr int SSTAGES = 6;
-constexpr int SGROUP = 8;                        // stages per promotion (256 of K)
+// Stages per promotion. The sum of a partial is truncated at every MMA, by up
+// to 2^-23 of what it holds by then, so short groups are more exact and long
+// ones leave the epilogue more time under the next tile's first two groups.
+// dx, whose rows of G hold one value near -1 among small ones, takes 128 of K
+// (its error at V = 517: 0.6e-6 of the result against 1.3e-6 with 256), which
+// its long K and few epilogues hide (277 us either way at 2048 x 1024 x
+// 32000); the logits and dw take 256 (284 us against 318, 260 against 276).
+template <bool A_MN, bool LOGITS>
+constexpr int group_stages() { return A_MN || LOGITS ? 8 : 4; }
+constexpr int SGROUP_MAX = 8;
 constexpr int STHREADS = 384;
 constexpr uint32_t PLANE_BYTES = SBM * SBK * 2;  // one plane of one operand, 8 KB
 constexpr uint32_t OPER_BYTES = 2 * PLANE_BYTES;
 constexpr uint32_t SSTAGE_BYTES = 2 * OPER_BYTES;
 constexpr int SPROMOTERS = 8;                    // warps
 constexpr int STILE = 256;
-constexpr int SEPI_LD = 33;
 constexpr uint32_t SBAR_OFFSET = SSTAGES * SSTAGE_BYTES;
 constexpr uint32_t SEPI_OFFSET = SBAR_OFFSET + 512;
-constexpr uint32_t SSMEM_BYTES = SEPI_OFFSET + SPROMOTERS * 32 * SEPI_LD * 4 + 1024;
+constexpr uint32_t SSMEM_BYTES = SEPI_OFFSET + SPROMOTERS * 32 * 32 * 4 + 1024;
 static_assert(SSMEM_BYTES <= 232448, "shared memory budget");
 constexpr int64_t STILE_ELEMS = (int64_t)STILE * STILE;
 // The launch gives every thread 65536 / 384 = 170, rounded down to 168: 4
@@ -78,6 +86,7 @@ struct SplitArgs {
   float* out;
   int64_t ldc;
   int accumulate;
+  int vec;     // out's rows are 16-byte aligned
   int m_fast;  // consecutive tiles share their columns of C, else their rows
   const float* bias;
   const int32_t* labels;
@@ -150,14 +159,52 @@ __device__ __forceinline__ void split_load(uint8_t* dst, const CUtensorMap* map,
   }
 }
 
+// The promoters' 32-column chunk J of the running total.
 template <int J>
-__device__ __forceinline__ void split_chunk(float* xpose, const float (&tot)[128], int lane) {
+__device__ __forceinline__ void split_chunk(float (&z)[32], const float (&tot)[128]) {
 #pragma unroll
-  for (int i = 0; i < 32; i++) xpose[lane * SEPI_LD + i] = tot[32 * J + i];
+  for (int i = 0; i < 32; i++) z[i] = tot[32 * J + i];
 }
 
-__device__ __forceinline__ float apply(const SplitScale& s, float v) {
-  return __fmul_rn(__fmul_rn(__fmul_rn(v, s.h1), s.h2), s.f);
+// A 32 x 32 block in a warp's transpose buffer: 16-byte chunk c of row r at
+// chunk c ^ (r % 8), so that 8 rows' same chunk and one row's 8 chunks are both
+// free of bank conflicts.
+__device__ __forceinline__ float4* block_chunk(float* xpose, int r, int c) {
+  return reinterpret_cast<float4*>(xpose) + r * 8 + (c ^ (r & 7));
+}
+__device__ __forceinline__ float& block_at(float* xpose, int r, int c) {
+  return xpose[r * 32 + ((((c >> 2) ^ (r & 7)) << 2) | (c & 3))];
+}
+
+__device__ __forceinline__ float apply(const SplitScale& s, float v) { return __fmul_rn(__fmul_rn(v, s.c1), s.c2); }
+
+// exp(d) for d <= 0 as the hardware's power of two: relative error about 2^-22
+// and 2^-24 |d| of the rounded exponent.
+__device__ __forceinline__ float exp_below(float d) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.4426950408889634f));
+  return r;
+}
+
+// tcgen05.ld of 32 columns without waiting, and the wait for all loads before.
+__device__ __forceinline__ void tmem_issue32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// The registers pass through the wait, so nothing reads them before it.
+__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
 template <bool A_MN, bool B_MN, bool LOGITS>
@@ -167,6 +214,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   SplitShared* sh = (SplitShared*)(smem + SBAR_OFFSET);
+  constexpr int SGROUP = group_stages<A_MN, LOGITS>();
   volatile int* failed = &sh->failed;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -314,7 +362,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
     // rows), half h the columns 128 h .. 128 h + 127.
     const int q = warp & 3, h = (warp - 4) >> 2;
     const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16) + 128 * h;
-    float* xpose = (float*)(smem + SEPI_OFFSET) + (warp - 4) * 32 * SEPI_LD;
+    float* xpose = (float*)(smem + SEPI_OFFSET) + (warp - 4) * 32 * 32;
     const SplitScale sc = *s.scale;
     int group = 0;
     for (int u = pair; u < units && !__shfl_sync(0xffffffffu, *failed, 0); u += pairs) {
@@ -333,12 +381,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
           break;
         }
         tc_fence_after();
+        {
+          uint32_t p[2][32];
+          tmem_issue32(lane_base + buf * 256, p[0]);
+          tmem_wait32(p[0]);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          float p[32];
-          tmem_load32(lane_base + buf * 256 + 32 * j, p);
+          for (int j = 0; j < 4; j++) {  // the next chunk's load runs under this one's adds
+            if (j < 3) tmem_issue32(lane_base + buf * 256 + 32 * (j + 1), p[(j + 1) & 1]);
 #pragma unroll
-          for (int i = 0; i < 32; i++) tot[32 * j + i] = __fadd_rn(tot[32 * j + i], p[i]);
+            for (int i = 0; i < 32; i++) tot[32 * j + i] = __fadd_rn(tot[32 * j + i], __uint_as_float(p[j & 1][i]));
+            if (j < 3) tmem_wait32(p[(j + 1) & 1]);
+          }
         }
         tc_fence_before();
         __syncwarp();
@@ -346,64 +399,105 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
       }
       if (!ok) break;
       const int64_t m0 = (int64_t)mt * STILE + rank * SBM + 32 * q, n0 = (int64_t)nt * STILE + 128 * h;
+      const int rows = (int)(s.M - m0 < 32 ? (s.M - m0 > 0 ? s.M - m0 : 0) : 32);
       float* part = sidx < 0 ? nullptr
                              : su.ws + ((int64_t)sidx * (tiles - su.whole) + (t - su.whole)) * STILE_ELEMS +
-                                   (int64_t)(rank * SBM + 32 * q) * STILE + 128 * h + lane;
-      const int rows = (int)(s.M - m0 < 32 ? (s.M - m0 > 0 ? s.M - m0 : 0) : 32);
+                                   (int64_t)(rank * SBM + 32 * q) * STILE + 128 * h;
+      float* dst = part ? part : s.out ? s.out + m0 * s.ldc + n0 : nullptr;
+      const int64_t ld = part ? STILE : s.ldc;
+      const bool vec = part || s.vec;
       float top = -INFINITY, sum = 0.0f;  // LOGITS: this lane's row over the strip
       const int32_t label = LOGITS && lane < rows ? s.labels[m0 + lane] : -1;
       // 32 x 32 blocks through the per-warp buffer (the switch keeps the
       // register indices static in a loop that is not unrolled).
 #pragma unroll 1
       for (int j = 0; j < 4; j++) {
+        float z[32];
         switch (j) {
-          case 0: split_chunk<0>(xpose, tot, lane); break;
-          case 1: split_chunk<1>(xpose, tot, lane); break;
-          case 2: split_chunk<2>(xpose, tot, lane); break;
-          default: split_chunk<3>(xpose, tot, lane); break;
+          case 0: split_chunk<0>(z, tot); break;
+          case 1: split_chunk<1>(z, tot); break;
+          case 2: split_chunk<2>(z, tot); break;
+          default: split_chunk<3>(z, tot); break;
         }
-        __syncwarp();
         const int64_t nb = n0 + 32 * j;
-        if (part) {
-#pragma unroll 4
-          for (int r = 0; r < 32; r++) part[r * STILE + 32 * j] = xpose[r * SEPI_LD + lane];
-        } else if constexpr (LOGITS) {
-          const float my_bias = s.bias && nb + lane < s.N ? __ldg(s.bias + nb + lane) : 0.0f;
-          const int cols = (int)(s.N - nb < 32 ? (s.N - nb > 0 ? s.N - nb : 0) : 32);
-          float z[32], block_top = -INFINITY;
+        const int cols = part ? 32 : (int)(s.N - nb < 32 ? (s.N - nb > 0 ? s.N - nb : 0) : 32);
+        if (!part) {
 #pragma unroll
-          for (int i = 0; i < 32; i++) {
-            z[i] = __fadd_rn(apply(sc, xpose[lane * SEPI_LD + i]), __shfl_sync(0xffffffffu, my_bias, i));
-            xpose[lane * SEPI_LD + i] = z[i];
-            if (i >= cols) z[i] = -INFINITY;
-            block_top = fmaxf(block_top, z[i]);
+          for (int i = 0; i < 32; i++) z[i] = apply(sc, z[i]);
+        }
+        if constexpr (LOGITS) {
+          if (s.bias) {
+            const float my_bias = lane < cols ? __ldg(s.bias + nb + lane) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 32; i++) z[i] = __fadd_rn(z[i], __shfl_sync(0xffffffffu, my_bias, i));
           }
+          if (cols < 32) {
+#pragma unroll
+            for (int i = 0; i < 32; i++) z[i] = i < cols ? z[i] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+          *block_chunk(xpose, lane, c) = make_float4(z[4 * c], z[4 * c + 1], z[4 * c + 2], z[4 * c + 3]);
+        __syncwarp();
+        if (dst) {
+          if (vec && cols == 32) {  // 4 rows x 128 bytes per access
+            const int r0 = lane >> 3, c = lane & 7;
+            float* o = dst + (int64_t)r0 * ld + 32 * j + 4 * c;
+            if (!LOGITS && s.accumulate && !part) {
+              // the old values of all rows before any is written: a load per
+              // row behind the store before it made the kernel three times as
+              // slow
+              float4 was[8];
+#pragma unroll
+              for (int k = 0; k < 8; k++)
+                was[k] = r0 + 4 * k < rows ? *reinterpret_cast<const float4*>(o + 4 * k * ld) : float4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int k = 0; k < 8; k++) {
+                const float4 v = *block_chunk(xpose, r0 + 4 * k, c);
+                if (r0 + 4 * k < rows)
+                  *reinterpret_cast<float4*>(o + 4 * k * ld) =
+                      make_float4(__fadd_rn(was[k].x, v.x), __fadd_rn(was[k].y, v.y), __fadd_rn(was[k].z, v.z),
+                                  __fadd_rn(was[k].w, v.w));
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 8; k++)
+                if (part || r0 + 4 * k < rows)
+                  *reinterpret_cast<float4*>(o + 4 * k * ld) = *block_chunk(xpose, r0 + 4 * k, c);
+            }
+          } else if (lane < cols) {
+            float* o = dst + 32 * j + lane;
+            if (!LOGITS && s.accumulate) {
+#pragma unroll 1
+              for (int r0 = 0; r0 < 32; r0 += 16) {
+                float was[16];
+#pragma unroll
+                for (int r = 0; r < 16; r++) was[r] = r0 + r < rows ? o[(r0 + r) * ld] : 0.0f;
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                  if (r0 + r < rows) o[(r0 + r) * ld] = __fadd_rn(was[r], block_at(xpose, r0 + r, lane));
+              }
+            } else {
+#pragma unroll 8
+              for (int r = 0; r < rows; r++) o[r * ld] = block_at(xpose, r, lane);
+            }
+          }
+        }
+        if constexpr (LOGITS) {
           // the running maximum and sum; a maximum of -infinity sums to 0, a
           // NaN (which fmaxf passes over) reaches the sum
-          const float up = fmaxf(top, block_top), from = up == -INFINITY ? 0.0f : up;
-          float add = 0.0f;
+          float block_top = z[0];
 #pragma unroll
-          for (int i = 0; i < 32; i++) add += expf(z[i] - from);
-          sum = sum * expf(top - from) + add;
+          for (int i = 1; i < 32; i++) block_top = fmaxf(block_top, z[i]);
+          const float up = fmaxf(top, block_top), from = up == -INFINITY ? 0.0f : up;
+          float add[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < 32; i++) add[i & 3] += exp_below(z[i] - from);
+          sum = sum * exp_below(top - from) + ((add[0] + add[1]) + (add[2] + add[3]));
           top = up;
           const int64_t at = (int64_t)label - nb;
-          if (at >= 0 && at < cols) s.picked[m0 + lane] = xpose[lane * SEPI_LD + at];
-          __syncwarp();
-          if (s.out && lane < cols) {
-            float* o = s.out + m0 * s.ldc + nb + lane;
-#pragma unroll 8
-            for (int r = 0; r < rows; r++) o[(int64_t)r * s.ldc] = xpose[r * SEPI_LD + lane];
-          }
-        } else if (nb + lane < s.N) {
-          float* o = s.out + m0 * s.ldc + nb + lane;
-          if (s.accumulate) {
-#pragma unroll 8
-            for (int r = 0; r < rows; r++)
-              o[(int64_t)r * s.ldc] = __fadd_rn(o[(int64_t)r * s.ldc], apply(sc, xpose[r * SEPI_LD + lane]));
-          } else {
-#pragma unroll 8
-            for (int r = 0; r < rows; r++) o[(int64_t)r * s.ldc] = apply(sc, xpose[r * SEPI_LD + lane]);
-          }
+          if (at >= 0 && at < cols) s.picked[m0 + lane] = block_at(xpose, lane, (int)at);
         }
         __syncwarp();
       }
@@ -466,7 +560,7 @@ static SplitUnits split_plan(int64_t tiles, int64_t pairs, int64_t num_k) {
   auto traffic = [&](int64_t t, int S) { return (S + 1) * (double)t * STILE_ELEMS * 4.0 / 5e6 / 0.42; };
   const double base = rounds(tiles) * (num_k + kOverhead);
   double cost = base;
-  for (int S = 2; S <= 64 && num_k / S >= 2 * SGROUP; S++) {
+  for (int S = 2; S <= 64 && num_k / S >= 2 * SGROUP_MAX; S++) {
     const double per = std::ceil((double)num_k / S) + kOverhead;
     if ((double)S * tiles * STILE_ELEMS * 4 <= (double)(1 << 30)) {
       const double c = rounds(tiles * S) * per + traffic(tiles, S);
@@ -503,7 +597,8 @@ static char* split_launch(gt_ctx* ctx, const SplitGemm& g) {
     su = split_plan(tiles, avail, ceil_div(g.K, SBK));
   su.wait_limit_ns = tc_wait_limit_ns();
   su.withhold = tc_take_withhold();
-  SplitArgs s{g.M, g.N, g.K, g.scale, g.out, g.ldc, g.accumulate, g.N > g.M, g.bias, g.labels, g.strips, g.strip_rows,
+  const int vec = (((uintptr_t)g.out & 15) | (g.ldc & 3)) == 0;
+  SplitArgs s{g.M, g.N, g.K, g.scale, g.out, g.ldc, g.accumulate, vec, g.N > g.M, g.bias, g.labels, g.strips, g.strip_rows,
               g.picked};
   void* ws = nullptr;
   if (su.splits > 1) {

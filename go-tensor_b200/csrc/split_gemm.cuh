@@ -16,11 +16,10 @@ struct HalfPlanes {
   int64_t rows = 0, cols = 0, pitch = 0, plane_elems = 0;
 };
 
-// Three factors that an accumulator is multiplied by, in order: a power of
-// two in two halves (so that no step overflows when the result does not) and
-// one more.
+// The two factors that an accumulator is multiplied by, in order: c2 is 1
+// unless one power of two cannot hold the scale.
 struct SplitScale {
-  float h1, h2, f;
+  float c1, c2;
 };
 
 // C (M x N) = A (M x K) B (K x N). A is stored with rows M and columns K, or
