@@ -29,6 +29,7 @@
 #include <cmath>
 
 #include "gemm.cuh"
+#include "linear_xent.cuh"
 #include "split_gemm.cuh"
 
 namespace gt {
@@ -154,16 +155,6 @@ __global__ void add_kernel(double* __restrict__ out, const double* __restrict__ 
     out[i] = out[i] + x[i];
 }
 
-template <typename T>
-struct XentCall {
-  const T *x, *w, *bias;
-  const int32_t* labels;
-  int64_t M, K, V;
-  int32_t ignore;
-  int64_t workspace;
-  T *loss, *rows, *dx, *dw, *db;
-  int32_t* bad;
-};
 
 // What the kernels of one float32 call share: the operands' largest finite
 // magnitudes (as ordered words), the rows that count, and the products' factors.
@@ -295,14 +286,6 @@ __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restr
   }
 }
 
-// Joins two (maximum, sum of exponentials) pairs; one without a finite or
-// infinite value has the maximum -infinity and the sum 0.
-__device__ __forceinline__ void join(float2& a, const float2 b) {
-  const float top = fmaxf(a.x, b.x), from = top == -INFINITY ? 0.0f : top;
-  a.y = a.y * expf(a.x - from) + b.y * expf(b.x - from);
-  a.x = top;
-}
-
 // Per row: the strips' pairs joined (32 rows per block; a warp takes every
 // 32nd strip, then the warps' pairs are joined in order), the row's loss, and
 // (maximum, 1 / sum) for the gradient; 1 / sum is 0 for an ignored row.
@@ -390,20 +373,9 @@ __global__ void __launch_bounds__(256) db_kernel(const float* __restrict__ part,
   db[c] = first ? d : db[c] + d;
 }
 
-// The pointers of one workspace block.
-struct Carver {
-  char* base;
-  int64_t used = 0;
-  template <typename U>
-  U* take(int64_t n) {
-    U* p = base ? (U*)(base + used) : nullptr;
-    used += ceil_div(n * (int64_t)sizeof(U), 256) * 256;
-    return p;
-  }
-};
-
 // float32: see the top of the file.
 static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
+  if (few_rows(c.M, c.K, c.V)) return linear_xent_few(ctx, c, held);
   const bool grad = c.dx || c.dw || c.db;
   const int64_t Kp = ceil_div(c.K, 8) * 8, Vp = ceil_div(c.V, 8) * 8, strips = ceil_div(c.V, kStripCols);
   // Rows per piece: as many as the workspace holds (z and the two planes of G

@@ -1,0 +1,53 @@
+// What the float32 paths of the large-vocabulary loss share.
+#pragma once
+#include "gt_common.cuh"
+
+namespace gt {
+
+// One call of gt_linear_xent_fwd_bwd (outputs that are not wanted are NULL).
+template <typename T>
+struct XentCall {
+  const T *x, *w, *bias;
+  const int32_t* labels;
+  int64_t M, K, V;
+  int32_t ignore;
+  int64_t workspace;
+  T *loss, *rows, *dx, *dw, *db;
+  int32_t* bad;
+};
+
+// The pointers of one workspace block.
+struct Carver {
+  char* base;
+  int64_t used = 0;
+  template <typename U>
+  U* take(int64_t n) {
+    U* p = base ? (U*)(base + used) : nullptr;
+    used += ceil_div(n * (int64_t)sizeof(U), 256) * 256;
+    return p;
+  }
+};
+
+// exp(d) for d <= 0 as the hardware's power of two: relative error about 2^-22
+// and 2^-24 |d| of the rounded exponent.
+__device__ __forceinline__ float exp_below(float d) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.4426950408889634f));
+  return r;
+}
+
+// Joins two (maximum, sum of exponentials) pairs; one without a finite or
+// infinite value has the maximum -infinity and the sum 0.
+__device__ __forceinline__ void join(float2& a, const float2 b) {
+  const float top = fmaxf(a.x, b.x), from = top == -INFINITY ? 0.0f : top;
+  a.y = a.y * expf(a.x - from) + b.y * expf(b.x - from);
+  a.x = top;
+}
+
+// Calls of few rows (linear_xent_few.cu, at most 64): all with at most 8 rows,
+// and those whose products stay below 2^27 terms, where the tensor-core path's
+// dozen launches and mostly empty tiles cost more.
+inline bool few_rows(int64_t M, int64_t K, int64_t V) { return M <= 8 || (M <= 64 && M * K * V <= (int64_t)1 << 27); }
+char* linear_xent_few(gt_ctx* ctx, const XentCall<float>& c, void** held);
+
+}  // namespace gt

@@ -29,6 +29,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "linear_xent.cuh"
 #include "tc_pipe.cuh"
 
 namespace gt {
@@ -177,14 +178,6 @@ __device__ __forceinline__ float& block_at(float* xpose, int r, int c) {
 }
 
 __device__ __forceinline__ float apply(const SplitScale& s, float v) { return __fmul_rn(__fmul_rn(v, s.c1), s.c2); }
-
-// exp(d) for d <= 0 as the hardware's power of two: relative error about 2^-22
-// and 2^-24 |d| of the rounded exponent.
-__device__ __forceinline__ float exp_below(float d) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.4426950408889634f));
-  return r;
-}
 
 // tcgen05.ld of 32 columns without waiting, and the wait for all loads before.
 __device__ __forceinline__ void tmem_issue32(uint32_t taddr, uint32_t (&r)[32]) {

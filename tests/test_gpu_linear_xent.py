@@ -169,7 +169,9 @@ def test_several_pieces(dt, M, K, V):
     compare(Head(x, w, b, y, dt, workspace_bytes=1).call().host(), *reference(x, w, b, y, dt))
 
 
-@pytest.mark.parametrize("M,K,V", [(2048, 300, 3001), (4100, 64, 1000), (600, 2048, 5003)])
+# (the last three: few rows on either side of the choice between the two float32 paths)
+@pytest.mark.parametrize("M,K,V", [(2048, 300, 3001), (4100, 64, 1000), (600, 2048, 5003), (40, 520, 8200),
+                                   (9, 1030, 14500), (64, 100, 20000)])
 def test_larger(M, K, V):
     x, w, b, y = inputs(M, K, V, 11, 0, ignored=0.1)
     compare(Head(x, w, b, y, 0).call().host(), *reference(x, w, b, y, 0))
