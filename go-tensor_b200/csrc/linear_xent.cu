@@ -126,6 +126,7 @@ __global__ void __launch_bounds__(256) xent_piece_f64_kernel(double* __restrict_
 template <typename T>
 __global__ void __launch_bounds__(1024) mean_rows_kernel(const T* __restrict__ rows, int64_t M,
                                                          const int64_t* __restrict__ counts, T* __restrict__ loss) {
+  after_predecessor();
   __shared__ double part[32];
   double acc = 0.0;
   for (int64_t i = threadIdx.x; i < M; i += blockDim.x) acc += (double)rows[i];
@@ -140,14 +141,23 @@ __global__ void __launch_bounds__(1024) mean_rows_kernel(const T* __restrict__ r
   }
 }
 
-// db (+)= column sums of a piece's gradient, rows in order.
-__global__ void piece_columns_kernel(const double* __restrict__ g, int64_t rows, int64_t V, bool first,
-                                     double* __restrict__ db) {
-  for (int64_t j = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; j < V; j += (int64_t)gridDim.x * blockDim.x) {
-    double acc = first ? 0.0 : db[j];
-    for (int64_t i = 0; i < rows; i++) acc += g[i * V + j];
-    db[j] = acc;
+// db (+)= column sums of a piece's gradient: 32 columns per block, warp w adds
+// the rows w, w + 32, ... in order, then the warps' sums in order.
+__global__ void __launch_bounds__(1024) piece_columns_kernel(const double* __restrict__ g, int64_t rows, int64_t V,
+                                                             bool first, double* __restrict__ db) {
+  __shared__ double ws[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  double acc = 0.0;
+  if (c < V) {
+#pragma unroll 4
+    for (int64_t i = warp; i < rows; i += 32) acc += g[i * V + c];
   }
+  ws[warp][lane] = acc;
+  __syncthreads();
+  if (warp != 0 || c >= V) return;
+  for (int i = 1; i < 32; i++) acc += ws[i][lane];
+  db[c] = first ? acc : db[c] + acc;
 }
 
 __global__ void add_kernel(double* __restrict__ out, const double* __restrict__ x, int64_t n) {
@@ -250,6 +260,7 @@ __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restr
                                                             const int32_t* __restrict__ labels, int64_t M, int64_t K,
                                                             int64_t V, int64_t Kp, int32_t ignore, XentMeta* meta,
                                                             __half* __restrict__ xp, __half* __restrict__ wp) {
+  after_predecessor();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ex = plane_exponent(meta->x_top), ew = plane_exponent(meta->w_top);
   if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -293,6 +304,7 @@ __global__ void __launch_bounds__(1024) strip_join_kernel(const float2* __restri
                                                           const int32_t* __restrict__ labels, int64_t rows, int64_t V,
                                                           int32_t ignore, const float* __restrict__ picked,
                                                           float2* __restrict__ stat, float* __restrict__ row_loss) {
+  after_predecessor();
   __shared__ float2 ws[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t m = (int64_t)blockIdx.x * 32 + lane;
@@ -312,19 +324,24 @@ __global__ void __launch_bounds__(1024) strip_join_kernel(const float2* __restri
   }
 }
 
-// n G = exp(z - maximum) / sum - [label] for 32 rows of 1024 columns (4 per
+// n G = exp(z - maximum) / sum - [label] for up to 32 rows of 1024 columns (4 per
 // thread), as two float16 planes of n G 2^15 and, for db, summed over the rows.
 constexpr int kGradCols = 1024;
+// Rows per block: 32, or 8 when that leaves SMs idle (15 us against 4 at 128 x 4000).
+static int grad_rows(const gt_ctx* ctx, int64_t rows, int64_t V) {
+  return ceil_div(rows, 32) * ceil_div(V, kGradCols) >= 2 * (int64_t)ctx->sm_count ? 32 : 8;
+}
 template <bool DB>
 __global__ void __launch_bounds__(256) grad_planes_kernel(const float* __restrict__ z, const float2* __restrict__ stat,
                                                           const int32_t* __restrict__ labels, int64_t rows, int64_t V,
-                                                          int64_t Vp, int across, __half* __restrict__ g,
+                                                          int64_t Vp, int across, int rpb, __half* __restrict__ g,
                                                           int64_t plane, float* __restrict__ part) {
+  after_predecessor();
   __shared__ float2 st[32];
   __shared__ int32_t ys[32];
   const int64_t rb = blockIdx.x / across, cb = blockIdx.x - rb * across;
-  const int64_t m0 = rb * 32, c = cb * kGradCols + 4 * threadIdx.x;
-  const int n = (int)min((int64_t)32, rows - m0);
+  const int64_t m0 = rb * rpb, c = cb * kGradCols + 4 * threadIdx.x;
+  const int n = (int)min((int64_t)rpb, rows - m0);
   if (threadIdx.x < n) st[threadIdx.x] = stat[m0 + threadIdx.x], ys[threadIdx.x] = labels[m0 + threadIdx.x];
   __syncthreads();
   if (c >= V) return;
@@ -353,10 +370,11 @@ __global__ void __launch_bounds__(256) grad_planes_kernel(const float* __restric
   }
 }
 
-// db (+)= the column sums of the blocks of 32 rows, / n: 32 columns per block,
+// db (+)= the column sums of the blocks of rows, / n: 32 columns per block,
 // warp w adds the rows w, w + 8, ... in order, then the warps' sums in order.
 __global__ void __launch_bounds__(256) db_kernel(const float* __restrict__ part, int64_t blocks, int64_t V,
                                                  const XentMeta* __restrict__ meta, bool first, float* __restrict__ db) {
+  after_predecessor();
   __shared__ double ws[8][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
@@ -384,7 +402,7 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
   const int64_t per_row = (grad ? 8 * Vp : 0) + 8 * strips;
   int64_t R = std::max<int64_t>(1, c.workspace / per_row / 256) * 256;
   R = std::min(c.M, ceil_div(ceil_div(c.M, ceil_div(c.M, R)), 256) * 256);
-  const int64_t blocks32 = ceil_div(R, 32);
+  const int64_t blocks = ceil_div(R, grad_rows(ctx, R, c.V));
   struct {
     XentMeta* meta;
     __half *x, *w, *g;
@@ -399,7 +417,7 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
     ws.z = k.take<float>(grad ? R * Vp : 0);
     ws.rows = k.take<float>(c.rows ? 0 : c.M);
     ws.picked = k.take<float>(R);
-    ws.part = k.take<float>(c.db ? blocks32 * c.V : 0);
+    ws.part = k.take<float>(c.db ? blocks * c.V : 0);
     ws.strips = k.take<float2>(strips * R);
     ws.stat = k.take<float2>(R);
   };
@@ -416,9 +434,8 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
                                                         c.bad);
   GT_LAUNCH_CHECK();
   const int sb = (int)std::min<int64_t>(ceil_div(c.M + c.V, 8), (int64_t)ctx->sm_count * 32);
-  operand_split_kernel<<<sb, 256, 0, ctx->stream>>>(c.x, c.w, c.labels, c.M, c.K, c.V, Kp, c.ignore, ws.meta, ws.x,
-                                                     ws.w);
-  GT_LAUNCH_CHECK();
+  GT_CUDA(launch_overlapped(ctx, operand_split_kernel, sb, 256, 0, c.x, c.w, c.labels, c.M, c.K, c.V, Kp, c.ignore,
+                            ws.meta, ws.x, ws.w));
   const HalfPlanes w{ws.w, c.V, c.K, Kp, c.V * Kp};
   for (int64_t r0 = 0; r0 < c.M; r0 += R) {
     const int64_t r = std::min(R, c.M - r0);
@@ -428,18 +445,15 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
     f.out = grad ? ws.z : nullptr, f.ldc = Vp, f.bias = c.bias, f.labels = c.labels + r0;
     f.strips = ws.strips, f.strip_rows = R, f.picked = ws.picked;
     GT_TRY(split_gemm(ctx, f));
-    strip_join_kernel<<<(unsigned)ceil_div(r, 32), 1024, 0, ctx->stream>>>(
-        ws.strips, R, (int)strips, c.labels + r0, r, c.V, c.ignore, ws.picked, ws.stat, rows + r0);
-    GT_LAUNCH_CHECK();
+    GT_CUDA(launch_overlapped(ctx, strip_join_kernel, (unsigned)ceil_div(r, 32), 1024, 0, ws.strips, R, (int)strips,
+                              c.labels + r0, r, c.V, c.ignore, ws.picked, ws.stat, rows + r0));
     if (!grad) continue;
-    const int64_t across = ceil_div(c.V, kGradCols), down = ceil_div(r, 32);
-    if (c.db)
-      grad_planes_kernel<true><<<(unsigned)(across * down), 256, 0, ctx->stream>>>(
-          ws.z, ws.stat, c.labels + r0, r, c.V, Vp, (int)across, ws.g, R * Vp, ws.part);
-    else
-      grad_planes_kernel<false><<<(unsigned)(across * down), 256, 0, ctx->stream>>>(
-          ws.z, ws.stat, c.labels + r0, r, c.V, Vp, (int)across, ws.g, R * Vp, nullptr);
-    GT_LAUNCH_CHECK();
+    const int64_t across = ceil_div(c.V, kGradCols);
+    const int rpb = grad_rows(ctx, r, c.V);
+    const int64_t down = ceil_div(r, rpb);
+    GT_CUDA(launch_overlapped(ctx, c.db ? grad_planes_kernel<true> : grad_planes_kernel<false>,
+                              (unsigned)(across * down), 256, 0, ws.z, ws.stat, c.labels + r0, r, c.V, Vp, (int)across,
+                              rpb, ws.g, R * Vp, ws.part));
     if (c.dx) {
       SplitGemm d;
       d.M = r, d.N = c.K, d.K = c.V, d.a = g, d.b = w, d.b_mn = true, d.scale = &ws.meta->dx;
@@ -453,13 +467,11 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
       GT_TRY(split_gemm(ctx, d));
     }
     if (c.db) {
-      db_kernel<<<(unsigned)ceil_div(c.V, 32), 256, 0, ctx->stream>>>(ws.part, ceil_div(r, 32), c.V, ws.meta, r0 == 0,
-                                                                      c.db);
-      GT_LAUNCH_CHECK();
+      GT_CUDA(launch_overlapped(ctx, db_kernel, (unsigned)ceil_div(c.V, 32), 256, 0, ws.part, down, c.V, ws.meta,
+                                r0 == 0, c.db));
     }
   }
-  mean_rows_kernel<float><<<1, 1024, 0, ctx->stream>>>(rows, c.M, &ws.meta->count, c.loss);
-  GT_LAUNCH_CHECK();
+  GT_CUDA(launch_overlapped(ctx, mean_rows_kernel<float>, 1, 1024, 0, rows, c.M, &ws.meta->count, c.loss));
   return nullptr;
 }
 
@@ -511,7 +523,7 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
       }
     }
     if (c.db) {
-      piece_columns_kernel<<<grid_for(ctx, c.V, 64), 64, 0, ctx->stream>>>(z, r, c.V, r0 == 0, c.db);
+      piece_columns_kernel<<<(unsigned)ceil_div(c.V, 32), 1024, 0, ctx->stream>>>(z, r, c.V, r0 == 0, c.db);
       GT_LAUNCH_CHECK();
     }
   }

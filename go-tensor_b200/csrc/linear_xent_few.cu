@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(1024) few_join_kernel(const float2* __restrict
                                                         const float* __restrict__ picked, float2* __restrict__ stat,
                                                         float* __restrict__ rows, float* __restrict__ loss,
                                                         FewMeta* __restrict__ meta, int32_t* bad) {
+  after_predecessor();
   constexpr int PARTS = MT >= 32 ? 1 : 32 / MT;
   __shared__ float2 pair[PARTS][MT];
   __shared__ float row_loss[MT];
@@ -203,6 +204,7 @@ __global__ void __launch_bounds__(256) few_grad_kernel(const float* __restrict__
                                                        int32_t ignore, int64_t per, const FewMeta* __restrict__ meta,
                                                        float* __restrict__ dw, float* __restrict__ db,
                                                        float* __restrict__ dx_part, int dw_vec) {
+  after_predecessor();
   constexpr int R = MT / 8;  // rows of dx per thread
   extern __shared__ __align__(16) uint8_t few_smem[];
   FewShared<MT>& sh = *reinterpret_cast<FewShared<MT>*>(few_smem);
@@ -311,6 +313,7 @@ __global__ void __launch_bounds__(256) few_grad_kernel(const float* __restrict__
 
 __global__ void __launch_bounds__(256) few_dx_kernel(const float* __restrict__ part, int runs, int64_t n,
                                                      const FewMeta* __restrict__ meta, float* __restrict__ dx) {
+  after_predecessor();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
   float s = part[i];
@@ -351,9 +354,8 @@ static char* few_run(gt_ctx* ctx, const XentCall<float>& c, void** held) {
                                                                      c.ignore, grad ? ws.z : nullptr, Vp, ws.strips,
                                                                      ws.picked);
   GT_LAUNCH_CHECK();
-  few_join_kernel<MT><<<1, 1024, 0, ctx->stream>>>(ws.strips, (int)strips, (int)c.M, c.labels, c.V, c.ignore,
-                                                   ws.picked, ws.stat, c.rows, c.loss, ws.meta, c.bad);
-  GT_LAUNCH_CHECK();
+  GT_CUDA(launch_overlapped(ctx, few_join_kernel<MT>, 1, 1024, 0, ws.strips, (int)strips, (int)c.M, c.labels, c.V,
+                            c.ignore, ws.picked, ws.stat, c.rows, c.loss, ws.meta, c.bad));
   if (!grad) return nullptr;
   static bool configured[64] = {};
   if (ctx->device < 0 || ctx->device >= 64 || !configured[ctx->device]) {
@@ -361,15 +363,12 @@ static char* few_run(gt_ctx* ctx, const XentCall<float>& c, void** held) {
                                  (int)sizeof(FewShared<MT>)));
     if (ctx->device >= 0 && ctx->device < 64) configured[ctx->device] = true;
   }
-  few_grad_kernel<MT><<<dim3((unsigned)kb, (unsigned)runs), 256, sizeof(FewShared<MT>), ctx->stream>>>(
-      c.x, c.w, ws.z, Vp, ws.stat, c.labels, (int)c.M, c.K, c.V, c.ignore, per, ws.meta, c.dw, c.db,
-      c.dx ? ws.part : nullptr, ((c.K & 3) | ((uintptr_t)c.dw & 15)) == 0);
-  GT_LAUNCH_CHECK();
-  if (c.dx) {
-    few_dx_kernel<<<(unsigned)ceil_div(c.M * c.K, 256), 256, 0, ctx->stream>>>(ws.part, (int)runs, c.M * c.K, ws.meta,
-                                                                               c.dx);
-    GT_LAUNCH_CHECK();
-  }
+  GT_CUDA(launch_overlapped(ctx, few_grad_kernel<MT>, dim3((unsigned)kb, (unsigned)runs), 256, sizeof(FewShared<MT>),
+                            c.x, c.w, ws.z, Vp, ws.stat, c.labels, (int)c.M, c.K, c.V, c.ignore, per, ws.meta, c.dw,
+                            c.db, c.dx ? ws.part : nullptr, ((c.K & 3) | ((uintptr_t)c.dw & 15)) == 0));
+  if (c.dx)
+    GT_CUDA(launch_overlapped(ctx, few_dx_kernel, (unsigned)ceil_div(c.M * c.K, 256), 256, 0, ws.part, (int)runs,
+                              c.M * c.K, ws.meta, c.dx));
   return nullptr;
 }
 

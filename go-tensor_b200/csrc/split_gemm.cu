@@ -220,6 +220,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
   const int pair = (int)cluster_id(), pairs = (int)num_clusters();
 
   if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmA)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmB)) : "memory");
     for (int i = 0; i < SSTAGES; i++) {
       mbar_init(&sh->full[i], 1);
       mbar_init(&sh->ready[i], 1);
@@ -243,6 +245,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
+  after_predecessor();
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SREGS_LOW));
@@ -511,6 +514,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
 
 // The split tiles: their partials added in split order, then the epilogue.
 __global__ void split_reduce_kernel(SplitUnits su, int m_tiles, int n_tiles, SplitArgs s) {
+  after_predecessor();
   const int rest = m_tiles * n_tiles - su.whole;
   const int64_t total = (int64_t)rest * STILE_ELEMS;
   const SplitScale sc = *s.scale;
@@ -599,18 +603,11 @@ static char* split_launch(gt_ctx* ctx, const SplitGemm& g) {
     su.ws = (float*)ws;
   }
   const int64_t units = su.whole + (tiles - su.whole) * su.splits;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(2 * std::min(units, avail)), 1, 1);
-  cfg.blockDim = dim3(STHREADS, 1, 1);
-  cfg.dynamicSmemBytes = SSMEM_BYTES;
-  cfg.stream = ctx->stream;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tb, s, su);
-  count_launch();
-  if (e == cudaSuccess && su.splits > 1) {
-    split_reduce_kernel<<<grid_for(ctx, (tiles - su.whole) * STILE_ELEMS, 256), 256, 0, ctx->stream>>>(
-        su, (int)m_tiles, (int)n_tiles, s);
-    count_launch();
-  }
+  cudaError_t e = launch_overlapped(ctx, kern, (unsigned)(2 * std::min(units, avail)), STHREADS, SSMEM_BYTES, ta, tb, s,
+                                    su);
+  if (e == cudaSuccess && su.splits > 1)
+    e = launch_overlapped(ctx, split_reduce_kernel, grid_for(ctx, (tiles - su.whole) * STILE_ELEMS, 256), 256, 0, su,
+                          (int)m_tiles, (int)n_tiles, s);
   if (e == cudaSuccess) e = cudaGetLastError();
   release(ctx, ws);
   if (e != cudaSuccess) return cuda_error(e, "split_gemm launch", __FILE__, __LINE__);
