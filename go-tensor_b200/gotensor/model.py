@@ -67,6 +67,7 @@ class Model:
         p = ctypes.c_void_p()
         check(self.lib.gth_model_new(self.ctx.ptr, dtype, arr, len(layers), shp, len(input_shape), ctypes.byref(p)))
         self.ptr = p
+        self._ignore = None  # the label of rows that the loss passes over (fused_head)
         self.params = []  # (name, shape, offset)
         for i in range(self.lib.gth_num_tensors(self.ptr)):
             name = ctypes.create_string_buffer(64)
@@ -145,6 +146,25 @@ class Model:
     def adam(self, lr=0.0, beta1=0.0, beta2=0.0, eps=0.0, weight_decay=0.0):
         check(self.lib.gth_set_adam(self.ptr, ctypes.byref(AdamCfg(lr, beta1, beta2, eps, weight_decay))))
 
+    def adamw(self, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, state=_lib.STATE_NATIVE,
+              max_norm=0.0, decay_vectors=False, seed=0):
+        """AdamW over all tensors in one launch; state STATE_E4M3 keeps the moments in 8 bits, max_norm > 0 clips the
+        gradients by their global norm, biases are decayed only with decay_vectors."""
+        check(self.lib.gth_set_adamw(self.ptr, ctypes.byref(AdamCfg(lr, beta1, beta2, eps, weight_decay)), state,
+                                     max_norm, int(decay_vectors), seed))
+
+    def grad_norm(self) -> float:
+        """The gradients' norm at the last clipped AdamW step."""
+        out = ctypes.c_double()
+        check(self.lib.gth_grad_norm(self.ptr, ctypes.byref(out)))
+        return out.value
+
+    def fused_head(self, on=True, ignore_label=-100):
+        """Trains the last Linear and the loss as one call that never keeps the logits; rows labelled ignore_label
+        take no part in the loss."""
+        check(self.lib.gth_set_fused_head(self.ptr, int(on), ignore_label))
+        self._ignore = ignore_label if on else None
+
     # -- data
     @property
     def input_device(self) -> int:
@@ -162,7 +182,8 @@ class Model:
         if y.shape != (self.input_shape[0],):
             raise ValueError("one label per row")
         ncls = self.classes
-        if y.size and (y.min() < 0 or y.max() >= ncls):
+        counted = y if self._ignore is None else y[y != self._ignore]
+        if counted.size and (counted.min() < 0 or counted.max() >= ncls):
             raise ValueError(f"label out of range for {ncls} classes")  # tensor/ops.go:352-354
         lib = self.ctx.lib
         check(lib.gt_upload(self.ctx.ptr, self.input_device, x.ctypes.data, x.nbytes))

@@ -92,6 +92,23 @@ GT_API char* gth_set_adam(gth_model* m, const gt_adam_cfg* cfg) {
   });
 }
 
+GT_API char* gth_set_adamw(gth_model* m, const gt_adam_cfg* cfg, int state, double max_norm, int decay_vectors,
+                           uint64_t seed) {
+  return guard([&] {
+    if (!cfg) throw Error("gth_set_adamw: null config");
+    m->m->set_adamw(*cfg, state, max_norm, decay_vectors != 0, seed);
+  });
+}
+GT_API char* gth_grad_norm(gth_model* m, double* out) {
+  return guard([&] {
+    if (!out) throw Error("gth_grad_norm: null output");
+    *out = m->m->grad_norm();
+  });
+}
+GT_API char* gth_set_fused_head(gth_model* m, int on, int32_t ignore_label) {
+  return guard([&] { m->m->set_fused_head(on != 0, ignore_label); });
+}
+
 GT_API void* gth_input_device(gth_model* m) { return m->m->input_device(); }
 GT_API int32_t* gth_labels_device(gth_model* m) { return m->m->labels_device(); }
 GT_API void* gth_loss_device(gth_model* m) { return m->m->loss_device(); }

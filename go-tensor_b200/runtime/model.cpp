@@ -71,6 +71,7 @@ Model::Model(gt_ctx* ctx, int dtype, const std::vector<gth_layer>& layers, const
 
 Model::~Model() {
   drop_graph();
+  free_adamw();
   gt_host_free(staging_);
   free_bucket_events();
   for (int p = 0; p < 2; p++) {
@@ -356,8 +357,14 @@ void Model::get_grads(void* host) {
     memcpy((char*)host + p.dense_offset * es_, tmp.data() + p.dev_offset * es_, p.numel * es_);
 }
 
+void Model::free_adamw() {
+  gt_free_error(gt_adamw_free(adamw_));
+  adamw_ = nullptr;
+}
+
 void Model::set_sgd(const gt_sgd_cfg& cfg) {
   drop_graph();
+  free_adamw();
   opt_ = OPT_SGD;
   sgd_ = cfg;
   opt_steps_ = 0;
@@ -368,6 +375,7 @@ void Model::set_sgd(const gt_sgd_cfg& cfg) {
 
 void Model::set_adam(const gt_adam_cfg& cfg) {
   drop_graph();
+  free_adamw();
   opt_ = OPT_ADAM;
   adam_ = cfg;
   opt_steps_ = 0;
@@ -378,11 +386,97 @@ void Model::set_adam(const gt_adam_cfg& cfg) {
   check(gt_zero(ctx_, step_dev_.get(), 64));
 }
 
+void Model::set_adamw(const gt_adam_cfg& cfg, int state, double max_norm, bool decay_vectors, uint64_t seed) {
+  if (state != GT_STATE_NATIVE && state != GT_STATE_E4M3) throw Error("gth_set_adamw: unknown state format");
+  if (state == GT_STATE_E4M3 && dtype_ != GT_FLOAT32) throw Error("gth_set_adamw: 8-bit states are for float32 only");
+  if (!(max_norm >= 0)) throw Error("gth_set_adamw: max_norm must be a number >= 0");
+  drop_graph();
+  free_adamw();
+  opt_ = OPT_NONE;  // until everything below has succeeded
+  const size_t held = state == GT_STATE_E4M3 ? 1 : es_;
+  int64_t blocks = 0;
+  for (auto& p : params_) blocks += (p.numel + 255) / 256;
+  opt_a_ = DevBuf(ctx_, dev_params_ * held);  // m
+  opt_b_ = DevBuf(ctx_, dev_params_ * held);  // v
+  opt_scales_ = DevBuf(ctx_, state == GT_STATE_E4M3 ? 2 * blocks * sizeof(float) : 16);
+  clip_ = DevBuf(ctx_, 2 * sizeof(double));
+  check(gt_zero(ctx_, opt_a_.get(), dev_params_ * held));
+  check(gt_zero(ctx_, opt_b_.get(), dev_params_ * held));
+  check(gt_zero(ctx_, opt_scales_.get(), opt_scales_.bytes()));
+  check(gt_zero(ctx_, clip_.get(), 2 * sizeof(double)));
+  check(gt_zero(ctx_, step_dev_.get(), 64));
+  std::vector<gt_adamw_tensor> ts;
+  int64_t block = 0;
+  for (auto& p : params_) {
+    gt_adamw_tensor t{};
+    t.p = (char*)pbuf_.get() + p.dev_offset * es_;
+    t.g = (char*)gbuf_.get() + p.dev_offset * es_;
+    t.m = (char*)opt_a_.get() + p.dev_offset * held;
+    t.v = (char*)opt_b_.get() + p.dev_offset * held;
+    if (state == GT_STATE_E4M3) {
+      t.m_scale = (float*)opt_scales_.get() + block;
+      t.v_scale = (float*)opt_scales_.get() + blocks + block;
+    }
+    t.n = p.numel;
+    t.lr_mul = 1.0;
+    t.wd_mul = p.shape.size() > 1 || decay_vectors ? 1.0 : 0.0;
+    block += (p.numel + 255) / 256;
+    ts.push_back(t);
+  }
+  check(gt_adamw_new(ctx_, dtype_, state, ts.data(), (int64_t)ts.size(), (int64_t*)step_dev_.get(), seed, &adamw_));
+  opt_ = OPT_ADAMW;
+  adam_ = cfg;
+  max_norm_ = max_norm;
+  opt_steps_ = 0;
+}
+
+double Model::grad_norm() {
+  if (opt_ != OPT_ADAMW || max_norm_ <= 0) throw Error("gth_grad_norm: needs AdamW with clipping (gth_set_adamw)");
+  double v[2] = {0, 0};
+  check(gt_download(ctx_, v, clip_.get(), sizeof v));
+  return v[0];
+}
+
+void Model::set_fused_head(bool on, int32_t ignore_label) {
+  Op& last = ops_.back();
+  if (on && (last.kind != Op::LINEAR || last.act != GT_ACT_NONE))
+    throw Error("gth_set_fused_head: the model must end in a Linear without an activation");
+  drop_graph();
+  ignore_label_ = ignore_label;
+  if (on == fused_head_) return;
+  // The gradient buffers of the backward pass, without the logits' gradient when it is never formed.
+  int64_t elems = 1;
+  for (size_t i = 0; i < ops_.size(); i++) {
+    if (!(on && i + 1 == ops_.size())) elems = std::max(elems, numel(ops_[i].out_shape));
+    elems = std::max(elems, numel(ops_[i].in_shape));
+  }
+  DevBuf a(ctx_, elems * es_), b(ctx_, elems * es_);
+  if (on) {
+    for (auto& buf : acts_)
+      if (buf.get() == last.out) buf.reset();
+    last.out = nullptr;
+  } else if (!last.out) {
+    logits_ = DevBuf(ctx_, (size_t)batch_ * classes_ * es_);
+    last.out = logits_.get();
+  }
+  grad_a_ = std::move(a);
+  grad_b_ = std::move(b);
+  grad_elems_ = elems;
+  fused_head_ = on;
+  // the Linear before the head: its bias gradient has no dX epilogue to come from
+  if (last.src >= 0 && ops_[last.src].kind == Op::LINEAR && last.needs_dx) ops_[last.src].db_upstream = !on;
+}
+
 // ---- step -------------------------------------------------------------------
 
-void Model::forward() {
+void Model::forward(bool train) {
   char* p = (char*)pbuf_.get();
+  if (fused_head_ && !train && !ops_.back().out) {  // an evaluation keeps the logits
+    logits_ = DevBuf(ctx_, (size_t)batch_ * classes_ * es_);
+    ops_.back().out = logits_.get();
+  }
   for (auto& op : ops_) {
+    if (fused_head_ && train && &op == &ops_.back()) break;  // with its loss, in backward()
     switch (op.kind) {
       case Op::LINEAR:
         if (op.bits)
@@ -439,14 +533,22 @@ void Model::backward(bool join) {
   // derivative of the activation that produced that output is already in it.
   void* g = grad_a_.get();
   void* spare = grad_b_.get();
-  if (ops_.back().db_upstream)  // the last Linear's bias gradient in the same pass
+  int top = (int)ops_.size() - 1;
+  if (fused_head_) {  // the last Linear, the loss and their gradients in one call
+    Op& op = ops_.back();
+    check(gt_linear_xent_fwd_bwd(ctx_, dtype_, op.in, p + op.w_off * es_, p + op.b_off * es_, labels_device(), op.M, op.K,
+                                 op.N, ignore_label_, 0, loss_.get(), nullptr, op.needs_dx ? g : nullptr,
+                                 gr + op.w_off * es_, gr + op.b_off * es_, nullptr));
+    top--;
+  } else if (ops_.back().db_upstream)  // the last Linear's bias gradient in the same pass
     check(gt_xent_fwd_bwd_db(ctx_, dtype_, ops_.back().out, labels_device(), batch_, classes_, loss_.get(), g,
                              gr + ops_.back().b_off * es_, nullptr));
   else
     check(gt_xent_fwd_bwd(ctx_, dtype_, ops_.back().out, labels_device(), batch_, classes_, loss_.get(), g, nullptr));
   bool g_pre = false;
   next_bucket_ = 0;
-  for (int i = (int)ops_.size() - 1; i >= first_param_op_; i--) {
+  if (fused_head_ && world_ > 1) issue_ready_buckets(ops_.back().w_off);
+  for (int i = top; i >= first_param_op_; i--) {
     Op& op = ops_[i];
     const bool has_act = (op.kind == Op::LINEAR || op.kind == Op::CONV || op.kind == Op::ACT) && op.act != GT_ACT_NONE;
     if (has_act && !g_pre) check(gt_act_bwd(ctx_, dtype_, op.act, g, op.out, g, numel(op.out_shape)));
@@ -547,13 +649,13 @@ void Model::backward(bool join) {
 
 void Model::forward_backward() {
   begin_read();
-  forward();
+  forward(true);
   backward();
   end_read();
 }
 
 void Model::optimizer_step() {
-  if (opt_ == OPT_NONE) throw Error("no optimizer: call gth_set_sgd or gth_set_adam");
+  if (opt_ == OPT_NONE) throw Error("no optimizer: call gth_set_sgd, gth_set_adam or gth_set_adamw");
   if (opt_ == OPT_SGD && world_ > 1 && !bucket_done_.empty()) {
     // Bucket by bucket, each as soon as its all-reduce is done: the updates of
     // the buckets averaged first overlap the all-reduce of the last ones.
@@ -571,6 +673,11 @@ void Model::optimizer_step() {
   } else if (opt_ == OPT_SGD) {
     if (world_ > 1) check(gt_comm_wait(ctx_));
     check(gt_sgd_step(ctx_, dtype_, pbuf_.get(), gbuf_.get(), opt_a_.get(), dev_params_, &sgd_, opt_steps_ == 0));
+  } else if (opt_ == OPT_ADAMW) {
+    if (world_ > 1) check(gt_comm_wait(ctx_));
+    double* clip = max_norm_ > 0 ? (double*)clip_.get() : nullptr;
+    if (clip) check(gt_adamw_clip(adamw_, max_norm_, clip));
+    check(gt_adamw_step(adamw_, &adam_, clip, nullptr));
   } else {
     if (world_ > 1) check(gt_comm_wait(ctx_));
     check(gt_adam_step_dev(ctx_, dtype_, pbuf_.get(), gbuf_.get(), opt_a_.get(), opt_b_.get(), dev_params_, &adam_,
@@ -580,7 +687,7 @@ void Model::optimizer_step() {
 }
 
 void Model::train_step() {
-  if (opt_ == OPT_NONE) throw Error("no optimizer: call gth_set_sgd or gth_set_adam");
+  if (opt_ == OPT_NONE) throw Error("no optimizer: call gth_set_sgd, gth_set_adam or gth_set_adamw");
   const int p = cur_;
   begin_read();  // outside any capture: the wait for a staged upload is per step
   if (use_graph_ && graph_[p]) {
@@ -593,7 +700,7 @@ void Model::train_step() {
     int64_t before = gt_launch_count();
     if (capture) check(gt_capture_begin(ctx_));
     try {
-      forward();
+      forward(true);
       backward(false);  // the optimizer waits for the gradient buckets itself
       optimizer_step();
     } catch (...) {
@@ -639,7 +746,7 @@ void Model::predict(int32_t* preds, int64_t* correct) {
   }
   begin_read();
   const int32_t* labels = labels_device();  // the pair this evaluation reads
-  forward();
+  forward(false);
   check(gt_argmax_rows(ctx_, dtype_, ops_.back().out, batch_, classes_, (int32_t*)pred_.get()));
   if (correct) check(gt_count_equal(ctx_, (const int32_t*)pred_.get(), labels, batch_, (int64_t*)count_.get()));
   end_read();
@@ -649,7 +756,7 @@ void Model::predict(int32_t* preds, int64_t* correct) {
 
 void Model::forward_eval(void* logits_host) {
   begin_read();
-  forward();
+  forward(false);
   end_read();
   check(gt_download(ctx_, logits_host, ops_.back().out, batch_ * classes_ * es_));
 }

@@ -117,6 +117,10 @@ class Model {
 
   void set_sgd(const gt_sgd_cfg& cfg);
   void set_adam(const gt_adam_cfg& cfg);
+  void set_adamw(const gt_adam_cfg& cfg, int state, double max_norm, bool decay_vectors, uint64_t seed);
+  double grad_norm();  // of the last clipped AdamW step
+  // The last Linear and the loss as one call over pieces of the logits.
+  void set_fused_head(bool on, int32_t ignore_label);
 
   // The input and label buffers the next step reads.
   void* input_device() const { return input_[cur_].get(); }
@@ -147,7 +151,8 @@ class Model {
 
  private:
   void plan(const std::vector<gth_layer>& layers, const std::vector<int64_t>& input_shape);
-  void forward();
+  void forward(bool train);
+  void free_adamw();
   // join: the compute stream waits for the gradient all-reduce before
   // returning (else the optimizer waits bucket by bucket).
   void backward(bool join = true);
@@ -190,7 +195,13 @@ class Model {
   char* param_staging();
   int64_t grad_elems_ = 0;
 
-  enum { OPT_NONE, OPT_SGD, OPT_ADAM } opt_ = OPT_NONE;
+  enum { OPT_NONE, OPT_SGD, OPT_ADAM, OPT_ADAMW } opt_ = OPT_NONE;
+  gt_adamw* adamw_ = nullptr;
+  DevBuf opt_scales_, clip_;  // AdamW: scales of 8-bit states; the norm and the clipping coefficient
+  double max_norm_ = 0;       // 0: no clipping
+  bool fused_head_ = false;
+  int32_t ignore_label_ = -1;
+  DevBuf logits_;  // with the fused head: the logits of an evaluation, allocated on first use
   gt_sgd_cfg sgd_{};
   gt_adam_cfg adam_{};
   int64_t opt_steps_ = 0;

@@ -71,6 +71,25 @@ GT_API void* gth_grads_device(gth_model* m);
 GT_API char* gth_set_sgd(gth_model* m, const gt_sgd_cfg* cfg);
 GT_API char* gth_set_adam(gth_model* m, const gt_adam_cfg* cfg);
 
+/* AdamW (gt_adamw_*): state GT_STATE_NATIVE or GT_STATE_E4M3 (float32 models);
+ * max_norm > 0 clips the gradients by their global norm before each step (a
+ * step whose norm is not finite changes nothing); weights are decayed,
+ * one-dimensional parameters (biases) only with decay_vectors; seed is the
+ * stochastic rounding's. Resets the optimizer state. No counterpart in the
+ * reference. */
+GT_API char* gth_set_adamw(gth_model* m, const gt_adam_cfg* cfg, int state, double max_norm, int decay_vectors,
+                           uint64_t seed);
+/* The gradients' norm at the last clipped AdamW step (synchronizes). */
+GT_API char* gth_grad_norm(gth_model* m, double* out);
+/* With on != 0, training runs the last Linear, the softmax cross-entropy and
+ * their gradients as one call over pieces of the rows
+ * (gt_linear_xent_fwd_bwd): for many classes, whose logits and logits'
+ * gradient are then never kept (their buffers are released; an evaluation
+ * allocates the logits again). Rows labelled ignore_label take no part in the
+ * loss (a value outside the classes to pass over none). The model must end in
+ * a Linear. The gradients are those of the separate calls within rounding. */
+GT_API char* gth_set_fused_head(gth_model* m, int on, int32_t ignore_label);
+
 /* Device buffers the next step reads: the input batch (input_shape, model
  * dtype) and the labels (batch int32). The model has two such pairs; a step
  * moves on to the other pair only when a batch has been staged into it
