@@ -569,7 +569,7 @@ extern "C" char* gt_linear_xent_fwd_bwd(gt_ctx* ctx, int dtype, const void* x, c
       if (&p != &o && overlap(o, p)) return errorf("gt_linear_xent_fwd_bwd: two outputs overlap");
   }
   GT_ENTER(ctx);
-  if (workspace_bytes == 0) workspace_bytes = (int64_t)1 << 30;
+  if (workspace_bytes == 0) workspace_bytes = (int64_t)2 << 30;
   void* held[5] = {};
   char* err = nullptr;
   GT_DISPATCH(dtype, {

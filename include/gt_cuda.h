@@ -353,7 +353,7 @@ GT_API char* gt_xent_fwd_bwd_noalloc(gt_ctx* ctx, int dtype, const void* logits,
  * of x that counts, or in w, may turn any output that depends on them into
  * NaN.
  * The logits exist only in pieces of rows whose workspace stays within
- * workspace_bytes (0: 1 GiB; one piece of 256 rows is used whatever it says;
+ * workspace_bytes (0: 2 GiB; one piece of 256 rows is used whatever it says;
  * float32 also keeps x and w as split planes, 4 bytes per value). No output may overlap an input or another output. The result does
  * not depend on timing: the same call gives the same bits. Replaces Linear
  * followed by CrossEntropyLoss (nn/module.go:51-53, nn/loss.go:12-14) and
