@@ -124,8 +124,7 @@ __global__ void __launch_bounds__(256) xent_piece_f64_kernel(double* __restrict_
 
 // loss = sum of the rows' losses / n, in float64, one block, a fixed order.
 template <typename T>
-__global__ void __launch_bounds__(1024) mean_rows_kernel(const T* __restrict__ rows, int64_t M,
-                                                         const int64_t* __restrict__ counts, T* __restrict__ loss) {
+__global__ void __launch_bounds__(1024) mean_rows_kernel(const T* rows, int64_t M, const int64_t* counts, T* loss) {
   after_predecessor();
   __shared__ double part[32];
   double acc = 0.0;
@@ -300,10 +299,9 @@ __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restr
 // Per row: the strips' pairs joined (32 rows per block; a warp takes every
 // 32nd strip, then the warps' pairs are joined in order), the row's loss, and
 // (maximum, 1 / sum) for the gradient; 1 / sum is 0 for an ignored row.
-__global__ void __launch_bounds__(1024) strip_join_kernel(const float2* __restrict__ strips, int64_t strip_rows, int n,
+__global__ void __launch_bounds__(1024) strip_join_kernel(const float2* strips, int64_t strip_rows, int n,
                                                           const int32_t* __restrict__ labels, int64_t rows, int64_t V,
-                                                          int32_t ignore, const float* __restrict__ picked,
-                                                          float2* __restrict__ stat, float* __restrict__ row_loss) {
+                                                          int32_t ignore, const float* picked, float2* stat, float* row_loss) {
   after_predecessor();
   __shared__ float2 ws[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -332,10 +330,10 @@ static int grad_rows(const gt_ctx* ctx, int64_t rows, int64_t V) {
   return ceil_div(rows, 32) * ceil_div(V, kGradCols) >= 2 * (int64_t)ctx->sm_count ? 32 : 8;
 }
 template <bool DB>
-__global__ void __launch_bounds__(256) grad_planes_kernel(const float* __restrict__ z, const float2* __restrict__ stat,
+__global__ void __launch_bounds__(256) grad_planes_kernel(const float* z, const float2* stat,
                                                           const int32_t* __restrict__ labels, int64_t rows, int64_t V,
-                                                          int64_t Vp, int across, int rpb, __half* __restrict__ g,
-                                                          int64_t plane, float* __restrict__ part) {
+                                                          int64_t Vp, int across, int rpb, __half* g,
+                                                          int64_t plane, float* part) {
   after_predecessor();
   __shared__ float2 st[32];
   __shared__ int32_t ys[32];
@@ -372,8 +370,8 @@ __global__ void __launch_bounds__(256) grad_planes_kernel(const float* __restric
 
 // db (+)= the column sums of the blocks of rows, / n: 32 columns per block,
 // warp w adds the rows w, w + 8, ... in order, then the warps' sums in order.
-__global__ void __launch_bounds__(256) db_kernel(const float* __restrict__ part, int64_t blocks, int64_t V,
-                                                 const XentMeta* __restrict__ meta, bool first, float* __restrict__ db) {
+__global__ void __launch_bounds__(256) db_kernel(const float* part, int64_t blocks, int64_t V, const XentMeta* meta, bool first,
+                                                 float* db) {
   after_predecessor();
   __shared__ double ws[8][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -555,6 +553,8 @@ extern "C" char* gt_linear_xent_fwd_bwd(gt_ctx* ctx, int dtype, const void* x, c
   if (M <= 0 || K <= 0 || V <= 0) return errorf("gt_linear_xent_fwd_bwd: M, K and V must be positive");
   if (M > INT32_MAX / 2 || K > INT32_MAX / 2 || V > INT32_MAX / 2)
     return errorf("gt_linear_xent_fwd_bwd: M, K and V must stay below 2^30");
+  if ((double)M * (double)K > 0x1p56 || (double)V * (double)K > 0x1p56)
+    return errorf("gt_linear_xent_fwd_bwd: x and w must stay below 2^56 elements");
   if (workspace_bytes < 0) return errorf("gt_linear_xent_fwd_bwd: negative workspace");
   const int64_t es = dtype == GT_FLOAT64 ? 8 : 4;
   if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)bias | (uintptr_t)loss | (uintptr_t)row_loss | (uintptr_t)dx |

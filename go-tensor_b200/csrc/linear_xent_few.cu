@@ -137,11 +137,11 @@ __global__ void __launch_bounds__(256) few_logits_kernel(const float* __restrict
 // joined, the rows' losses, the loss. stat[m] = (maximum, 1 / sum), the latter 0
 // for an ignored row.
 template <int MT>
-__global__ void __launch_bounds__(1024) few_join_kernel(const float2* __restrict__ strips, int n, int M,
+__global__ void __launch_bounds__(1024) few_join_kernel(const float2* strips, int n, int M,
                                                         const int32_t* __restrict__ labels, int64_t V, int32_t ignore,
-                                                        const float* __restrict__ picked, float2* __restrict__ stat,
-                                                        float* __restrict__ rows, float* __restrict__ loss,
-                                                        FewMeta* __restrict__ meta, int32_t* bad) {
+                                                        const float* picked, float2* stat,
+                                                        float* rows, float* loss,
+                                                        FewMeta* meta, int32_t* bad) {
   after_predecessor();
   constexpr int PARTS = MT >= 32 ? 1 : 32 / MT;
   __shared__ float2 pair[PARTS][MT];
@@ -198,12 +198,12 @@ struct FewShared {
 // step, of dx the rows (tid / 32) MT / 8 ....
 template <int MT>
 __global__ void __launch_bounds__(256) few_grad_kernel(const float* __restrict__ x, const float* __restrict__ w,
-                                                       const float* __restrict__ z, int64_t Vp,
-                                                       const float2* __restrict__ stat,
+                                                       const float* z, int64_t Vp,
+                                                       const float2* stat,
                                                        const int32_t* __restrict__ labels, int M, int64_t K, int64_t V,
-                                                       int32_t ignore, int64_t per, const FewMeta* __restrict__ meta,
-                                                       float* __restrict__ dw, float* __restrict__ db,
-                                                       float* __restrict__ dx_part, int dw_vec) {
+                                                       int32_t ignore, int64_t per, const FewMeta* meta,
+                                                       float* dw, float* db,
+                                                       float* dx_part, int dw_vec) {
   after_predecessor();
   constexpr int R = MT / 8;  // rows of dx per thread
   extern __shared__ __align__(16) uint8_t few_smem[];
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(256) few_grad_kernel(const float* __restrict__
       const float2 s = sh.stat[m];
       float g = 0.0f;
       if (s.y != 0.0f && v0 + lane < vb)
-        g = expf(__ldg(z + m * Vp + v0 + lane) - s.x) * s.y - (sh.label[m] == v0 + lane ? 1.0f : 0.0f);
+        g = expf(z[m * Vp + v0 + lane] - s.x) * s.y - (sh.label[m] == v0 + lane ? 1.0f : 0.0f);
       sh.gm[m][lane] = g;
       sh.gv[lane][m] = g;
     }
@@ -311,8 +311,8 @@ __global__ void __launch_bounds__(256) few_grad_kernel(const float* __restrict__
   }
 }
 
-__global__ void __launch_bounds__(256) few_dx_kernel(const float* __restrict__ part, int runs, int64_t n,
-                                                     const FewMeta* __restrict__ meta, float* __restrict__ dx) {
+__global__ void __launch_bounds__(256) few_dx_kernel(const float* part, int runs, int64_t n,
+                                                     const FewMeta* meta, float* dx) {
   after_predecessor();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
@@ -331,7 +331,6 @@ static char* few_run(gt_ctx* ctx, const XentCall<float>& c, void** held) {
   const int64_t kb = c.dx || c.dw ? ceil_div(c.K, kFewCols) : 1, steps = ceil_div(c.V, kFewClasses);
   const int64_t runs0 = std::min(steps, std::max<int64_t>(ceil_div(4 * (int64_t)ctx->sm_count, kb), ceil_div(steps, 32)));
   const int64_t per = ceil_div(steps, runs0) * kFewClasses, runs = ceil_div(c.V, per);
-  if (runs > 65535) return errorf("gt_linear_xent_fwd_bwd: too many classes");
   struct {
     FewMeta* meta;
     float *z, *picked, *part;

@@ -423,11 +423,13 @@ typedef struct gt_adamw gt_adamw;
  * caller's; 0 at the start of training). Any alignment of the elements works;
  * 16-byte aligned (native: equally misaligned) arrays are fastest. Nothing
  * that the step writes may overlap anything else it touches. Not during
- * capture. Free the handle before its context. */
+ * capture. Free the handle before its context; a graph that captured its
+ * steps must not be replayed after that. */
 GT_API char* gt_adamw_new(gt_ctx* ctx, int dtype, int state, const gt_adamw_tensor* tensors, int64_t count,
                           int64_t* step_dev, uint64_t seed, gt_adamw** out);
 GT_API char* gt_adamw_free(gt_adamw* opt);
-/* New gradient addresses, one per tensor, for every later call (not during capture). */
+/* New gradient addresses, one per tensor, for every later call and every later
+ * replay of a graph that captured one (not during capture). */
 GT_API char* gt_adamw_set_grads(gt_adamw* opt, const void* const* grads, int64_t count);
 /* clip (device, 2 doubles) = the Euclidean norm of all gradients, and the
  * coefficient min(1, max_norm / norm), NaN when the norm is not finite. */

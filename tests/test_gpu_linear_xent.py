@@ -385,6 +385,23 @@ def test_two_calls_in_a_row_without_waiting():
             assert np.array_equal(got[k], want[k]), k
 
 
+@pytest.mark.parametrize("M,K,V", [(16, 30, 3336), (60, 100, 2000), (200, 64, 900), (7, 33, 500)])
+def test_calls_with_other_counts_without_waiting(M, K, V):
+    """Calls of one shape whose rows that count differ, one after another: they use the same workspace, and nothing of
+    the call before may be read from it."""
+    heads = [Head(*inputs(M, K, V, 30 + i, 0, ignored=p), 0) for i, p in enumerate((0.1, 0.8, 0.5))]
+    alone = []
+    for h in heads:
+        alone.append(h.call().host())
+    for _ in range(20):
+        for h in heads:
+            h.call()
+    for h, want in zip(heads, alone):
+        got = h.host()
+        for k in got:
+            assert np.array_equal(got[k], want[k]), k
+
+
 def test_timed_out_wait_returns_an_error_and_the_context_recovers():
     """The bounded waits of the split GEMM: with the limit at 20 ms, the peer CTA of each pair withholds one arrival, so
     the MMA issuer's wait runs out and the kernel returns; gt_sync reports it, and the next call is right."""

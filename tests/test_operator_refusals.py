@@ -28,6 +28,7 @@ def test_head_valid_arguments_reach_the_context_check():
     ({"dtype": 2}, "dtype"), ({"dtype": -1}, "dtype"), ({"x": None}, "null"), ({"w": None}, "null"),
     ({"labels": None}, "null"), ({"loss": None}, "null"), ({"M": 0}, "positive"), ({"K": 0}, "positive"),
     ({"V": 0}, "positive"), ({"M": -1}, "positive"), ({"V": 2 ** 30}, "2\\^30"), ({"M": 2 ** 40}, "2\\^30"),
+    ({"M": 2 ** 29, "K": 2 ** 29}, "2\\^56"), ({"V": 2 ** 29, "K": 2 ** 29, "dtype": 1}, "2\\^56"),
     ({"ws": -1}, "negative"), ({"x": X + 2}, "aligned"), ({"labels": Y + 1}, "aligned"),
     ({"dtype": 1, "dw": DW + 4}, "aligned"), ({"dx": X}, "overlaps"), ({"dw": W + 4}, "overlaps"),
     ({"db": B}, "overlaps"), ({"loss": Y}, "overlaps"), ({"rows": LOSS}, "two outputs"),
