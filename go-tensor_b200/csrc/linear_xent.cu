@@ -14,8 +14,9 @@
 // (split_gemm.cu):
 //
 //   operand_top_kernel   largest magnitudes of x and w, the rows that count
-//   operand_split_kernel x and w as two float16 planes each
-//   per piece of rows:
+//   operand_split_kernel w and the rows of x that count, which are listed: only
+//                        they go through the products, as two float16 planes each
+//   per piece of these rows:
 //     split_gemm         z, and per strip of 128 classes of a row its maximum
 //                        and sum of exponentials, from the registers of the
 //                        product; a forward pass alone never writes z
@@ -124,10 +125,12 @@ __global__ void __launch_bounds__(256) xent_piece_f64_kernel(double* __restrict_
 
 // loss = sum of the rows' losses / n, in float64, one block, a fixed order.
 template <typename T>
-__global__ void __launch_bounds__(1024) mean_rows_kernel(const T* rows, int64_t M, const int64_t* counts, T* loss) {
+__global__ void __launch_bounds__(1024) mean_rows_kernel(const T* rows, int64_t M, bool compact,
+                                                         const int64_t* counts, T* loss) {
   after_predecessor();
   __shared__ double part[32];
   double acc = 0.0;
+  if (compact) M = counts[0];  // only the rows that count are listed
   for (int64_t i = threadIdx.x; i < M; i += blockDim.x) acc += (double)rows[i];
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
@@ -182,15 +185,27 @@ __device__ __forceinline__ uint32_t finite_bits4(float4 v) {
   return max(max(finite_bits(v.x), finite_bits(v.y)), max(finite_bits(v.z), finite_bits(v.w)));
 }
 
+constexpr int kCompactRows = 1024;  // rows per block of the compaction
+
 // The largest magnitudes of w (blocks 0 .. w_blocks - 1) and of the rows of x
-// that count (the other blocks, a warp per row), and those rows' number; a
-// label outside [0, V) sets *bad.
+// that count (the next x_blocks, a warp per row), and how many of each 1024 rows
+// count (the others); a label outside [0, V) sets *bad.
 __global__ void __launch_bounds__(256) operand_top_kernel(const float* __restrict__ x, const float* __restrict__ w,
                                                           const int32_t* __restrict__ labels, int64_t M, int64_t K,
-                                                          int64_t V, int32_t ignore, int w_blocks, XentMeta* meta,
-                                                          int32_t* bad) {
+                                                          int64_t V, int32_t ignore, int w_blocks, int x_blocks,
+                                                          XentMeta* meta, int32_t* counts, int32_t* bad) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t top = 0;
+  if ((int)blockIdx.x >= w_blocks + x_blocks) {
+    const int64_t b = blockIdx.x - w_blocks - x_blocks;
+    int kept = 0;
+    for (int i = threadIdx.x; i < kCompactRows; i += 256) {
+      const int64_t m = b * kCompactRows + i;
+      kept += __syncthreads_count(m < M && labels[m] != ignore);
+    }
+    if (threadIdx.x == 0) counts[b] = kept;
+    return;
+  }
   if ((int)blockIdx.x < w_blocks) {
     const int64_t n = V * K, stride = (int64_t)w_blocks * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t n4 = ((uintptr_t)w & 15) == 0 ? n / 4 : 0;
@@ -204,11 +219,9 @@ __global__ void __launch_bounds__(256) operand_top_kernel(const float* __restric
     }
     for (int64_t i = n4 * 4 + at; i < n; i += stride) top = max(top, finite_bits(w[i]));
   } else {
-    int64_t kept = 0;
-    for (int64_t m = (int64_t)(blockIdx.x - w_blocks) * 8 + warp; m < M; m += (int64_t)(gridDim.x - w_blocks) * 8) {
+    for (int64_t m = (int64_t)(blockIdx.x - w_blocks) * 8 + warp; m < M; m += (int64_t)x_blocks * 8) {
       const int32_t y = labels[m];
       if (y == ignore) continue;
-      kept++;
       if (lane == 0 && bad && (y < 0 || y >= V)) *bad = 1;
       const float* r = x + m * K;
       const int64_t k4 = ((K & 3) | ((uintptr_t)x & 15)) == 0 ? K / 4 : 0;
@@ -223,7 +236,6 @@ __global__ void __launch_bounds__(256) operand_top_kernel(const float* __restric
 #pragma unroll 4
       for (int64_t k = 4 * k4 + lane; k < K; k += 32) top = max(top, finite_bits(r[k]));
     }
-    if (lane == 0 && kept) atomicAdd((unsigned long long*)&meta->count, (unsigned long long)kept);
   }
   top = __reduce_max_sync(0xffffffffu, top);
   if (lane == 0 && top) atomicMax((int)blockIdx.x < w_blocks ? &meta->w_top : &meta->x_top, top);
@@ -254,30 +266,70 @@ __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
 
 constexpr int kGradExponent = 15;  // n G lies in [-1, 1]
 
-// x (ignored rows as zeros) and w as planes of pitch Kp, a warp per row.
+// w and the rows of x that count, in their order, as planes of pitch Kp, a warp
+// per row: index[j] = the j-th such row, y[j] its label; an ignored row's dx
+// and loss are 0. Behind the last row of x come zeros up to a multiple of 32
+// rows (dw's products read that far). A row's place is the number of rows that
+// count before it: the counts of the 1024-row blocks before its own, and a
+// ballot over the labels of its own (a kernel of its own for this took 4 us more).
 __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restrict__ x, const float* __restrict__ w,
                                                             const int32_t* __restrict__ labels, int64_t M, int64_t K,
-                                                            int64_t V, int64_t Kp, int32_t ignore, XentMeta* meta,
-                                                            __half* __restrict__ xp, __half* __restrict__ wp) {
+                                                            int64_t V, int64_t Kp, int32_t ignore,
+                                                            const int32_t* counts, XentMeta* meta, int32_t* index,
+                                                            int32_t* y, __half* __restrict__ xp,
+                                                            __half* __restrict__ wp, float* __restrict__ dx,
+                                                            float* rows) {
   after_predecessor();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ex = plane_exponent(meta->x_top), ew = plane_exponent(meta->w_top);
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    const float inv = (float)(1.0 / (double)meta->count);
-    meta->logits = undo(ex + ew, 1.0f);
-    meta->dx = undo(ew + kGradExponent, inv);
-    meta->dw = undo(ex + kGradExponent, inv);
-    if (meta->count == 0) meta->dx.c1 = meta->dw.c1 = meta->dx.c2 = meta->dw.c2 = 0.0f;  // no row counts: the gradients are 0
+  // the rows that count before row `end`
+  auto count_before = [&](int64_t end) {
+    const int64_t full = end / kCompactRows;
+    int64_t n = 0;
+    for (int64_t b = lane; b < full; b += 32) n += counts[b];
+#pragma unroll 4
+    for (int64_t m = full * kCompactRows + lane; m < end; m += 32) n += labels[m] != ignore;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
+    return n;
+  };
+  if (blockIdx.x == 0 && warp == 0) {
+    const int64_t count = count_before(M);
+    if (lane == 0) {
+      const float inv = (float)(1.0 / (double)count);
+      meta->count = count;
+      meta->logits = undo(ex + ew, 1.0f);
+      meta->dx = undo(ew + kGradExponent, inv);
+      meta->dw = undo(ex + kGradExponent, inv);
+      if (count == 0)  // no row counts: the gradients are 0
+        meta->dx.c1 = meta->dw.c1 = meta->dx.c2 = meta->dw.c2 = 0.0f;
+    }
   }
-  for (int64_t i = (int64_t)blockIdx.x * 8 + warp; i < M + V; i += (int64_t)gridDim.x * 8) {
+  for (int64_t i = (int64_t)blockIdx.x * 8 + warp; i < V + M + 32; i += (int64_t)gridDim.x * 8) {
     const bool is_x = i >= V;
-    const int64_t row = is_x ? i - V : i;
+    bool keep = true;
+    int64_t row = is_x ? i - V : i, to = row;
+    if (is_x && row < M) {
+      const int32_t label = labels[row];
+      if (label == ignore) {
+        if (rows && lane == 0) rows[row] = 0.0f;
+        if (dx)
+          for (int64_t k = lane; k < K; k += 32) dx[row * K + k] = 0.0f;
+        continue;
+      }
+      to = count_before(row);
+      if (lane == 0) index[to] = (int32_t)row, y[to] = label;
+    } else if (is_x) {  // the zeros behind the last row
+      const int64_t count = count_before(M);
+      to = count + (row - M);
+      if (to >= M || to >= (count + 31) / 32 * 32) continue;
+      keep = false, row = 0;
+    }
     const float* src = (is_x ? x : w) + row * K;
-    __half* hi = (is_x ? xp : wp) + row * Kp;
+    __half* hi = (is_x ? xp : wp) + to * Kp;
     __half* lo = hi + (is_x ? M : V) * Kp;
     const int e = is_x ? ex : ew;
     const float f1 = exp2_int(e / 2), f2 = exp2_int(e - e / 2);
-    const bool keep = !is_x || labels[row] != ignore;
     if ((K & 7) == 0 && ((uintptr_t)src & 15) == 0) {
       for (int64_t k = lane; k < K / 8; k += 32) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
@@ -296,29 +348,37 @@ __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restr
   }
 }
 
+// The rows of the piece at r0 that there are.
+__device__ __forceinline__ int64_t rows_here(const XentMeta* meta, int64_t r0, int64_t R) {
+  return max((int64_t)0, min(R, meta->count - r0));
+}
+
 // Per row: the strips' pairs joined (32 rows per block; a warp takes every
-// 32nd strip, then the warps' pairs are joined in order), the row's loss, and
-// (maximum, 1 / sum) for the gradient; 1 / sum is 0 for an ignored row.
-__global__ void __launch_bounds__(1024) strip_join_kernel(const float2* strips, int64_t strip_rows, int n,
-                                                          const int32_t* __restrict__ labels, int64_t rows, int64_t V,
-                                                          int32_t ignore, const float* picked, float2* stat, float* row_loss) {
+// 32nd strip, then the warps' pairs are joined in order), the row's loss (also
+// at its place in the caller's rows), and (maximum, 1 / sum) for the gradient.
+__global__ void __launch_bounds__(1024) strip_join_kernel(const float2* strips, int64_t R, int n, const int32_t* y,
+                                                          const int32_t* index, const XentMeta* meta, int64_t r0,
+                                                          int64_t V, const float* picked, float2* stat,
+                                                          float* losses, float* rows) {
   after_predecessor();
   __shared__ float2 ws[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t m = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t m = (int64_t)blockIdx.x * 32 + lane, here = rows_here(meta, r0, R);
+  if ((int64_t)blockIdx.x * 32 >= here) return;
   float2 a = make_float2(-INFINITY, 0.0f);
-  if (m < rows) {
+  if (m < here) {
 #pragma unroll 4
-    for (int i = warp; i < n; i += 32) join(a, strips[(int64_t)i * strip_rows + m]);
+    for (int i = warp; i < n; i += 32) join(a, strips[(int64_t)i * R + m]);
   }
   ws[warp][lane] = a;
   __syncthreads();
-  if (warp == 0 && m < rows) {
+  if (warp == 0 && m < here) {
     for (int i = 1; i < 32; i++) join(a, ws[i][lane]);
-    const int32_t y = labels[m];
-    const bool kept = y != ignore;
-    stat[m] = kept ? make_float2(a.x, __fdiv_rn(1.0f, a.y)) : make_float2(0.0f, 0.0f);
-    row_loss[m] = !kept ? 0.0f : y < 0 || y >= V ? NAN : logf(a.y) + (a.x - picked[m]);
+    const int32_t label = y[r0 + m];
+    stat[m] = make_float2(a.x, __fdiv_rn(1.0f, a.y));
+    const float loss = label < 0 || label >= V ? NAN : logf(a.y) + (a.x - picked[m]);
+    losses[r0 + m] = loss;
+    if (rows) rows[index[r0 + m]] = loss;
   }
 }
 
@@ -330,17 +390,23 @@ static int grad_rows(const gt_ctx* ctx, int64_t rows, int64_t V) {
   return ceil_div(rows, 32) * ceil_div(V, kGradCols) >= 2 * (int64_t)ctx->sm_count ? 32 : 8;
 }
 template <bool DB>
-__global__ void __launch_bounds__(256) grad_planes_kernel(const float* z, const float2* stat,
-                                                          const int32_t* __restrict__ labels, int64_t rows, int64_t V,
-                                                          int64_t Vp, int across, int rpb, __half* g,
-                                                          int64_t plane, float* part) {
+__global__ void __launch_bounds__(256) grad_planes_kernel(const float* z, const float2* stat, const int32_t* y,
+                                                          const XentMeta* meta, int64_t r0, int64_t R, int64_t V,
+                                                          int64_t Vp, int across, int rpb, __half* g, int64_t plane,
+                                                          float* part) {
   after_predecessor();
   __shared__ float2 st[32];
   __shared__ int32_t ys[32];
   const int64_t rb = blockIdx.x / across, cb = blockIdx.x - rb * across;
-  const int64_t m0 = rb * rpb, c = cb * kGradCols + 4 * threadIdx.x;
-  const int n = (int)min((int64_t)rpb, rows - m0);
-  if (threadIdx.x < n) st[threadIdx.x] = stat[m0 + threadIdx.x], ys[threadIdx.x] = labels[m0 + threadIdx.x];
+  const int64_t m0 = rb * rpb, c = cb * kGradCols + 4 * threadIdx.x, here = rows_here(meta, r0, R);
+  // behind the last row come zeros up to a multiple of 32 rows (dw's products read that far)
+  const int n = (int)min((int64_t)rpb, min(R, (here + 31) / 32 * 32) - m0);
+  if (n <= 0) return;
+  if (threadIdx.x < n) {
+    const bool row = m0 + threadIdx.x < here;
+    st[threadIdx.x] = row ? stat[m0 + threadIdx.x] : make_float2(0.0f, 0.0f);
+    ys[threadIdx.x] = row ? y[r0 + m0 + threadIdx.x] : -1;
+  }
   __syncthreads();
   if (c >= V) return;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -370,12 +436,12 @@ __global__ void __launch_bounds__(256) grad_planes_kernel(const float* z, const 
 
 // db (+)= the column sums of the blocks of rows, / n: 32 columns per block,
 // warp w adds the rows w, w + 8, ... in order, then the warps' sums in order.
-__global__ void __launch_bounds__(256) db_kernel(const float* part, int64_t blocks, int64_t V, const XentMeta* meta, bool first,
+__global__ void __launch_bounds__(256) db_kernel(const float* part, int rpb, int64_t r0, int64_t R, int64_t V, const XentMeta* meta,
                                                  float* db) {
   after_predecessor();
   __shared__ double ws[8][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane, blocks = (rows_here(meta, r0, R) + rpb - 1) / rpb;
   double acc = 0.0;
   if (c < V) {
 #pragma unroll 8
@@ -386,7 +452,7 @@ __global__ void __launch_bounds__(256) db_kernel(const float* part, int64_t bloc
   if (warp != 0 || c >= V) return;
   for (int i = 1; i < 8; i++) acc += ws[i][lane];
   const float d = (float)(meta->count ? acc / (double)meta->count : 0.0);
-  db[c] = first ? d : db[c] + d;
+  db[c] = r0 == 0 ? d : db[c] + d;
 }
 
 // float32: see the top of the file.
@@ -400,12 +466,14 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
   const int64_t per_row = (grad ? 8 * Vp : 0) + 8 * strips;
   int64_t R = std::max<int64_t>(1, c.workspace / per_row / 256) * 256;
   R = std::min(c.M, ceil_div(ceil_div(c.M, ceil_div(c.M, R)), 256) * 256);
-  const int64_t blocks = ceil_div(R, grad_rows(ctx, R, c.V));
+  const int rpb = grad_rows(ctx, R, c.V);
+  const int64_t row_blocks = ceil_div(c.M, kCompactRows);
   struct {
     XentMeta* meta;
     __half *x, *w, *g;
-    float *z, *rows, *picked, *part;
+    float *z, *losses, *picked, *part;
     float2 *strips, *stat;
+    int32_t *counts, *index, *y;
   } ws;
   auto carve = [&](Carver& k) {
     ws.meta = k.take<XentMeta>(1);
@@ -413,63 +481,66 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
     ws.w = k.take<__half>(2 * c.V * Kp);
     ws.g = k.take<__half>(grad ? 2 * R * Vp : 0);
     ws.z = k.take<float>(grad ? R * Vp : 0);
-    ws.rows = k.take<float>(c.rows ? 0 : c.M);
+    ws.losses = k.take<float>(c.M);
     ws.picked = k.take<float>(R);
-    ws.part = k.take<float>(c.db ? blocks * c.V : 0);
+    ws.part = k.take<float>(c.db ? ceil_div(R, rpb) * c.V : 0);
     ws.strips = k.take<float2>(strips * R);
     ws.stat = k.take<float2>(R);
+    ws.counts = k.take<int32_t>(row_blocks);
+    ws.index = k.take<int32_t>(c.M);
+    ws.y = k.take<int32_t>(c.M);
   };
   Carver size{nullptr};
   carve(size);
   GT_TRY(scratch(ctx, (size_t)size.used, &held[0]));
   Carver at{(char*)held[0]};
   carve(at);
-  float* rows = c.rows ? c.rows : ws.rows;
 
   GT_CUDA(cudaMemsetAsync(ws.meta, 0, sizeof(XentMeta), ctx->stream));
   const int wb = grid_for(ctx, c.V * c.K, 256, 16), xb = grid_for(ctx, c.M * c.K, 256, 16);
-  operand_top_kernel<<<wb + xb, 256, 0, ctx->stream>>>(c.x, c.w, c.labels, c.M, c.K, c.V, c.ignore, wb, ws.meta,
-                                                        c.bad);
+  operand_top_kernel<<<(unsigned)(wb + xb + row_blocks), 256, 0, ctx->stream>>>(
+      c.x, c.w, c.labels, c.M, c.K, c.V, c.ignore, wb, xb, ws.meta, ws.counts, c.bad);
   GT_LAUNCH_CHECK();
-  const int sb = (int)std::min<int64_t>(ceil_div(c.M + c.V, 8), (int64_t)ctx->sm_count * 32);
+  const int sb = (int)std::min<int64_t>(ceil_div(c.M + c.V + 32, 8), (int64_t)ctx->sm_count * 32);
   GT_CUDA(launch_overlapped(ctx, operand_split_kernel, sb, 256, 0, c.x, c.w, c.labels, c.M, c.K, c.V, Kp, c.ignore,
-                            ws.meta, ws.x, ws.w));
+                            ws.counts, ws.meta, ws.index, ws.y, ws.x, ws.w, c.dx, c.rows));
   const HalfPlanes w{ws.w, c.V, c.K, Kp, c.V * Kp};
   for (int64_t r0 = 0; r0 < c.M; r0 += R) {
+    // As many pieces as all rows would need; those behind the rows that count find nothing to do.
     const int64_t r = std::min(R, c.M - r0);
     const HalfPlanes x{ws.x + r0 * Kp, r, c.K, Kp, c.M * Kp}, g{ws.g, r, c.V, Vp, R * Vp};
     SplitGemm f;
-    f.M = r, f.N = c.V, f.K = c.K, f.a = x, f.b = w, f.scale = &ws.meta->logits;
-    f.out = grad ? ws.z : nullptr, f.ldc = Vp, f.bias = c.bias, f.labels = c.labels + r0;
+    f.M = r, f.N = c.V, f.K = c.K, f.kept = &ws.meta->count, f.kept_from = r0, f.a = x, f.b = w;
+    f.scale = &ws.meta->logits;
+    f.out = grad ? ws.z : nullptr, f.ldc = Vp, f.bias = c.bias, f.labels = ws.y + r0;
     f.strips = ws.strips, f.strip_rows = R, f.picked = ws.picked;
     GT_TRY(split_gemm(ctx, f));
     GT_CUDA(launch_overlapped(ctx, strip_join_kernel, (unsigned)ceil_div(r, 32), 1024, 0, ws.strips, R, (int)strips,
-                              c.labels + r0, r, c.V, c.ignore, ws.picked, ws.stat, rows + r0));
+                              ws.y, ws.index, ws.meta, r0, c.V, ws.picked, ws.stat, ws.losses, c.rows));
     if (!grad) continue;
     const int64_t across = ceil_div(c.V, kGradCols);
-    const int rpb = grad_rows(ctx, r, c.V);
-    const int64_t down = ceil_div(r, rpb);
     GT_CUDA(launch_overlapped(ctx, c.db ? grad_planes_kernel<true> : grad_planes_kernel<false>,
-                              (unsigned)(across * down), 256, 0, ws.z, ws.stat, c.labels + r0, r, c.V, Vp, (int)across,
-                              rpb, ws.g, R * Vp, ws.part));
+                              (unsigned)(across * ceil_div(r, rpb)), 256, 0, ws.z, ws.stat, ws.y, ws.meta, r0, r, c.V,
+                              Vp, (int)across, rpb, ws.g, R * Vp, ws.part));
     if (c.dx) {
       SplitGemm d;
-      d.M = r, d.N = c.K, d.K = c.V, d.a = g, d.b = w, d.b_mn = true, d.scale = &ws.meta->dx;
-      d.out = c.dx + r0 * c.K, d.ldc = c.K;
+      d.M = r, d.N = c.K, d.K = c.V, d.kept = &ws.meta->count, d.kept_from = r0, d.a = g, d.b = w, d.b_mn = true;
+      d.scale = &ws.meta->dx;
+      d.out = c.dx, d.ldc = c.K, d.row_index = ws.index + r0;
       GT_TRY(split_gemm(ctx, d));
     }
     if (c.dw) {
       SplitGemm d;
-      d.M = c.V, d.N = c.K, d.K = r, d.a = g, d.a_mn = true, d.b = x, d.b_mn = true, d.scale = &ws.meta->dw;
+      d.M = c.V, d.N = c.K, d.K = r, d.kept = &ws.meta->count, d.kept_from = r0, d.a = g, d.a_mn = true, d.b = x;
+      d.b_mn = true, d.scale = &ws.meta->dw;
       d.out = c.dw, d.ldc = c.K, d.accumulate = r0 > 0;
       GT_TRY(split_gemm(ctx, d));
     }
-    if (c.db) {
-      GT_CUDA(launch_overlapped(ctx, db_kernel, (unsigned)ceil_div(c.V, 32), 256, 0, ws.part, down, c.V, ws.meta,
-                                r0 == 0, c.db));
-    }
+    if (c.db)
+      GT_CUDA(launch_overlapped(ctx, db_kernel, (unsigned)ceil_div(c.V, 32), 256, 0, ws.part, rpb, r0, r, c.V, ws.meta,
+                                c.db));
   }
-  GT_CUDA(launch_overlapped(ctx, mean_rows_kernel<float>, 1, 1024, 0, rows, c.M, &ws.meta->count, c.loss));
+  GT_CUDA(launch_overlapped(ctx, mean_rows_kernel<float>, 1, 1024, 0, ws.losses, c.M, true, &ws.meta->count, c.loss));
   return nullptr;
 }
 
@@ -525,7 +596,7 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
       GT_LAUNCH_CHECK();
     }
   }
-  mean_rows_kernel<double><<<1, 1024, 0, ctx->stream>>>(rows, c.M, counts, c.loss);
+  mean_rows_kernel<double><<<1, 1024, 0, ctx->stream>>>(rows, c.M, false, counts, c.loss);
   GT_LAUNCH_CHECK();
   return nullptr;
 }

@@ -66,6 +66,7 @@ static_assert(128 * SREGS_LOW + 256 * SREGS_HIGH <= STHREADS * 168, "register sp
 
 struct SplitUnits {
   int whole = 0, splits = 1;  // tiles computed whole; K-splits of the others
+  int pairs = 1;              // SM pairs
   float* ws = nullptr;        // [splits][tiles - whole][256 * 256]
   uint64_t wait_limit_ns = kTimeoutNs;
   int withhold = 0;  // test hook: the peer's relay withholds its first arrival
@@ -83,6 +84,10 @@ struct SplitShared {
 
 struct SplitArgs {
   int64_t M, N, K;
+  const int64_t* kept;
+  int64_t kept_from;
+  int kept_k;  // the rows that there are limit K, not M
+  const int32_t* row_index;
   const SplitScale* scale;
   float* out;
   int64_t ldc;
@@ -96,8 +101,38 @@ struct SplitArgs {
   float* picked;
 };
 
+// The sizes that there really are (SplitGemm::kept), and the units for them: the
+// host planned for all rows. Whole tiles stay whole and tiles that were all
+// split stay split S ways; where only the last round's tiles were, the new
+// last round's are split as far as the pairs go round (so the workspace, one
+// partial tile per pair, holds them).
+struct SplitSizes {
+  int M, K;  // (below 2^30)
+  int whole, splits;
+};
+__device__ __forceinline__ SplitSizes actual_sizes(const SplitArgs& s, const SplitUnits& su) {
+  SplitSizes z{(int)s.M, (int)s.K, su.whole, su.splits};
+  if (!s.kept) return z;
+  const int host = s.kept_k ? z.K : z.M, n = (int)max((int64_t)0, min((int64_t)host, *s.kept - s.kept_from));
+  if (n == host) return z;
+  if (s.kept_k) {
+    z.K = n;
+    if (n == 0 && s.accumulate) z = {0, 0, 0, 1};  // nothing to add
+    return z;
+  }
+  z.M = n;
+  const int tiles = (z.M + STILE - 1) / STILE * (int)((s.N + STILE - 1) / STILE);
+  if (su.splits > 1 && su.whole > 0) {
+    z.whole = tiles / su.pairs * su.pairs;
+    const int rest = tiles - z.whole;
+    z.splits = rest ? max(1, min(min(su.pairs / rest, 64), (z.K + SBK - 1) / SBK / (2 * SGROUP_MAX))) : 1;
+  }
+  if (z.splits == 1) z.whole = tiles;
+  return z;
+}
+
 // Unit u: tile (mt, nt) over the stages [kb, ke); the split index or -1.
-__device__ __forceinline__ int split_unit(int u, int m_tiles, int n_tiles, int m_fast, const SplitUnits& su, int num_k,
+__device__ __forceinline__ int split_unit(int u, int m_tiles, int n_tiles, int m_fast, const SplitSizes& su, int num_k,
                                           int& t, int& mt, int& nt, int& kb, int& ke) {
   const int tiles = m_tiles * n_tiles;
   int sidx = -1;
@@ -202,21 +237,18 @@ __device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
 
 template <bool A_MN, bool B_MN, bool LOGITS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
-    split_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const SplitArgs s,
-                      const SplitUnits su) {
+    split_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                      const SplitArgs s, const SplitUnits su) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   SplitShared* sh = (SplitShared*)(smem + SBAR_OFFSET);
   constexpr int SGROUP = group_stages<A_MN, LOGITS>();
+  constexpr bool INDEXED = !A_MN && !LOGITS;  // dx: the rows of C are scattered
   volatile int* failed = &sh->failed;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const bool leader = rank == 0;
-  const int num_k = (int)((s.K + SBK - 1) / SBK);
-  const int m_tiles = (int)((s.M + STILE - 1) / STILE), n_tiles = (int)((s.N + STILE - 1) / STILE);
-  const int tiles = m_tiles * n_tiles;
-  const int units = su.whole + (tiles - su.whole) * su.splits;
   const int pair = (int)cluster_id(), pairs = (int)num_clusters();
 
   if (threadIdx.x == 0) {
@@ -246,6 +278,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
   after_predecessor();
+  const SplitSizes sz = actual_sizes(s, su);
+  const int num_k = (sz.K + SBK - 1) / SBK;
+  const int m_tiles = (sz.M + STILE - 1) / STILE, n_tiles = (int)((s.N + STILE - 1) / STILE);
+  const int tiles = m_tiles * n_tiles;
+  const int units = sz.whole + (tiles - sz.whole) * sz.splits;
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SREGS_LOW));
@@ -254,7 +291,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
       int it = 0, issued_to = 0;
       for (int u = pair; u < units && !__shfl_sync(0xffffffffu, *failed, 0); u += pairs) {
         int t, mt, nt, kb, ke;
-        split_unit(u, m_tiles, n_tiles, s.m_fast, su, num_k, t, mt, nt, kb, ke);
+        split_unit(u, m_tiles, n_tiles, s.m_fast, sz, num_k, t, mt, nt, kb, ke);
         const int a_row = mt * STILE + (int)rank * SBM, b_row = nt * STILE + (int)rank * SBM;
         for (int kt = kb; kt < ke; kt++, it++) {
           const int st = it % SSTAGES;
@@ -286,7 +323,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
         bool stop = false;
         for (int u = pair; u < units && !stop; u += pairs) {
           int t, mt, nt, kb, ke;
-          split_unit(u, m_tiles, n_tiles, s.m_fast, su, num_k, t, mt, nt, kb, ke);
+          split_unit(u, m_tiles, n_tiles, s.m_fast, sz, num_k, t, mt, nt, kb, ke);
           for (int kt = kb; kt < ke; kt++, it++) {
             const int st = it % SSTAGES;
             const uint32_t phase = (it / SSTAGES) & 1;
@@ -338,7 +375,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
       bool stop = false;
       for (int u = pair; u < units && !stop; u += pairs) {
         int t, mt, nt, kb, ke;
-        split_unit(u, m_tiles, n_tiles, s.m_fast, su, num_k, t, mt, nt, kb, ke);
+        split_unit(u, m_tiles, n_tiles, s.m_fast, sz, num_k, t, mt, nt, kb, ke);
         for (int kt = kb; kt < ke; kt++, it++) {
           const int st = it % SSTAGES;
           if (__shfl_sync(0xffffffffu, *failed, 0) ||
@@ -363,8 +400,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
     int group = 0;
     for (int u = pair; u < units && !__shfl_sync(0xffffffffu, *failed, 0); u += pairs) {
       int t, mt, nt, kb, ke;
-      const int sidx = split_unit(u, m_tiles, n_tiles, s.m_fast, su, num_k, t, mt, nt, kb, ke);
+      const int sidx = split_unit(u, m_tiles, n_tiles, s.m_fast, sz, num_k, t, mt, nt, kb, ke);
       const int groups = (ke - kb + SGROUP - 1) / SGROUP;
+      const int m0 = mt * STILE + (int)rank * SBM + 32 * q, n0 = nt * STILE + 128 * h;  // (sizes stay below 2^30)
+      const int rows = max(0, min(32, sz.M - m0));
+      // What the epilogue reads besides, fetched while the products run: row m0 +
+      // r of C in out (lane r holds it; without an index, and in the
+      // workspace, the r-th), the row's label, the columns' biases.
+      int32_t my_row = lane;
+      if constexpr (INDEXED) {
+        if (sidx < 0 && lane < rows) my_row = s.row_index[m0 + lane] - m0;
+      }
+      const int32_t label = LOGITS && lane < rows ? s.labels[m0 + lane] : -1;
+      float bias[LOGITS ? 4 : 1];
+      if constexpr (LOGITS) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) bias[j] = s.bias && n0 + 32 * j + lane < s.N ? __ldg(s.bias + n0 + 32 * j + lane) : 0.0f;
+      }
       float tot[128];
 #pragma unroll
       for (int i = 0; i < 128; i++) tot[i] = 0.0f;
@@ -394,16 +446,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
         if (lane == 0) mbar_arrive_rank(&sh->pempty[buf], 0);
       }
       if (!ok) break;
-      const int64_t m0 = (int64_t)mt * STILE + rank * SBM + 32 * q, n0 = (int64_t)nt * STILE + 128 * h;
-      const int rows = (int)(s.M - m0 < 32 ? (s.M - m0 > 0 ? s.M - m0 : 0) : 32);
       float* part = sidx < 0 ? nullptr
-                             : su.ws + ((int64_t)sidx * (tiles - su.whole) + (t - su.whole)) * STILE_ELEMS +
+                             : su.ws + ((int64_t)sidx * (tiles - sz.whole) + (t - sz.whole)) * STILE_ELEMS +
                                    (int64_t)(rank * SBM + 32 * q) * STILE + 128 * h;
-      float* dst = part ? part : s.out ? s.out + m0 * s.ldc + n0 : nullptr;
+      float* dst = part ? part : s.out ? s.out + (int64_t)m0 * s.ldc + n0 : nullptr;
       const int64_t ld = part ? STILE : s.ldc;
       const bool vec = part || s.vec;
       float top = -INFINITY, sum = 0.0f;  // LOGITS: this lane's row over the strip
-      const int32_t label = LOGITS && lane < rows ? s.labels[m0 + lane] : -1;
       // 32 x 32 blocks through the per-warp buffer (the switch keeps the
       // register indices static in a loop that is not unrolled).
 #pragma unroll 1
@@ -415,15 +464,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
           case 2: split_chunk<2>(z, tot); break;
           default: split_chunk<3>(z, tot); break;
         }
-        const int64_t nb = n0 + 32 * j;
-        const int cols = part ? 32 : (int)(s.N - nb < 32 ? (s.N - nb > 0 ? s.N - nb : 0) : 32);
+        const int nb = n0 + 32 * j, cols = part ? 32 : max(0, min(32, (int)s.N - nb));
         if (!part) {
 #pragma unroll
           for (int i = 0; i < 32; i++) z[i] = apply(sc, z[i]);
         }
         if constexpr (LOGITS) {
           if (s.bias) {
-            const float my_bias = lane < cols ? __ldg(s.bias + nb + lane) : 0.0f;
+            const float my_bias = j == 0 ? bias[0] : j == 1 ? bias[1] : j == 2 ? bias[2] : bias[3];
 #pragma unroll
             for (int i = 0; i < 32; i++) z[i] = __fadd_rn(z[i], __shfl_sync(0xffffffffu, my_bias, i));
           }
@@ -439,8 +487,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
         if (dst) {
           if (vec && cols == 32) {  // 4 rows x 128 bytes per access
             const int r0 = lane >> 3, c = lane & 7;
-            float* o = dst + (int64_t)r0 * ld + 32 * j + 4 * c;
-            if (!LOGITS && s.accumulate && !part) {
+            float* o = dst + (INDEXED ? 0 : (int64_t)r0 * ld) + 32 * j + 4 * c;
+            if (A_MN && s.accumulate && !part) {
               // the old values of all rows before any is written: a load per
               // row behind the store before it made the kernel three times as
               // slow
@@ -458,13 +506,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
               }
             } else {
 #pragma unroll
-              for (int k = 0; k < 8; k++)
+              for (int k = 0; k < 8; k++) {
+                const int64_t row = INDEXED ? __shfl_sync(0xffffffffu, my_row, r0 + 4 * k) : 4 * k;
                 if (part || r0 + 4 * k < rows)
-                  *reinterpret_cast<float4*>(o + 4 * k * ld) = *block_chunk(xpose, r0 + 4 * k, c);
+                  *reinterpret_cast<float4*>(o + row * ld) = *block_chunk(xpose, r0 + 4 * k, c);
+              }
+            }
+          } else if constexpr (INDEXED) {  // (every lane: the rows come by shuffle)
+            float* o = dst + 32 * j + lane;
+#pragma unroll 8
+            for (int r = 0; r < rows; r++) {
+              const int64_t row = __shfl_sync(0xffffffffu, my_row, r);
+              if (lane < cols) o[row * ld] = block_at(xpose, r, lane);
             }
           } else if (lane < cols) {
             float* o = dst + 32 * j + lane;
-            if (!LOGITS && s.accumulate) {
+            if (A_MN && s.accumulate) {
 #pragma unroll 1
               for (int r0 = 0; r0 < 32; r0 += 16) {
                 float was[16];
@@ -492,14 +549,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
           for (int i = 0; i < 32; i++) add[i & 3] += exp_below(z[i] - from);
           sum = sum * exp_below(top - from) + ((add[0] + add[1]) + (add[2] + add[3]));
           top = up;
-          const int64_t at = (int64_t)label - nb;
-          if (at >= 0 && at < cols) s.picked[m0 + lane] = block_at(xpose, lane, (int)at);
+          if (label >= nb && label < nb + cols) s.picked[m0 + lane] = block_at(xpose, lane, label - nb);
         }
         __syncwarp();
       }
       if constexpr (LOGITS) {
         if (!part && lane < rows && n0 < s.N)
-          s.strips[(n0 / kStripCols) * s.strip_rows + m0 + lane] = make_float2(top, sum);
+          s.strips[(int64_t)(n0 / kStripCols) * s.strip_rows + m0 + lane] = make_float2(top, sum);
       }
     }
   }
@@ -513,19 +569,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
 }
 
 // The split tiles: their partials added in split order, then the epilogue.
-__global__ void split_reduce_kernel(SplitUnits su, int m_tiles, int n_tiles, SplitArgs s) {
+__global__ void split_reduce_kernel(SplitUnits su, SplitArgs s) {
   after_predecessor();
-  const int rest = m_tiles * n_tiles - su.whole;
+  const SplitSizes sz = actual_sizes(s, su);
+  const int m_tiles = (sz.M + STILE - 1) / STILE, n_tiles = (int)((s.N + STILE - 1) / STILE);
+  const int rest = m_tiles * n_tiles - sz.whole;
   const int64_t total = (int64_t)rest * STILE_ELEMS;
   const SplitScale sc = *s.scale;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int r = (int)(i / STILE_ELEMS), e = (int)(i - (int64_t)r * STILE_ELEMS), t = su.whole + r;
+    const int r = (int)(i / STILE_ELEMS), e = (int)(i - (int64_t)r * STILE_ELEMS), t = sz.whole + r;
     const int mt = s.m_fast ? t % m_tiles : t / n_tiles, nt = s.m_fast ? t / m_tiles : t % n_tiles;
     const int64_t m = (int64_t)mt * STILE + e / STILE, n = (int64_t)nt * STILE + e % STILE;
-    if (m >= s.M || n >= s.N) continue;
+    if (m >= sz.M || n >= s.N) continue;
     float acc = su.ws[i];
-    for (int k = 1; k < su.splits; k++) acc = __fadd_rn(acc, su.ws[(int64_t)k * total + i]);
-    float* o = s.out + m * s.ldc + n;
+    for (int k = 1; k < sz.splits; k++) acc = __fadd_rn(acc, su.ws[(int64_t)k * total + i]);
+    float* o = s.out + (s.row_index ? (int64_t)s.row_index[m] : m) * s.ldc + n;
     acc = apply(sc, acc);
     *o = s.accumulate ? __fadd_rn(*o, acc) : acc;
   }
@@ -592,22 +650,24 @@ static char* split_launch(gt_ctx* ctx, const SplitGemm& g) {
     su.whole = (int)tiles;
   else
     su = split_plan(tiles, avail, ceil_div(g.K, SBK));
+  su.pairs = (int)avail;
   su.wait_limit_ns = tc_wait_limit_ns();
   su.withhold = tc_take_withhold();
   const int vec = (((uintptr_t)g.out & 15) | (g.ldc & 3)) == 0;
-  SplitArgs s{g.M, g.N, g.K, g.scale, g.out, g.ldc, g.accumulate, vec, g.N > g.M, g.bias, g.labels, g.strips, g.strip_rows,
-              g.picked};
+  SplitArgs s{g.M,   g.N,          g.K, g.kept,      g.kept_from, A_MN,     g.row_index, g.scale,      g.out,
+              g.ldc, g.accumulate, vec, g.N > g.M,   g.bias,      g.labels, g.strips,    g.strip_rows, g.picked};
   void* ws = nullptr;
   if (su.splits > 1) {
-    GT_TRY(scratch(ctx, (size_t)su.splits * (tiles - su.whole) * STILE_ELEMS * sizeof(float), &ws));
+    // (with fewer rows than planned, the tiles split in the last round may be up to one per pair)
+    const int64_t parts = su.whole > 0 ? std::max(avail, su.splits * (tiles - su.whole)) : su.splits * tiles;
+    GT_TRY(scratch(ctx, (size_t)parts * STILE_ELEMS * sizeof(float), &ws));
     su.ws = (float*)ws;
   }
   const int64_t units = su.whole + (tiles - su.whole) * su.splits;
   cudaError_t e = launch_overlapped(ctx, kern, (unsigned)(2 * std::min(units, avail)), STHREADS, SSMEM_BYTES, ta, tb, s,
                                     su);
   if (e == cudaSuccess && su.splits > 1)
-    e = launch_overlapped(ctx, split_reduce_kernel, grid_for(ctx, (tiles - su.whole) * STILE_ELEMS, 256), 256, 0, su,
-                          (int)m_tiles, (int)n_tiles, s);
+    e = launch_overlapped(ctx, split_reduce_kernel, grid_for(ctx, (tiles - su.whole) * STILE_ELEMS, 256), 256, 0, su, s);
   if (e == cudaSuccess) e = cudaGetLastError();
   release(ctx, ws);
   if (e != cudaSuccess) return cuda_error(e, "split_gemm launch", __FILE__, __LINE__);
@@ -625,6 +685,8 @@ char* split_gemm(gt_ctx* ctx, const SplitGemm& g) {
     if (g.a_mn || g.b_mn) return errorf("split_gemm: the logits' operands are K-major");
     return tc::split_launch<false, false, true>(ctx, g);
   }
+  if (g.a_mn ? g.row_index != nullptr : !g.row_index || g.accumulate)
+    return errorf("split_gemm: an index of rows goes with K-major A and no accumulation");
   if (!g.a_mn && g.b_mn) return tc::split_launch<false, true, false>(ctx, g);
   if (g.a_mn && g.b_mn) return tc::split_launch<true, true, false>(ctx, g);
   return errorf("split_gemm: layout not built");

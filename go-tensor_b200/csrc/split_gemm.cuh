@@ -27,6 +27,12 @@ struct SplitScale {
 // K and columns N (b_mn).
 struct SplitGemm {
   int64_t M = 0, N = 0, K = 0;
+  // The rows (a_mn: the K) that there really are, known on the device only:
+  // min(M or K, max(0, *kept - kept_from)); NULL: all. What lies behind them, up
+  // to a multiple of 32 of K, is zero.
+  const int64_t* kept = nullptr;
+  int64_t kept_from = 0;
+  const int32_t* row_index = nullptr;  // row m of C goes to row row_index[m] of out
   HalfPlanes a, b;
   bool a_mn = false, b_mn = false;
   const SplitScale* scale = nullptr;  // device

@@ -250,11 +250,29 @@ def test_ignored_rows_may_hold_anything(dt):
         assert np.array_equal(got[k], clean[k]), k
 
 
+@pytest.mark.parametrize("M,V,workspace", [(700, 2049, 1), (1500, 9000, 16 << 20), (1100, 20011, 0), (300, 260, 0)])
+@pytest.mark.parametrize("which", ["half", "most", "first", "last", "one", "all but one", "a piece"])
+def test_rows_that_count_anywhere(M, V, workspace, which):
+    """Only the rows that count go through the products: their order, pieces without one, counts at and beside the
+    multiples of 32 and 256."""
+    x, w, b, y = inputs(M, 70, V, M + V, 0)
+    m = np.arange(M)
+    drop = {"half": np.random.default_rng(2).random(M) < 0.5, "most": np.random.default_rng(3).random(M) < 0.97,
+            "first": m < M - 257, "last": m >= 256, "one": m != M // 2, "all but one": m == M - 1,
+            "a piece": (m // 256) % 2 == 0}[which]
+    y = np.where(drop, IGN, y)
+    x[drop] = np.nan
+    clean = np.where(drop[:, None], 0, x)
+    h = Head(x, w, b, y, 0, workspace_bytes=workspace).call()
+    compare(h.host(), *reference(clean, w, b, y, 0))
+
+
 @pytest.mark.parametrize("dt", [0, 1])
-def test_every_row_ignored(dt):
-    x, w, b, _ = inputs(70, 16, 300, 13, dt)
+@pytest.mark.parametrize("M,workspace", [(70, 0), (10, 0), (600, 1)])
+def test_every_row_ignored(dt, M, workspace):
+    x, w, b, _ = inputs(M, 16, 300, 13, dt)
     x[3] = np.nan
-    h = Head(x, w, b, np.full(70, IGN), dt).call()
+    h = Head(x, w, b, np.full(M, IGN), dt, workspace_bytes=workspace).call()
     got = h.host()
     assert np.isnan(got["loss"]).all() and h.bad.host()[0] == 0
     for k in ("rows", "dx", "dw", "db"):
