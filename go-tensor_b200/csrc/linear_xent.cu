@@ -194,6 +194,7 @@ __global__ void __launch_bounds__(256) operand_top_kernel(const float* __restric
                                                           const int32_t* __restrict__ labels, int64_t M, int64_t K,
                                                           int64_t V, int32_t ignore, int w_blocks, int x_blocks,
                                                           XentMeta* meta, int32_t* counts, int32_t* bad) {
+  __shared__ uint32_t tops[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t top = 0;
   if ((int)blockIdx.x >= w_blocks + x_blocks) {
@@ -238,7 +239,12 @@ __global__ void __launch_bounds__(256) operand_top_kernel(const float* __restric
     }
   }
   top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0 && top) atomicMax((int)blockIdx.x < w_blocks ? &meta->w_top : &meta->x_top, top);
+  if (lane == 0) tops[warp] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; i++) top = max(top, tops[i]);
+    if (top) atomicMax((int)blockIdx.x < w_blocks ? &meta->w_top : &meta->x_top, top);
+  }
 }
 
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
@@ -342,8 +348,14 @@ __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restr
         reinterpret_cast<uint4*>(lo)[k] = *reinterpret_cast<uint4*>(l);
       }
     } else {
-#pragma unroll 4
-      for (int64_t k = lane; k < K; k += 32) split_half(__fmul_rn(__fmul_rn(keep ? src[k] : 0.0f, f1), f2), hi[k], lo[k]);
+      for (int64_t k = lane; k < K; k += 256) {  // eight loads in flight
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = keep && k + 32 * j < K ? src[k + 32 * j] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (k + 32 * j < K) split_half(__fmul_rn(__fmul_rn(v[j], f1), f2), hi[k + 32 * j], lo[k + 32 * j]);
+      }
     }
   }
 }
@@ -497,7 +509,8 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
   carve(at);
 
   GT_CUDA(cudaMemsetAsync(ws.meta, 0, sizeof(XentMeta), ctx->stream));
-  const int wb = grid_for(ctx, c.V * c.K, 256, 16), xb = grid_for(ctx, c.M * c.K, 256, 16);
+  const int most = 8 * ctx->sm_count;  // resident blocks: one round each
+  const int wb = std::min(most, grid_for(ctx, c.V * c.K, 256, 16)), xb = std::min(most, grid_for(ctx, c.M * c.K, 256, 16));
   operand_top_kernel<<<(unsigned)(wb + xb + row_blocks), 256, 0, ctx->stream>>>(
       c.x, c.w, c.labels, c.M, c.K, c.V, c.ignore, wb, xb, ws.meta, ws.counts, c.bad);
   GT_LAUNCH_CHECK();
