@@ -190,6 +190,15 @@ def test_bits_against_numpy(state, dt, sizes):
         a.same()
 
 
+def test_bits_of_many_values():
+    """A million and a half values with 8-bit states: the packed square roots and quotients are the rounded ones."""
+    a = Many([1500007, 300000], 0, 1)
+    for _ in range(3):
+        a.opt.step()
+        a.host_step()
+        a.same()
+
+
 @pytest.mark.parametrize("state,dt,shift", [(0, 0, 4), (0, 0, 12), (0, 1, 8), (1, 0, 4), (0, 0, {"g": 4}), (0, 0, {"m": 8}),
                                             (0, 1, {"p": 8}), (1, 0, {"m": 1}), (1, 0, {"v": 3, "m": 7}), (1, 0, {"g": 8})])
 def test_any_alignment(state, dt, shift):

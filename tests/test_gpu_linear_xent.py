@@ -152,7 +152,8 @@ def inputs(M, K, V, seed, dt, gain=2.0, bias=True, ignored=0.0):
 @pytest.mark.parametrize("dt", [0, 1])
 @pytest.mark.parametrize("M,K,V", [(1, 1, 1), (1, 1, 2), (1, 16, 200), (2, 3, 5), (7, 96, 517), (31, 33, 255),
                                    (33, 65, 129), (64, 32, 256), (128, 64, 1000), (129, 31, 257), (257, 130, 1025),
-                                   (300, 257, 2049), (513, 512, 300), (5, 1000, 4099), (1000, 8, 777), (256, 256, 256)])
+                                   (300, 257, 2049), (513, 512, 300), (5, 1000, 4099), (1000, 8, 777), (256, 256, 256),
+                                   (100, 20, 1), (100, 1, 2), (70, 3, 33), (500, 16, 7), (65, 1, 1), (66, 7, 128)])
 @pytest.mark.parametrize("bias,ignored", [(True, 0.0), (False, 0.3)])
 def test_against_float64(dt, M, K, V, bias, ignored):
     x, w, b, y = inputs(M, K, V, M * 7 + K * 3 + V, dt, bias=bias, ignored=ignored)
@@ -201,10 +202,11 @@ def test_masked_classes(dt):
     assert (got["db"][np.isinf(b)] == 0).all() and (got["dw"][np.isinf(b)] == 0).all()
 
 
+@pytest.mark.parametrize("M", [40, 140])  # on the FP32 pipe and on the tensor cores
 @pytest.mark.parametrize("dt", [0, 1])
-def test_lowest_value_masks(dt):
+def test_lowest_value_masks(dt, M):
     """The type's lowest value as a mask, on some classes and on all of them (then the softmax is that of equal logits)."""
-    x, w, b, y = inputs(40, 32, 300, 8, dt)
+    x, w, b, y = inputs(M, 32, 300, 8, dt)
     low = np.finfo(NP[dt]).min
     b[100:] = low
     y = y % 100
@@ -215,9 +217,10 @@ def test_lowest_value_masks(dt):
     np.testing.assert_allclose(got["db"].sum(), 0, atol=1e-5)
 
 
+@pytest.mark.parametrize("M", [20, 150])  # on the FP32 pipe and on the tensor cores
 @pytest.mark.parametrize("dt", [0, 1])
-def test_label_on_a_masked_class(dt):
-    x, w, b, y = inputs(20, 16, 90, 9, dt)
+def test_label_on_a_masked_class(dt, M):
+    x, w, b, y = inputs(M, 16, 90, 9, dt)
     b[7] = -np.inf
     y[:] = 3
     y[4] = 7
@@ -226,9 +229,10 @@ def test_label_on_a_masked_class(dt):
     assert np.isfinite(got["dx"]).all() and np.isfinite(got["dw"]).all() and got["db"][7] < 0
 
 
+@pytest.mark.parametrize("M", [20, 150])  # on the FP32 pipe and on the tensor cores
 @pytest.mark.parametrize("dt", [0, 1])
-def test_every_class_masked(dt):
-    x, w, b, y = inputs(20, 16, 300, 10, dt)
+def test_every_class_masked(dt, M):
+    x, w, b, y = inputs(M, 16, 300, 10, dt)
     b[:] = -np.inf
     got = Head(x, w, b, y, dt).call().host()
     for k in got:
@@ -279,10 +283,11 @@ def test_every_row_ignored(dt, M, workspace):
         assert (got[k] == 0).all(), k
 
 
+@pytest.mark.parametrize("M", [20, 150])  # on the FP32 pipe and on the tensor cores
 @pytest.mark.parametrize("dt", [0, 1])
 @pytest.mark.parametrize("label", [-1, 90, 2 ** 31 - 1, -2 ** 31])
-def test_label_outside(dt, label):
-    x, w, b, y = inputs(20, 16, 90, 14, dt)
+def test_label_outside(dt, label, M):
+    x, w, b, y = inputs(M, 16, 90, 14, dt)
     y[5] = label
     h = Head(x, w, b, y, dt).call()
     got = h.host()
@@ -290,9 +295,10 @@ def test_label_outside(dt, label):
     assert np.isfinite(np.delete(got["rows"], 5)).all()
 
 
+@pytest.mark.parametrize("M", [60, 200])  # on the FP32 pipe and on the tensor cores
 @pytest.mark.parametrize("dt", [0, 1])
-def test_ignored_label_may_be_a_class(dt):
-    x, w, b, y = inputs(60, 16, 90, 15, dt)
+def test_ignored_label_may_be_a_class(dt, M):
+    x, w, b, y = inputs(M, 16, 90, 15, dt)
     y[::4] = 17
     want, tol = reference(x, w, b, np.where(y == 17, IGN, y), dt)
     compare(Head(x, w, b, y, dt, ignore_label=17).call().host(), want, tol)
@@ -316,23 +322,25 @@ def test_uneven_rows():
     compare(Head(x, w, b, y, 0).call().host(), *reference(x, w, b, y, 0))
 
 
-def test_all_zero_operands():
-    x, w, b, y = inputs(40, 32, 260, 18, 0)
+@pytest.mark.parametrize("M", [40, 140])
+def test_all_zero_operands(M):
+    x, w, b, y = inputs(M, 32, 260, 18, 0)
     compare(Head(x * 0, w, b, y, 0).call().host(), *reference(x * 0, w, b, y, 0))
     compare(Head(x, w * 0, b, y, 0).call().host(), *reference(x, w * 0, b, y, 0))
 
 
+@pytest.mark.parametrize("M", [40, 140])  # on the FP32 pipe and on the tensor cores
 @pytest.mark.parametrize("what", ["x", "w"])
 @pytest.mark.parametrize("value", [np.nan, np.inf])
-def test_not_finite_in_a_row_that_counts(what, value):
+def test_not_finite_in_a_row_that_counts(what, value, M):
     """The other rows' losses do not see it in x; in w every row does."""
-    x, w, b, y = inputs(40, 32, 260, 19, 0)
+    x, w, b, y = inputs(M, 32, 260, 19, 0)
     want, tol = reference(x, w, b, y, 0)
     (x if what == "x" else w)[6, 5] = value
     got = Head(x, w, b, y, 0).call().host()
     assert np.isnan(got["loss"][0]) or np.isinf(got["loss"][0])
     if what == "x":
-        rest = np.arange(40) != 6
+        rest = np.arange(M) != 6
         assert (np.abs(got["rows"] - want["rows"])[rest] <= tol["rows"][rest]).all()
         assert (np.abs(got["dx"] - want["dx"])[rest] <= tol["dx"][rest]).all()
         assert not np.isfinite(got["rows"][6])
@@ -418,6 +426,60 @@ def test_calls_with_other_counts_without_waiting(M, K, V):
         got = h.host()
         for k in got:
             assert np.array_equal(got[k], want[k]), k
+
+
+@pytest.mark.parametrize("dt", [0, 1])
+@pytest.mark.parametrize("M,K,V", [(20, 36, 300), (150, 64, 520), (300, 33, 129)])
+def test_addresses_beside_16_bytes(dt, M, K, V):
+    """Every operand and result one element past a 16-byte boundary, in pieces and at once; what lies around them stays."""
+    from test_gpu_adamw import Raw
+    t, es = NP[dt], 8 if dt else 4
+    x, w, b, y = inputs(M, K, V, 27, dt, ignored=0.2)
+    want, tol = reference(x, w, b, y, dt)
+    be = cuda_backend()
+    held = {k: Raw(np.full(a.size + 8, 7.0, t)) for k, a in (("x", x), ("w", w), ("b", b))}
+    for k, a in (("x", x), ("w", w), ("b", b)):
+        v = np.full(a.size + 8, 7.0, t)
+        v[1:1 + a.size] = a.reshape(-1)
+        held[k].set(v)
+    out = {k: Raw(np.full(a.size + 8, 7.0, t)) for k, a in want.items()}
+    labels = Ints(np.concatenate([[5], y]))
+    for workspace in (0, 1):
+        linear_cross_entropy(held["x"].ptr + es, held["w"].ptr + es, held["b"].ptr + es, labels.ptr + 4, M, K, V,
+                             **{k: r.ptr + es for k, r in out.items()}, dtype=dt, workspace_bytes=workspace)
+        be.Sync()
+        got = {}
+        for k, r in out.items():
+            v = r.host()
+            n = want[k].size
+            assert v[0] == 7 and (v[1 + n:] == 7).all(), k
+            got[k] = v[1:1 + n].reshape(want[k].shape)
+        compare(got, want, tol)
+
+
+def test_two_contexts_at_once():
+    """Two contexts of one device (two streams) run calls at the same time; each gets its own results."""
+    be = cuda_backend()
+    lib = be.lib
+    other = ctypes.c_void_p()
+    check(lib.gt_init(0, ctypes.byref(other)))
+    try:
+        heads = [Head(*inputs(500, 128, 3000, 40 + i, 0, ignored=0.3 * i), 0) for i in range(2)]
+        alone = [h.call().host() for h in heads]
+        be.Sync()
+        for _ in range(10):
+            for h, ctx in zip(heads, (be.ctx.ptr, other)):
+                o = h.out
+                check(lib.gt_linear_xent_fwd_bwd(ctx, 0, h.x.ptr, h.w.ptr, h.b.ptr, h.y.ptr, h.M, h.K, h.V, IGN, 0,
+                                                 o["loss"].ptr, o["rows"].ptr, o["dx"].ptr, o["dw"].ptr, o["db"].ptr, None))
+        check(lib.gt_sync(other))
+        be.Sync()
+        for h, want in zip(heads, alone):
+            got = h.host()
+            for k in got:
+                assert np.array_equal(got[k], want[k]), k
+    finally:
+        check(lib.gt_destroy(other))
 
 
 def test_timed_out_wait_returns_an_error_and_the_context_recovers():
