@@ -6,23 +6,26 @@
 // tensor-core path does, moves 12 more bytes per value, and its 256-row tiles
 // are mostly empty. So the products run on the FP32 pipe from w as it is:
 //
-//   few_logits_kernel  a block per strip of 64 classes: z for all rows, the
-//                      strip's maximum and sum of exponentials per row
+//   few_logits_kernel  a block per strip of classes: z for all rows, the strip's
+//                      maximum and sum of exponentials per row
 //   few_join_kernel    one block: the strips joined, the rows' losses, the loss
-//   few_grad_kernel    a block per 128 columns of w and run of classes: G from
+//   few_grad_kernel    a block per columns of w and run of classes: G from
 //                      z on the fly, dw (finished: all rows are here), a
 //                      partial dx, and db
-//   few_dx_kernel      the partial dx of the runs, added in order
+//   few_dx_kernel      the partial dx of the runs, added up
+// (few8_logits_kernel and few8_grad_kernel for at most 8 rows)
 //
 // Sums are float32 in runs of at most 256 (logits) or 1024 (dx) terms that are
 // then added up, so they stay as exact as the tensor-core path's.
 //
-// Measured (the tensor-core path in brackets): 7 x 96 x 517 26 us (71), 64 x 128
-// x 1000 46 us (92), 64 x 512 x 5000 105 us (103), 8 x 2048 x 50000 489 us (598),
-// 16 x 2048 x 50000 674 us (583): it is bound by shared-memory reads there, so
-// the choice goes by the products' size (few_rows).
+// Measured (the tensor-core path in brackets): 7 x 96 x 517 17 us (62), 64 x 128 x
+// 1000 39 us (82), 64 x 512 x 5000 105 us (103), 8 x 2048 x 50000 395 us (600; w read
+// twice and dw written once take 190 at HBM rate), 16 x 2048 x 50000 674 us (583): it
+// is bound by shared-memory reads there, so the choice goes by the products'
+// size (few_rows).
 #include <algorithm>
 
+#include "f32x2.cuh"
 #include "linear_xent.cuh"
 
 namespace gt {
@@ -37,7 +40,113 @@ struct FewMeta {
   float inv_n;  // 0 when no row counts
 };
 
-// MT: rows rounded up to 8, 16, 32 or 64. A thread has the classes tv + TV i
+// At most 8 rows. A warp has 4 classes, whose rows of w go straight to its
+// registers one step of K ahead, its lanes sharing out K; x comes from shared
+// memory once for the 4 classes. (From tiles of both in shared memory, as below,
+// its reads bounded the call: 216 us at 8 x 2048 x 50000.)
+constexpr int kEight = 8;
+constexpr int kEightStrip = 32;    // classes per block
+constexpr int kEightChunk = 1024;  // K per stage of x
+__global__ void __launch_bounds__(256, 2) few8_logits_kernel(const float* __restrict__ x, const float* __restrict__ w,
+                                                             const float* __restrict__ bias,
+                                                             const int32_t* __restrict__ labels, int M, int64_t K,
+                                                             int64_t V, int32_t ignore, float* __restrict__ z,
+                                                             int64_t Vp, float2* __restrict__ strips,
+                                                             float* __restrict__ picked) {
+  __shared__ __align__(16) float xs[kEight][kEightChunk];
+  __shared__ float zs[kEight][kEightStrip + 1];
+  __shared__ bool keep[kEight];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t v0 = (int64_t)blockIdx.x * kEightStrip, mine = v0 + 4 * warp;
+  if (tid < kEight) keep[tid] = tid < M && labels[tid] != ignore;
+  // A lane's four values of a step: 4 lane .. + 3 where rows of w are 16-byte
+  // aligned, else lane + 32 j.
+  const bool vec = ((K & 3) | ((uintptr_t)w & 15)) == 0;
+  const float* row[4];
+#pragma unroll
+  for (int c = 0; c < 4; c++) row[c] = w + min(mine + c, V - 1) * K;
+  float4 next[4];
+  auto fetch = [&](int64_t k) {  // the step at k
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      next[c] = float4{0.f, 0.f, 0.f, 0.f};
+      if (vec) {
+        if (k + 4 * lane < K) next[c] = __ldg(reinterpret_cast<const float4*>(row[c] + k + 4 * lane));
+      } else {
+        if (k + lane < K) next[c].x = __ldg(row[c] + k + lane);
+        if (k + lane + 32 < K) next[c].y = __ldg(row[c] + k + lane + 32);
+        if (k + lane + 64 < K) next[c].z = __ldg(row[c] + k + lane + 64);
+        if (k + lane + 96 < K) next[c].w = __ldg(row[c] + k + lane + 96);
+      }
+    }
+  };
+  float acc[32];  // [class][row]
+#pragma unroll
+  for (int i = 0; i < 32; i++) acc[i] = 0.0f;
+  fetch(0);
+  for (int64_t k0 = 0; k0 < K; k0 += kEightChunk) {
+    __syncthreads();
+    for (int i = tid; i < kEight * kEightChunk; i += 256) {
+      const int m = i / kEightChunk, k = i % kEightChunk;
+      xs[m][k] = keep[m] && k0 + k < K ? __ldg(x + m * K + k0 + k) : 0.0f;
+    }
+    __syncthreads();
+    const int left = (int)min((int64_t)kEightChunk, K - k0);
+#pragma unroll 1
+    for (int k = 0; k < left; k += 128) {
+      float4 a[4];
+#pragma unroll
+      for (int c = 0; c < 4; c++) a[c] = next[c];
+      fetch(k0 + k + 128);
+#pragma unroll
+      for (int m = 0; m < kEight; m++) {
+        float4 b;
+        if (vec)
+          b = *reinterpret_cast<const float4*>(&xs[m][k + 4 * lane]);
+        else
+          b = make_float4(xs[m][k + lane], xs[m][k + lane + 32], xs[m][k + lane + 64], xs[m][k + lane + 96]);
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+          acc[c * kEight + m] =
+              fmaf(a[c].w, b.w, fmaf(a[c].z, b.z, fmaf(a[c].y, b.y, fmaf(a[c].x, b.x, acc[c * kEight + m]))));
+      }
+    }
+  }
+  // The 32 sums over the lanes by halving exchanges: lane l ends with sum l.
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    const bool up = lane & off;
+#pragma unroll
+    for (int j = 0; j < off; j++) {
+      const float keep_v = up ? acc[j + off] : acc[j], send = up ? acc[j] : acc[j + off];
+      acc[j] = keep_v + __shfl_xor_sync(0xffffffffu, send, off);
+    }
+  }
+  {
+    const int c = lane / kEight, m = lane % kEight;
+    const int64_t v = mine + c;
+    zs[m][4 * warp + c] = v < V ? acc[0] + (bias ? __ldg(bias + v) : 0.0f) : -INFINITY;
+  }
+  __syncthreads();
+  if (warp < M) {
+    const int m = warp;
+    const float a = zs[m][lane];
+    float top = a;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    float sum = expf(a - (top == -INFINITY ? 0.0f : top));
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (lane == 0) {
+      strips[(int64_t)blockIdx.x * kEight + m] = make_float2(top, sum);
+      const int64_t at = (int64_t)labels[m] - v0;
+      if (at >= 0 && at < kEightStrip && v0 + at < V) picked[m] = zs[m][at];
+    }
+    if (z && v0 + lane < V) z[m * Vp + v0 + lane] = a;
+  }
+}
+
+// More rows (MT: rounded up to 16, 32 or 64). A thread has the classes tv + TV i
 // and the rows tm + TM j.
 template <int MT>
 __global__ void __launch_bounds__(256) few_logits_kernel(const float* __restrict__ x, const float* __restrict__ w,
@@ -45,7 +154,7 @@ __global__ void __launch_bounds__(256) few_logits_kernel(const float* __restrict
                                                          const int32_t* __restrict__ labels, int M, int64_t K,
                                                          int64_t V, int32_t ignore, float* __restrict__ z, int64_t Vp,
                                                          float2* __restrict__ strips, float* __restrict__ picked) {
-  constexpr int TV = MT >= 16 ? 16 : 32, TM = 256 / TV, VI = kFewStrip / TV, MJ = MT / TM;
+  constexpr int TV = 16, TM = 16, VI = kFewStrip / TV, MJ = MT / TM;
   __shared__ __align__(16) float buf[2 * (kFewStrip + MT) * kFewPitch];
   auto ws = reinterpret_cast<float (*)[kFewStrip][kFewPitch]>(buf);
   auto xs = reinterpret_cast<float (*)[MT][kFewPitch]>(buf + 2 * kFewStrip * kFewPitch);
@@ -183,6 +292,120 @@ __global__ void __launch_bounds__(1024) few_join_kernel(const float2* strips, in
   }
 }
 
+// At most 8 rows: block (kb, run) has the columns 64 kb .. and the classes [run *
+// per, + per). A warp has 8 classes of a step of 64, a lane the columns lane and
+// lane + 32 of all of them, packed: x and the warp's part of dx stay in
+// registers, a value of w goes from memory to a register that both products
+// use and that is refilled for the next step at once, and only n G (twice, as a
+// pair) comes from shared memory, one address for the whole warp.
+constexpr int kEightCols = 64, kEightStep = 64;
+__global__ void __launch_bounds__(256, 2) few8_grad_kernel(const float* __restrict__ x, const float* __restrict__ w,
+                                                           const float* z, int64_t Vp, const float2* stat,
+                                                           const int32_t* __restrict__ labels, int M, int64_t K,
+                                                           int64_t V, int32_t ignore, int64_t per, const FewMeta* meta,
+                                                           float* dw, float* db, float* dx_part) {
+  after_predecessor();
+  __shared__ __align__(16) F2 gs[2][kEightStep][kEight];
+  __shared__ float parts[8][kEight][kEightCols];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t k0 = (int64_t)blockIdx.x * kEightCols + lane;
+  const bool in0 = k0 < K, in1 = k0 + 32 < K;
+  const int64_t va = (int64_t)blockIdx.y * per;
+  const int n = (int)(min(va + per, V) - va);  // classes of the run
+  const float inv_n = meta->inv_n;
+  F2 xr[kEight], acc[kEight];
+  float w0[8], w1[8];
+#pragma unroll
+  for (int m = 0; m < kEight; m++) {
+    const bool keep = m < M && labels[m] != ignore;
+    xr[m] = f2(keep && in0 ? __ldg(x + m * K + k0) : 0.0f, keep && in1 ? __ldg(x + m * K + k0 + 32) : 0.0f);
+    acc[m] = both(0.0f);
+  }
+  const float* wp = w + (va + 8 * warp) * K + k0;
+  float* dp = dw ? dw + (va + 8 * warp) * K + k0 : nullptr;
+  auto fetch = [&](int at, int c) {  // class c of the warp's in the step at `at`
+    const bool live = dx_part && at + 8 * warp + c < n;
+    const float* r = wp + (int64_t)(at + c) * K;
+    w0[c] = live && in0 ? __ldg(r) : 0.0f, w1[c] = live && in1 ? __ldg(r + 32) : 0.0f;
+  };
+  // n G: a thread has the class zc of a step for the rows zm and zm + 4
+  const int zc = tid & 63, zm = tid >> 6;
+  float zr[2], top[2], inv[2];
+  int y[2];
+  auto fetch_z = [&](int at) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) zr[u] = zm + 4 * u < M && at + zc < n ? z[(zm + 4 * u) * Vp + va + at + zc] : 0.0f;
+  };
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    const int m = zm + 4 * u;
+    const float2 s = m < M ? stat[m] : make_float2(0.0f, 0.0f);
+    top[u] = s.x, inv[u] = s.y;
+    const int64_t label = m < M ? (int64_t)labels[m] - va : -1;
+    y[u] = label >= 0 && label < n ? (int)label : -1;  // in the run
+  }
+#pragma unroll
+  for (int c = 0; c < 8; c++) fetch(0, c);
+  fetch_z(0);
+  int b = 0;
+#pragma unroll 1
+  for (int at = 0; at < n; at += kEightStep, b ^= 1) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      float g = 0.0f;
+      if (inv[u] != 0.0f && at + zc < n) g = expf(zr[u] - top[u]) * inv[u] - (y[u] == at + zc ? 1.0f : 0.0f);
+      gs[b][zc][zm + 4 * u] = both(g);
+    }
+    fetch_z(at + kEightStep);
+    __syncthreads();  // (the other buffer's readers are a barrier behind by now)
+#pragma unroll
+    for (int c = 0; c < 8; c++) {
+      F2 d = both(0.0f);
+      const F2 wv = f2(w0[c], w1[c]);
+      float sum = 0.0f;
+#pragma unroll
+      for (int m = 0; m < kEight; m++) {
+        const F2 g = gs[b][8 * warp + c][m];
+        d = fma2(g, xr[m], d);
+        acc[m] = fma2(g, wv, acc[m]);
+        if (db && blockIdx.x == 0) {
+          float lo, hi;
+          unpack(g, lo, hi);
+          sum += lo;
+        }
+      }
+      const int v = at + 8 * warp + c;
+      fetch(at + kEightStep, c);  // on its way while the others are computed
+      if (v >= n) continue;
+      if (dp) {
+        float lo, hi;
+        unpack(d * both(inv_n), lo, hi);
+        float* o = dp + (int64_t)(at + c) * K;
+        if (in0) o[0] = lo;
+        if (in1) o[32] = hi;
+      }
+      if (db && blockIdx.x == 0 && lane == 0) db[va + v] = sum * inv_n;
+    }
+  }
+  if (!dx_part) return;
+#pragma unroll
+  for (int m = 0; m < kEight; m++) {
+    float lo, hi;
+    unpack(acc[m], lo, hi);
+    parts[warp][m][lane] = lo, parts[warp][m][lane + 32] = hi;
+  }
+  __syncthreads();
+  for (int i = tid; i < kEight * kEightCols; i += 256) {
+    const int m = i / kEightCols, c = i % kEightCols;
+    const int64_t k = (int64_t)blockIdx.x * kEightCols + c;
+    if (m >= M || k >= K) continue;
+    float s = parts[0][m][c];
+#pragma unroll
+    for (int u = 1; u < 8; u++) s += parts[u][m][c];
+    dx_part[((int64_t)blockIdx.y * M + m) * K + k] = s;
+  }
+}
+
 template <int MT>
 struct FewShared {
   float w[kFewClasses][kFewCols];
@@ -311,26 +534,39 @@ __global__ void __launch_bounds__(256) few_grad_kernel(const float* __restrict__
   }
 }
 
-__global__ void __launch_bounds__(256) few_dx_kernel(const float* part, int runs, int64_t n,
-                                                     const FewMeta* meta, float* dx) {
+// dx = the runs' partials, added by 8 warps (warp w the runs w, w + 8, ... in
+// order, then the warps' sums in order), 32 values per block.
+__global__ void __launch_bounds__(256) few_dx_kernel(const float* part, int runs, int64_t n, const FewMeta* meta,
+                                                     float* dx) {
   after_predecessor();
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  float s = part[i];
+  __shared__ float ws[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t i = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.0f;
+  if (i < n) {
 #pragma unroll 8
-  for (int r = 1; r < runs; r++) s += part[r * n + i];
+    for (int r = warp; r < runs; r += 8) s += part[r * n + i];
+  }
+  ws[warp][lane] = s;
+  __syncthreads();
+  if (warp != 0 || i >= n) return;
+#pragma unroll
+  for (int u = 1; u < 8; u++) s += ws[u][lane];
   dx[i] = s * meta->inv_n;
 }
 
 template <int MT>
 static char* few_run(gt_ctx* ctx, const XentCall<float>& c, void** held) {
   const bool grad = c.dx || c.dw || c.db;
-  const int64_t strips = ceil_div(c.V, kFewStrip), Vp = ceil_div(c.V, 8) * 8;
-  // Runs of classes: enough blocks for four on every SM, at most 1024 classes
-  // (the longest plain sum of dx).
-  const int64_t kb = c.dx || c.dw ? ceil_div(c.K, kFewCols) : 1, steps = ceil_div(c.V, kFewClasses);
-  const int64_t runs0 = std::min(steps, std::max<int64_t>(ceil_div(4 * (int64_t)ctx->sm_count, kb), ceil_div(steps, 32)));
-  const int64_t per = ceil_div(steps, runs0) * kFewClasses, runs = ceil_div(c.V, per);
+  const int64_t strips = ceil_div(c.V, MT == kEight ? kEightStrip : kFewStrip), Vp = ceil_div(c.V, 8) * 8;
+  // Runs of classes: whole rounds of blocks (2 or more are resident on every SM), at most 1024 classes
+  // (the longest plain sum of dx; 4096 where a warp adds an eighth of them).
+  constexpr bool eight = MT == kEight;
+  const int64_t kb = c.dx || c.dw ? ceil_div(c.K, eight ? kEightCols : kFewCols) : 1;
+  const int64_t step = eight ? kEightStep : kFewClasses, steps = ceil_div(c.V, step);
+  const int64_t runs0 = std::min(steps, std::max<int64_t>((eight ? 6 : 4) * (int64_t)ctx->sm_count / kb,
+                                                          std::max<int64_t>(1, ceil_div(c.V, eight ? 4096 : 1024))));
+  const int64_t per = ceil_div(steps, runs0) * step, runs = ceil_div(c.V, per);
   struct {
     FewMeta* meta;
     float *z, *picked, *part;
@@ -349,24 +585,35 @@ static char* few_run(gt_ctx* ctx, const XentCall<float>& c, void** held) {
   GT_TRY(scratch(ctx, (size_t)size.used, &held[0]));
   Carver at{(char*)held[0]};
   carve(at);
-  few_logits_kernel<MT><<<(unsigned)strips, 256, 0, ctx->stream>>>(c.x, c.w, c.bias, c.labels, (int)c.M, c.K, c.V,
-                                                                     c.ignore, grad ? ws.z : nullptr, Vp, ws.strips,
-                                                                     ws.picked);
+  if constexpr (eight)
+    few8_logits_kernel<<<(unsigned)strips, 256, 0, ctx->stream>>>(c.x, c.w, c.bias, c.labels, (int)c.M, c.K, c.V,
+                                                                  c.ignore, grad ? ws.z : nullptr, Vp, ws.strips,
+                                                                  ws.picked);
+  else
+    few_logits_kernel<MT><<<(unsigned)strips, 256, 0, ctx->stream>>>(c.x, c.w, c.bias, c.labels, (int)c.M, c.K, c.V,
+                                                                       c.ignore, grad ? ws.z : nullptr, Vp, ws.strips,
+                                                                       ws.picked);
   GT_LAUNCH_CHECK();
   GT_CUDA(launch_overlapped(ctx, few_join_kernel<MT>, 1, 1024, 0, ws.strips, (int)strips, (int)c.M, c.labels, c.V,
                             c.ignore, ws.picked, ws.stat, c.rows, c.loss, ws.meta, c.bad));
   if (!grad) return nullptr;
-  static bool configured[64] = {};
-  if (ctx->device < 0 || ctx->device >= 64 || !configured[ctx->device]) {
-    GT_CUDA(cudaFuncSetAttribute(few_grad_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)sizeof(FewShared<MT>)));
-    if (ctx->device >= 0 && ctx->device < 64) configured[ctx->device] = true;
+  const dim3 grid((unsigned)kb, (unsigned)runs);
+  if constexpr (eight) {
+    GT_CUDA(launch_overlapped(ctx, few8_grad_kernel, grid, 256, 0, c.x, c.w, ws.z, Vp, ws.stat, c.labels, (int)c.M, c.K,
+                              c.V, c.ignore, per, ws.meta, c.dw, c.db, c.dx ? ws.part : nullptr));
+  } else {
+    static bool configured[64] = {};
+    if (ctx->device < 0 || ctx->device >= 64 || !configured[ctx->device]) {
+      GT_CUDA(cudaFuncSetAttribute(few_grad_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)sizeof(FewShared<MT>)));
+      if (ctx->device >= 0 && ctx->device < 64) configured[ctx->device] = true;
+    }
+    GT_CUDA(launch_overlapped(ctx, few_grad_kernel<MT>, grid, 256, sizeof(FewShared<MT>),
+                              c.x, c.w, ws.z, Vp, ws.stat, c.labels, (int)c.M, c.K, c.V, c.ignore, per, ws.meta, c.dw,
+                              c.db, c.dx ? ws.part : nullptr, ((c.K & 3) | ((uintptr_t)c.dw & 15)) == 0));
   }
-  GT_CUDA(launch_overlapped(ctx, few_grad_kernel<MT>, dim3((unsigned)kb, (unsigned)runs), 256, sizeof(FewShared<MT>),
-                            c.x, c.w, ws.z, Vp, ws.stat, c.labels, (int)c.M, c.K, c.V, c.ignore, per, ws.meta, c.dw,
-                            c.db, c.dx ? ws.part : nullptr, ((c.K & 3) | ((uintptr_t)c.dw & 15)) == 0));
   if (c.dx)
-    GT_CUDA(launch_overlapped(ctx, few_dx_kernel, (unsigned)ceil_div(c.M * c.K, 256), 256, 0, ws.part, (int)runs,
+    GT_CUDA(launch_overlapped(ctx, few_dx_kernel, (unsigned)ceil_div(c.M * c.K, 32), 256, 0, ws.part, (int)runs,
                               c.M * c.K, ws.meta, c.dx));
   return nullptr;
 }
