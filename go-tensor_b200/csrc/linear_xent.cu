@@ -67,20 +67,29 @@ __global__ void keep_rows_kernel(const double* __restrict__ x, const int32_t* __
     out[i] = labels[i / K] == ignore ? 0.0 : x[i];
 }
 
-// Joins two running (maximum, sum of exp(z - maximum)) pairs.
-__device__ __forceinline__ void join(double& m, double& s, double m2, double s2) {
-  const double top = go_max(m, m2);
-  s = (m == top ? s : s * exp(m - top)) + (m2 == top ? s2 : s2 * exp(m2 - top));
-  m = top;
+__device__ __forceinline__ double block_reduce(double v, double* ws, bool sum) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    const double o = __shfl_xor_sync(0xffffffffu, v, off);
+    v = sum ? v + o : go_max(v, o);
+  }
+  if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = ws[0];
+  for (int w = 1; w < 8; w++) v = sum ? v + ws[w] : go_max(v, ws[w]);
+  __syncthreads();
+  return v;
 }
 
-// A block per row: the running maximum and sum in one pass over the row, then
-// the gradient in place.
+// A block per row: its maximum, then each exponential once (kept in place of z,
+// from L2: a running maximum and sum in one pass needs every exponential
+// twice, and the whole call at 512 x 512 x 8192 took 705 us against 690; this
+// kernel 41), then the gradient in place.
 __global__ void __launch_bounds__(256) xent_piece_f64_kernel(double* __restrict__ z, const int32_t* __restrict__ labels,
-                                                         int64_t rows, int64_t V, int32_t ignore,
-                                                         const int64_t* __restrict__ counts, double* __restrict__ row_loss,
-                                                         bool grad) {
-  __shared__ double wm[8], wsum[8];
+                                                             int64_t rows, int64_t V, int32_t ignore,
+                                                             const int64_t* __restrict__ counts,
+                                                             double* __restrict__ row_loss, bool grad) {
+  __shared__ double ws[8];
   const double inv = 1.0 / (double)counts[0];
   for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
     double* zr = z + i * V;
@@ -91,35 +100,29 @@ __global__ void __launch_bounds__(256) xent_piece_f64_kernel(double* __restrict_
         for (int64_t j = threadIdx.x; j < V; j += blockDim.x) zr[j] = 0.0;
       continue;
     }
-    double m = -INFINITY, s = 0.0;
-    for (int64_t j = threadIdx.x; j < V; j += blockDim.x) {
-      const double v = zr[j];
-      if (v > m) {
-        s = s * exp(m - v) + 1.0;
-        m = v;
-      } else if (v != -INFINITY) {  // (a NaN comes here too)
-        s += exp(v - m);
-      }
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      const double m2 = __shfl_xor_sync(0xffffffffu, m, off), s2 = __shfl_xor_sync(0xffffffffu, s, off);
-      join(m, s, m2, s2);
-    }
-    if ((threadIdx.x & 31) == 0) wm[threadIdx.x >> 5] = m, wsum[threadIdx.x >> 5] = s;
-    __syncthreads();
-    m = wm[0], s = wsum[0];
-    for (int w = 1; w < 8; w++) join(m, s, wm[w], wsum[w]);
+    double m = -INFINITY;
+#pragma unroll 4
+    for (int64_t j = threadIdx.x; j < V; j += blockDim.x) m = go_max(m, zr[j]);
+    m = block_reduce(m, ws, false);
     const bool bad = y < 0 || y >= V;
-    if (threadIdx.x == 0) row_loss[i] = bad ? (double)NAN : log(s) + (m - zr[y]);
-    __syncthreads();  // the label's logit is read, and wm / wsum are free
-    if (grad)
+    const double picked = bad ? (double)NAN : zr[y];
+    __syncthreads();  // every thread has read it
+    double s = 0.0;
+#pragma unroll 4
+    for (int64_t j = threadIdx.x; j < V; j += blockDim.x) {
       // (not exp(z - lse): the logarithm would vanish beside a maximum that is
       // a mask's lowest value)
-      for (int64_t j = threadIdx.x; j < V; j += blockDim.x) {
-        const double e = exp(zr[j] - m) / s * inv;
-        zr[j] = j == y ? e - inv : e;
-      }
+      const double e = exp(zr[j] - m);
+      s += e;
+      if (grad) zr[j] = e;
+    }
+    s = block_reduce(s, ws, true);
+    if (threadIdx.x == 0) row_loss[i] = log(s) + (m - picked);
+    if (grad) {
+      const double f = inv / s;
+#pragma unroll 4
+      for (int64_t j = threadIdx.x; j < V; j += blockDim.x) zr[j] = j == y ? zr[j] * f - inv : zr[j] * f;
+    }
   }
 }
 
