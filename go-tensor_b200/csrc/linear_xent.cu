@@ -67,6 +67,15 @@ __global__ void keep_rows_kernel(const double* __restrict__ x, const int32_t* __
     out[i] = labels[i / K] == ignore ? 0.0 : x[i];
 }
 
+// The ignored rows of dx are 0 whatever w holds (0 times an infinity is not): a
+// warp per row.
+__global__ void __launch_bounds__(256) zero_rows_kernel(const int32_t* __restrict__ labels, int64_t M, int64_t K,
+                                                        int32_t ignore, double* __restrict__ dx) {
+  for (int64_t m = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); m < M; m += (int64_t)gridDim.x * 8)
+    if (labels[m] == ignore)
+      for (int64_t k = threadIdx.x & 31; k < K; k += 32) dx[m * K + k] = 0.0;
+}
+
 __device__ __forceinline__ double block_reduce(double v, double* ws, bool sum) {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
@@ -611,6 +620,10 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
       piece_columns_kernel<<<(unsigned)ceil_div(c.V, 32), 1024, 0, ctx->stream>>>(z, r, c.V, r0 == 0, c.db);
       GT_LAUNCH_CHECK();
     }
+  }
+  if (c.dx) {
+    zero_rows_kernel<<<grid_for(ctx, c.M, 8), 256, 0, ctx->stream>>>(c.labels, c.M, c.K, c.ignore, c.dx);
+    GT_LAUNCH_CHECK();
   }
   mean_rows_kernel<double><<<1, 1024, 0, ctx->stream>>>(rows, c.M, false, counts, c.loss);
   GT_LAUNCH_CHECK();

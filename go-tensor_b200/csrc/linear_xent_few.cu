@@ -535,9 +535,10 @@ __global__ void __launch_bounds__(256) few_grad_kernel(const float* __restrict__
 }
 
 // dx = the runs' partials, added by 8 warps (warp w the runs w, w + 8, ... in
-// order, then the warps' sums in order), 32 values per block.
-__global__ void __launch_bounds__(256) few_dx_kernel(const float* part, int runs, int64_t n, const FewMeta* meta,
-                                                     float* dx) {
+// order, then the warps' sums in order), 32 values per block. An ignored row's
+// is 0 whatever w holds (0 times an infinity in the partials is not).
+__global__ void __launch_bounds__(256) few_dx_kernel(const float* part, int runs, int64_t n, int64_t K,
+                                                     const float2* stat, const FewMeta* meta, float* dx) {
   after_predecessor();
   __shared__ float ws[8][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -552,7 +553,7 @@ __global__ void __launch_bounds__(256) few_dx_kernel(const float* part, int runs
   if (warp != 0 || i >= n) return;
 #pragma unroll
   for (int u = 1; u < 8; u++) s += ws[u][lane];
-  dx[i] = s * meta->inv_n;
+  dx[i] = stat[i / K].y == 0.0f ? 0.0f : s * meta->inv_n;
 }
 
 template <int MT>
@@ -614,7 +615,7 @@ static char* few_run(gt_ctx* ctx, const XentCall<float>& c, void** held) {
   }
   if (c.dx)
     GT_CUDA(launch_overlapped(ctx, few_dx_kernel, (unsigned)ceil_div(c.M * c.K, 32), 256, 0, ws.part, (int)runs,
-                              c.M * c.K, ws.meta, c.dx));
+                              c.M * c.K, c.K, ws.stat, ws.meta, c.dx));
   return nullptr;
 }
 

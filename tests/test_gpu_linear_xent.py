@@ -254,6 +254,22 @@ def test_ignored_rows_may_hold_anything(dt):
         assert np.array_equal(got[k], clean[k]), k
 
 
+@pytest.mark.parametrize("value", [np.inf, np.nan])
+@pytest.mark.parametrize("dt,M,K,V", [(0, 6, 70, 517), (0, 20, 70, 517), (0, 60, 33, 517), (0, 300, 70, 2049),
+                                      (1, 6, 70, 517), (1, 150, 33, 517)])
+def test_ignored_rows_beside_a_weight_that_is_not_finite(dt, M, K, V, value):
+    """They take no part, so their dx and loss stay 0; the rows that count carry the weight's NaN."""
+    x, w, b, y = inputs(M, K, V, M, dt)
+    y[1::2] = IGN
+    w[V // 3, K // 2] = value
+    got = Head(x, w, b, y, dt).call().host()
+    assert (got["dx"][1::2] == 0).all() and (got["rows"][1::2] == 0).all()
+    assert np.isnan(got["dx"][0::2, K // 2]).all()
+    got = Head(x, w, b, np.full(M, IGN), dt).call().host()
+    for k in ("rows", "dx", "dw", "db"):
+        assert (got[k] == 0).all(), k
+
+
 @pytest.mark.parametrize("M,V,workspace", [(700, 2049, 1), (1500, 9000, 16 << 20), (1100, 20011, 0), (300, 260, 0)])
 @pytest.mark.parametrize("which", ["half", "most", "first", "last", "one", "all but one", "a piece"])
 def test_rows_that_count_anywhere(M, V, workspace, which):
