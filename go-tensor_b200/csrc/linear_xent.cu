@@ -25,160 +25,14 @@
 //     split_gemm         dx = G w, dw (+)= G^T x
 //   mean_rows_kernel     the loss
 //
-// float64 runs the same pieces over the FP64 GEMM.
+// float64: linear_xent_f64.cu.
 #include <algorithm>
 #include <cmath>
 
-#include "gemm.cuh"
 #include "linear_xent.cuh"
 #include "split_gemm.cuh"
 
 namespace gt {
-
-// counts[0] = rows that count (label != ignore); a label outside [0, V) sets *bad.
-__global__ void __launch_bounds__(1024) label_count_kernel(const int32_t* __restrict__ labels, int64_t M, int64_t V,
-                                                           int32_t ignore, int64_t* counts, int32_t* bad) {
-  __shared__ int64_t ws[32];
-  int64_t n = 0;
-  bool outside = false;
-  for (int64_t i = threadIdx.x; i < M; i += blockDim.x) {
-    const int32_t y = labels[i];
-    if (y != ignore) {
-      n++;
-      outside |= y < 0 || y >= V;
-    }
-  }
-  if (outside && bad) *bad = 1;
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
-  if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = n;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    n = 0;
-    for (int w = 0; w < 32; w++) n += ws[w];
-    counts[0] = n;
-  }
-}
-
-// out = x with the ignored rows zeroed (padding may hold anything).
-__global__ void keep_rows_kernel(const double* __restrict__ x, const int32_t* __restrict__ labels, int64_t rows, int64_t K,
-                                 int32_t ignore, double* __restrict__ out) {
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < rows * K; i += (int64_t)gridDim.x * blockDim.x)
-    out[i] = labels[i / K] == ignore ? 0.0 : x[i];
-}
-
-// The ignored rows of dx are 0 whatever w holds (0 times an infinity is not): a
-// warp per row.
-__global__ void __launch_bounds__(256) zero_rows_kernel(const int32_t* __restrict__ labels, int64_t M, int64_t K,
-                                                        int32_t ignore, double* __restrict__ dx) {
-  for (int64_t m = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); m < M; m += (int64_t)gridDim.x * 8)
-    if (labels[m] == ignore)
-      for (int64_t k = threadIdx.x & 31; k < K; k += 32) dx[m * K + k] = 0.0;
-}
-
-__device__ __forceinline__ double block_reduce(double v, double* ws, bool sum) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    const double o = __shfl_xor_sync(0xffffffffu, v, off);
-    v = sum ? v + o : go_max(v, o);
-  }
-  if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = ws[0];
-  for (int w = 1; w < 8; w++) v = sum ? v + ws[w] : go_max(v, ws[w]);
-  __syncthreads();
-  return v;
-}
-
-// A block per row: its maximum, then each exponential once (kept in place of z,
-// from L2: a running maximum and sum in one pass needs every exponential
-// twice, and the whole call at 512 x 512 x 8192 took 705 us against 690; this
-// kernel 41), then the gradient in place.
-__global__ void __launch_bounds__(256) xent_piece_f64_kernel(double* __restrict__ z, const int32_t* __restrict__ labels,
-                                                             int64_t rows, int64_t V, int32_t ignore,
-                                                             const int64_t* __restrict__ counts,
-                                                             double* __restrict__ row_loss, bool grad) {
-  __shared__ double ws[8];
-  const double inv = 1.0 / (double)counts[0];
-  for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
-    double* zr = z + i * V;
-    const int32_t y = labels[i];
-    if (y == ignore) {
-      if (threadIdx.x == 0) row_loss[i] = 0.0;
-      if (grad)
-        for (int64_t j = threadIdx.x; j < V; j += blockDim.x) zr[j] = 0.0;
-      continue;
-    }
-    double m = -INFINITY;
-#pragma unroll 4
-    for (int64_t j = threadIdx.x; j < V; j += blockDim.x) m = go_max(m, zr[j]);
-    m = block_reduce(m, ws, false);
-    const bool bad = y < 0 || y >= V;
-    const double picked = bad ? (double)NAN : zr[y];
-    __syncthreads();  // every thread has read it
-    double s = 0.0;
-#pragma unroll 4
-    for (int64_t j = threadIdx.x; j < V; j += blockDim.x) {
-      // (not exp(z - lse): the logarithm would vanish beside a maximum that is
-      // a mask's lowest value)
-      const double e = exp(zr[j] - m);
-      s += e;
-      if (grad) zr[j] = e;
-    }
-    s = block_reduce(s, ws, true);
-    if (threadIdx.x == 0) row_loss[i] = log(s) + (m - picked);
-    if (grad) {
-      const double f = inv / s;
-#pragma unroll 4
-      for (int64_t j = threadIdx.x; j < V; j += blockDim.x) zr[j] = j == y ? zr[j] * f - inv : zr[j] * f;
-    }
-  }
-}
-
-// loss = sum of the rows' losses / n, in float64, one block, a fixed order.
-template <typename T>
-__global__ void __launch_bounds__(1024) mean_rows_kernel(const T* rows, int64_t M, bool compact,
-                                                         const int64_t* counts, T* loss) {
-  after_predecessor();
-  __shared__ double part[32];
-  double acc = 0.0;
-  if (compact) M = counts[0];  // only the rows that count are listed
-  for (int64_t i = threadIdx.x; i < M; i += blockDim.x) acc += (double)rows[i];
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = acc;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    acc = 0.0;
-    for (int w = 0; w < 32; w++) acc += part[w];
-    *loss = (T)(acc / (double)counts[0]);
-  }
-}
-
-// db (+)= column sums of a piece's gradient: 32 columns per block, warp w adds
-// the rows w, w + 32, ... in order, then the warps' sums in order.
-__global__ void __launch_bounds__(1024) piece_columns_kernel(const double* __restrict__ g, int64_t rows, int64_t V,
-                                                             bool first, double* __restrict__ db) {
-  __shared__ double ws[32][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
-  double acc = 0.0;
-  if (c < V) {
-#pragma unroll 4
-    for (int64_t i = warp; i < rows; i += 32) acc += g[i * V + c];
-  }
-  ws[warp][lane] = acc;
-  __syncthreads();
-  if (warp != 0 || c >= V) return;
-  for (int i = 1; i < 32; i++) acc += ws[i][lane];
-  db[c] = first ? acc : db[c] + acc;
-}
-
-__global__ void add_kernel(double* __restrict__ out, const double* __restrict__ x, int64_t n) {
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
-    out[i] = out[i] + x[i];
-}
-
 
 // What the kernels of one float32 call share: the operands' largest finite
 // magnitudes (as ordered words), the rows that count, and the products' factors.
@@ -566,67 +420,6 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
                                 c.db));
   }
   GT_CUDA(launch_overlapped(ctx, mean_rows_kernel<float>, 1, 1024, 0, ws.losses, c.M, true, &ws.meta->count, c.loss));
-  return nullptr;
-}
-
-// float64: pieces of rows over the FP64 GEMM, one piece's logits in workspace.
-static char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
-  const bool grad = c.dx || c.dw || c.db;
-  int64_t R = std::max<int64_t>(1, c.workspace / (int64_t)(c.V * sizeof(double)));
-  R = std::min(c.M, R >= 128 ? R / 128 * 128 : 128);
-  const int64_t pieces = ceil_div(c.M, R);
-  double *z, *xk, *more = nullptr, *rows = c.rows;
-  int64_t* counts;
-  GT_TRY(scratch(ctx, (size_t)R * c.V * sizeof(double), &held[0]));
-  GT_TRY(scratch(ctx, (size_t)R * c.K * sizeof(double), &held[1]));
-  GT_TRY(scratch(ctx, 64, &held[2]));
-  if (!rows) {
-    GT_TRY(scratch(ctx, (size_t)c.M * sizeof(double), &held[3]));
-    rows = (double*)held[3];
-  }
-  if (c.dw && pieces > 1) {
-    GT_TRY(scratch(ctx, (size_t)c.V * c.K * sizeof(double), &held[4]));
-    more = (double*)held[4];
-  }
-  z = (double*)held[0], xk = (double*)held[1], counts = (int64_t*)held[2];
-  label_count_kernel<<<1, 1024, 0, ctx->stream>>>(c.labels, c.M, c.V, c.ignore, counts, c.bad);
-  GT_LAUNCH_CHECK();
-  for (int64_t r0 = 0; r0 < c.M; r0 += R) {
-    const int64_t r = std::min(R, c.M - r0);
-    keep_rows_kernel<<<grid_for(ctx, r * c.K, 256), 256, 0, ctx->stream>>>(c.x + r0 * c.K, c.labels + r0, r, c.K,
-                                                                               c.ignore, xk);
-    GT_LAUNCH_CHECK();
-    Epi<double> e;
-    e.out = z, e.ldc = c.V, e.bias = c.bias;
-    GT_TRY(gemm<double>(ctx, GemmShape{r, c.V, c.K, false, true, c.K, c.K}, xk, c.w, e));
-    xent_piece_f64_kernel<<<(unsigned)std::min<int64_t>(r, (int64_t)ctx->sm_count * 8), 256, 0, ctx->stream>>>(
-        z, c.labels + r0, r, c.V, c.ignore, counts, rows + r0, grad);
-    GT_LAUNCH_CHECK();
-    if (c.dx) {
-      Epi<double> d;
-      d.out = c.dx + r0 * c.K, d.ldc = c.K;
-      GT_TRY(gemm<double>(ctx, GemmShape{r, c.K, c.V, false, false, c.V, c.K}, z, c.w, d));
-    }
-    if (c.dw) {
-      Epi<double> d;
-      d.out = r0 ? more : c.dw, d.ldc = c.K;
-      GT_TRY(gemm<double>(ctx, GemmShape{c.V, c.K, r, true, false, c.V, c.K}, z, xk, d));
-      if (r0) {
-        add_kernel<<<grid_for(ctx, c.V * c.K, 256), 256, 0, ctx->stream>>>(c.dw, more, c.V * c.K);
-        GT_LAUNCH_CHECK();
-      }
-    }
-    if (c.db) {
-      piece_columns_kernel<<<(unsigned)ceil_div(c.V, 32), 1024, 0, ctx->stream>>>(z, r, c.V, r0 == 0, c.db);
-      GT_LAUNCH_CHECK();
-    }
-  }
-  if (c.dx) {
-    zero_rows_kernel<<<grid_for(ctx, c.M, 8), 256, 0, ctx->stream>>>(c.labels, c.M, c.K, c.ignore, c.dx);
-    GT_LAUNCH_CHECK();
-  }
-  mean_rows_kernel<double><<<1, 1024, 0, ctx->stream>>>(rows, c.M, false, counts, c.loss);
-  GT_LAUNCH_CHECK();
   return nullptr;
 }
 

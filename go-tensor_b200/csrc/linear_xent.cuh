@@ -1,4 +1,4 @@
-// What the float32 paths of the large-vocabulary loss share.
+// What the paths of the large-vocabulary loss share.
 #pragma once
 #include "gt_common.cuh"
 
@@ -71,6 +71,26 @@ __device__ __forceinline__ void join(float2& a, const float2 b) {
   a.x = top;
 }
 
+// loss = sum of the rows' losses / n, in float64, one block, a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(1024) mean_rows_kernel(const T* rows, int64_t M, bool compact,
+                                                         const int64_t* counts, T* loss) {
+  after_predecessor();
+  __shared__ double part[32];
+  double acc = 0.0;
+  if (compact) M = counts[0];  // only the rows that count are listed
+  for (int64_t i = threadIdx.x; i < M; i += blockDim.x) acc += (double)rows[i];
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    acc = 0.0;
+    for (int w = 0; w < 32; w++) acc += part[w];
+    *loss = (T)(acc / (double)counts[0]);
+  }
+}
+
 // Calls of few rows (linear_xent_few.cu, at most 64): all with at most 8 rows,
 // and those whose products stay below 2^27 terms, where the tensor-core path's
 // dozen launches and mostly empty tiles cost more. (Its grid holds 2^25 classes.)
@@ -78,5 +98,7 @@ inline bool few_rows(int64_t M, int64_t K, int64_t V) {
   return V <= (int64_t)1 << 25 && (M <= 8 || (M <= 64 && (double)M * (double)K * (double)V <= 134217728.0));
 }
 char* linear_xent_few(gt_ctx* ctx, const XentCall<float>& c, void** held);
+
+char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held);  // linear_xent_f64.cu
 
 }  // namespace gt
