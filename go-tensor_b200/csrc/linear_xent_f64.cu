@@ -6,7 +6,7 @@
 //   per piece:
 //     keep_rows_kernel    x with the ignored rows zeroed, its pitch even
 //     f64_tile_kernel     z = x w^T + b
-//     xent_piece_kernel   the rows' losses, G in place of z
+//     xent_segment_kernel, xent_scale_kernel  the rows' losses, G in place of z
 //     f64_tile_kernel     dx = G w, dw (+)= G^T x
 //     piece_columns_kernel  db
 //   mean_rows_kernel      the loss
@@ -47,15 +47,22 @@ __global__ void __launch_bounds__(1024) label_count_kernel(const int32_t* __rest
   }
 }
 
-// out = x with the ignored rows zeroed (padding may hold anything), a warp per row.
+// out = x with the ignored rows zeroed (padding may hold anything), a warp per
+// 256 values of a row.
 __global__ void __launch_bounds__(256) keep_rows_kernel(const double* __restrict__ x, const int32_t* __restrict__ labels,
                                                         int64_t rows, int64_t K, int64_t Kp, int32_t ignore,
                                                         double* out) {
   after_predecessor();
-  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < rows; i += (int64_t)gridDim.x * 8) {
+  const int64_t across = (K + 255) / 256;
+  for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < rows * across; u += (int64_t)gridDim.x * 8) {
+    const int64_t i = u / across, k0 = (u - i * across) * 256 + (threadIdx.x & 31);
     const bool keep = labels[i] != ignore;
-#pragma unroll 4
-    for (int64_t k = threadIdx.x & 31; k < K; k += 32) out[i * Kp + k] = keep ? x[i * K + k] : 0.0;
+    double v[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = keep && k0 + 32 * j < K ? x[i * K + k0 + 32 * j] : 0.0;
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (k0 + 32 * j < K) out[i * Kp + k0 + 32 * j] = v[j];
   }
 }
 
@@ -68,53 +75,118 @@ __device__ __forceinline__ double block_reduce(double v, double* ws, bool sum) {
   if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = v;
   __syncthreads();
   v = ws[0];
-  for (int w = 1; w < (int)blockDim.x >> 5; w++) v = sum ? v + ws[w] : go_max(v, ws[w]);
+  for (int w = 1; w < 8; w++) v = sum ? v + ws[w] : go_max(v, ws[w]);
   __syncthreads();
   return v;
 }
 
-// A block per row: its maximum, then each exponential once (kept in place of z,
-// from L2: a running maximum and sum in one pass needs every exponential
-// twice, and the whole call at 512 x 512 x 8192 took 15 us more; this kernel
-// 41), then the gradient in place.
-__global__ void __launch_bounds__(512) xent_piece_kernel(double* z, const int32_t* __restrict__ labels, int64_t rows,
-                                                         int64_t V, int64_t Vp, int32_t ignore, const int64_t* counts,
-                                                         double* row_loss, bool grad) {
+// A block per segment of 4096 classes of a row, in registers: the segment's
+// maximum and sum of exponentials. A row of one segment is finished here (z read
+// once, G written once: 8000 x 3000 took 215 us in three passes over a row);
+// of more, e = exp(z - the segment's maximum) is left in place of z for
+// xent_scale_kernel.
+constexpr int kSegment = 4096;
+__global__ void __launch_bounds__(256) xent_segment_kernel(double* z, const int32_t* __restrict__ labels, int64_t V,
+                                                           int64_t Vp, int64_t segments, int32_t ignore,
+                                                           const int64_t* counts, double2* pairs, double* picked,
+                                                           double* row_loss, bool grad) {
   after_predecessor();
-  __shared__ double ws[32];
+  __shared__ double ws[8];
+  const int64_t i = blockIdx.x / segments, seg = blockIdx.x - i * segments;
+  const int32_t y = labels[i];
+  const int64_t n = min((int64_t)kSegment, V - seg * kSegment), at = (int64_t)y - seg * kSegment;
+  double* zr = z + i * Vp + seg * kSegment;
+  auto put = [&](const double(&e)[16]) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int c = 2 * (threadIdx.x + 256 * j);
+      if (c < n) *reinterpret_cast<double2*>(zr + c) = make_double2(e[2 * j], e[2 * j + 1]);  // (the pitch is even)
+    }
+  };
+  double e[16];
+  if (y == ignore) {
+    if (seg == 0 && threadIdx.x == 0) row_loss[i] = 0.0;
+#pragma unroll
+    for (int j = 0; j < 16; j++) e[j] = 0.0;
+    if (grad) put(e);
+    return;
+  }
+  double m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const int c = 2 * (threadIdx.x + 256 * j);
+    double2 v = make_double2(-INFINITY, -INFINITY);
+    if (c < n) v = *reinterpret_cast<const double2*>(zr + c);
+    e[2 * j] = v.x, e[2 * j + 1] = c + 1 < n ? v.y : -INFINITY;
+  }
+#pragma unroll
+  for (int j = 0; j < 16; j++) m = go_max(m, e[j]);
+  m = block_reduce(m, ws, false);
+  const bool outside = y < 0 || y >= V;
+  const double label_z = at >= 0 && at < n && !outside ? zr[at] : (double)NAN;
+  // (from 0 where nothing is above -infinity: the sum is then 0, not NaN)
+  const double from = segments > 1 && m == -INFINITY ? 0.0 : m;
+  double s = 0.0;
+#pragma unroll
+  for (int j = 0; j < 16; j++) {
+    // (not exp(z - lse): the logarithm would vanish beside a maximum that is a
+    // mask's lowest value)
+    const int c = 2 * (threadIdx.x + 256 * (j >> 1)) + (j & 1);
+    e[j] = c < n ? exp(e[j] - from) : 0.0;
+    s += e[j];
+  }
+  s = block_reduce(s, ws, true);  // (every thread has read label_z by now)
+  if (segments > 1) {
+    if (threadIdx.x == 0) {
+      pairs[i * segments + seg] = make_double2(m, s);
+      if (at >= 0 && at < n) picked[i] = label_z;
+    }
+  } else {
+    if (threadIdx.x == 0) row_loss[i] = log(s) + (m - label_z);
+    const double inv = 1.0 / (double)counts[0], f = inv / s;
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+      const int c = 2 * (threadIdx.x + 256 * (j >> 1)) + (j & 1);
+      e[j] = c == at ? e[j] * f - inv : e[j] * f;
+    }
+  }
+  if (grad) put(e);
+}
+
+// Rows of several segments: the pairs joined (by every block of the row), the
+// row's loss, and e -> G.
+__global__ void __launch_bounds__(256) xent_scale_kernel(double* z, const int32_t* __restrict__ labels, int64_t V,
+                                                         int64_t Vp, int64_t segments, int64_t blocks, int32_t ignore,
+                                                         const int64_t* counts, const double2* pairs,
+                                                         const double* picked, double* row_loss, bool grad) {
+  after_predecessor();
+  __shared__ double ws[8];
+  const int64_t i = blockIdx.x / blocks, seg = blockIdx.x - i * blocks;
+  const int32_t y = labels[i];
+  if (y == ignore) return;  // done
+  double m = -INFINITY, s = 0.0;
+  for (int64_t g = threadIdx.x; g < segments; g += 256) m = go_max(m, pairs[i * segments + g].x);
+  m = block_reduce(m, ws, false);
+  const double from = m == -INFINITY ? 0.0 : m;
+  for (int64_t g = threadIdx.x; g < segments; g += 256) {
+    const double2 p = pairs[i * segments + g];
+    s += p.y * exp(p.x - from);
+  }
+  s = block_reduce(s, ws, true);
+  if (seg == 0 && threadIdx.x == 0) row_loss[i] = y < 0 || y >= V ? (double)NAN : log(s) + (m - picked[i]);
+  if (!grad) return;
   const double inv = 1.0 / (double)counts[0];
-  for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
-    double* zr = z + i * Vp;
-    const int32_t y = labels[i];
-    if (y == ignore) {
-      if (threadIdx.x == 0) row_loss[i] = 0.0;
-      if (grad)
-        for (int64_t j = threadIdx.x; j < V; j += blockDim.x) zr[j] = 0.0;
-      continue;
-    }
-    double m = -INFINITY;
-#pragma unroll 4
-    for (int64_t j = threadIdx.x; j < V; j += blockDim.x) m = go_max(m, zr[j]);
-    m = block_reduce(m, ws, false);
-    const bool bad = y < 0 || y >= V;
-    const double picked = bad ? (double)NAN : zr[y];
-    __syncthreads();  // every thread has read it
-    double s = 0.0;
-#pragma unroll 4
-    for (int64_t j = threadIdx.x; j < V; j += blockDim.x) {
-      // (not exp(z - lse): the logarithm would vanish beside a maximum that is
-      // a mask's lowest value)
-      const double e = exp(zr[j] - m);
-      s += e;
-      if (grad) zr[j] = e;
-    }
-    s = block_reduce(s, ws, true);
-    if (threadIdx.x == 0) row_loss[i] = log(s) + (m - picked);
-    if (grad) {
-      const double f = inv / s;
-#pragma unroll 4
-      for (int64_t j = threadIdx.x; j < V; j += blockDim.x) zr[j] = j == y ? zr[j] * f - inv : zr[j] * f;
-    }
+  const double f = exp(pairs[i * segments + seg].x - from) * (inv / s);
+  const int64_t n = min((int64_t)kSegment, V - seg * kSegment), at = (int64_t)y - seg * kSegment;
+  double* zr = z + i * Vp + seg * kSegment;
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const int c = 2 * (threadIdx.x + 256 * j);
+    if (c >= n) continue;
+    double2 v = *reinterpret_cast<const double2*>(zr + c);
+    v.x = c == at ? v.x * f - inv : v.x * f;
+    v.y = c + 1 == at ? v.y * f - inv : v.y * f;
+    *reinterpret_cast<double2*>(zr + c) = v;
   }
 }
 
@@ -382,7 +454,7 @@ __global__ void __launch_bounds__(1024) piece_columns_kernel(const double* g, in
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   double acc = 0.0;
   if (c < V) {
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t i = warp; i < rows; i += 32) acc += g[i * Vp + c];
   }
   ws[warp][lane] = acc;
@@ -399,7 +471,8 @@ char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
   R = std::min(c.M, R >= 128 ? R / 128 * 128 : 128);
   struct {
     int64_t* counts;
-    double *z, *x, *rows, *parts;
+    double *z, *x, *rows, *parts, *picked;
+    double2* pairs;
   } ws{};
   // The products of the piece of r rows at r0, one kind at a time.
   auto logits = [&](int64_t r, int64_t* need) {
@@ -417,6 +490,7 @@ char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
     p.accumulate = r0 > 0;
     return f64_product<false, false>(ctx, p, ws.parts, need);
   };
+  const int64_t segments = ceil_div(c.V, kSegment);
   int64_t need = 0;
   for (const int64_t r : {R, c.M - (c.M - 1) / R * R}) {  // a full piece, the last one
     GT_TRY(logits(r, &need));
@@ -429,6 +503,8 @@ char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
     ws.x = k.take<double>(R * Kp);
     ws.rows = k.take<double>(c.rows ? 0 : c.M);
     ws.parts = k.take<double>(need);
+    ws.pairs = k.take<double2>(segments > 1 ? R * segments : 0);
+    ws.picked = k.take<double>(segments > 1 ? R : 0);
   };
   Carver size{nullptr};
   carve(size);
@@ -441,13 +517,16 @@ char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
   for (int64_t r0 = 0; r0 < c.M; r0 += R) {
     const int64_t r = std::min(R, c.M - r0);
     const int32_t* labels = c.labels + r0;
-    GT_CUDA(launch_overlapped(ctx, keep_rows_kernel, grid_for(ctx, r, 8), 256, 0, c.x + r0 * c.K, labels, r, c.K, Kp,
+    GT_CUDA(launch_overlapped(ctx, keep_rows_kernel, grid_for(ctx, r * ceil_div(c.K, 256), 8), 256, 0, c.x + r0 * c.K, labels, r, c.K, Kp,
                               c.ignore, ws.x));
     GT_TRY(logits(r, nullptr));
-    // few rows: more threads for each
-    GT_CUDA(launch_overlapped(ctx, xent_piece_kernel, (unsigned)std::min<int64_t>(r, (int64_t)ctx->sm_count * 8),
-                              r < 2 * (int64_t)ctx->sm_count ? 512 : 256, 0, ws.z, labels, r, c.V, Vp, c.ignore,
-                              ws.counts, rows + r0, grad));
+    GT_CUDA(launch_overlapped(ctx, xent_segment_kernel, (unsigned)(r * segments), 256, 0, ws.z, labels, c.V, Vp, segments,
+                              c.ignore, ws.counts, ws.pairs, ws.picked, rows + r0, grad));
+    if (segments > 1) {
+      const int64_t blocks = grad ? segments : 1;
+      GT_CUDA(launch_overlapped(ctx, xent_scale_kernel, (unsigned)(r * blocks), 256, 0, ws.z, labels, c.V, Vp, segments,
+                                blocks, c.ignore, ws.counts, ws.pairs, ws.picked, rows + r0, grad));
+    }
     if (c.dx) GT_TRY(dx(r0, r, nullptr));
     if (c.dw) GT_TRY(dw(r0, r, nullptr));
     if (c.db)

@@ -254,6 +254,44 @@ def test_ignored_rows_may_hold_anything(dt):
         assert np.array_equal(got[k], clean[k]), k
 
 
+# Every tile of the float64 products, odd pitches (8-byte copies), K split over the SMs, rows of one and of several
+# segments of 4096 classes, pieces of 128 rows.
+@pytest.mark.parametrize("M,K,V,workspace", [
+    (1, 1, 1, 0), (2, 1, 5000, 0), (3, 70, 20011, 0), (14, 33, 9000, 0), (16, 1000, 257, 0), (20, 100, 4096, 0),
+    (30, 64, 4097, 0), (70, 129, 8193, 0), (142, 407, 3555, 0), (300, 20, 1000, 0), (1000, 40, 300, 0),
+    (777, 17, 5000, 1), (129, 500, 4095, 1), (400, 31, 30, 0), (130, 2000, 2000, 0)])
+@pytest.mark.parametrize("ignored", [0.0, 0.3])
+def test_float64_shapes(M, K, V, workspace, ignored):
+    x, w, b, y = inputs(M, K, V, M + K + V, 1, ignored=ignored)
+    compare(Head(x, w, b, y, 1, workspace_bytes=workspace).call().host(), *reference(x, w, b, y, 1))
+    evaluated = Head(x, w, b, y, 1, outputs=("rows",), workspace_bytes=workspace).call().host()
+    full = Head(x, w, b, y, 1, workspace_bytes=workspace).call().host()
+    for k in evaluated:
+        assert np.array_equal(evaluated[k], full[k], equal_nan=True), k
+
+
+@pytest.mark.parametrize("low", [-np.inf, np.finfo(np.float64).min])
+@pytest.mark.parametrize("segment", [0, 1, 2])
+def test_float64_masked_segment(segment, low):
+    """All 4096 classes that a block has of a row masked: its maximum is the mask's value."""
+    M, K, V = 9, 24, 2 * 4096 + 1000
+    x, w, b, y = inputs(M, K, V, 31, 1)
+    b[segment * 4096:(segment + 1) * 4096] = low
+    y = (segment + 1) % 3 * 4096 + np.arange(M) * 100  # in the segment after it, its first class among them
+    got = Head(x, w, b, y, 1).call().host()
+    compare(got, *reference(x, w, b, y, 1))
+    masked = slice(segment * 4096, (segment + 1) * 4096)
+    assert (got["db"][masked] == 0).all() and (got["dw"][masked] == 0).all()
+
+
+@pytest.mark.parametrize("at", [0, 4095, 4096, 4097, 8191, 8192, 9000])
+def test_float64_label_in_any_segment(at):
+    M, K, V = 5, 24, 9001
+    x, w, b, _ = inputs(M, K, V, 32, 1)
+    y = np.full(M, at)
+    compare(Head(x, w, b, y, 1).call().host(), *reference(x, w, b, y, 1))
+
+
 @pytest.mark.parametrize("value", [np.inf, np.nan])
 @pytest.mark.parametrize("dt,M,K,V", [(0, 6, 70, 517), (0, 20, 70, 517), (0, 60, 33, 517), (0, 300, 70, 2049),
                                       (1, 6, 70, 517), (1, 150, 33, 517)])
