@@ -258,7 +258,9 @@ __device__ __forceinline__ double f64_finish(const F64Product& p, int64_t m, int
   return v;
 }
 
-// KA, KB: K is contiguous in A, in B.
+// KA, KB: K is contiguous in A, in B. 512 x 512 x 8192: z 177 us, dx 155, dw 174 (24 to 28 of 37
+// TFLOP/s, bound by the FP64 tensor pipe and, at 512 tiles on 296 places, by
+// rounds); 4 x 1000 x 50000: 76, 71, 129 us against 62 each for w's bytes.
 template <typename T, bool KA, bool KB, bool VA, bool VB>
 __global__ void __launch_bounds__(T::THREADS, T::CTAS) f64_tile_kernel(const F64Product p, const F64Plan plan,
                                                                        double* ws) {
