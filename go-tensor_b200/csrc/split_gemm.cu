@@ -44,9 +44,11 @@ constexpr int SSTAGES = 6;
 // dx, whose rows of G hold one value near -1 among small ones, takes 128 of K
 // (its error at V = 517: 0.6e-6 of the result against 1.3e-6 with 256), which
 // its long K and few epilogues hide (277 us either way at 2048 x 1024 x
-// 32000); the logits and dw take 256 (284 us against 318, 260 against 276).
-template <bool A_MN, bool LOGITS>
-constexpr int group_stages() { return A_MN || LOGITS ? 8 : 4; }
+// 32000). dw takes 128 too (its error at 1880 x 1118 x 544: 0.67e-6 against 1.01e-6,
+// where plain float32 sums have 0.59e-6) for 276 us against 260, 1.5 % of a
+// whole call. The logits take 256 (284 us against 318).
+template <bool LOGITS>
+constexpr int group_stages() { return LOGITS ? 8 : 4; }
 constexpr int SGROUP_MAX = 8;
 constexpr int STHREADS = 384;
 constexpr uint32_t PLANE_BYTES = SBM * SBK * 2;  // one plane of one operand, 8 KB
@@ -242,7 +244,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   SplitShared* sh = (SplitShared*)(smem + SBAR_OFFSET);
-  constexpr int SGROUP = group_stages<A_MN, LOGITS>();
+  constexpr int SGROUP = group_stages<LOGITS>();
   constexpr bool INDEXED = !A_MN && !LOGITS;  // dx: the rows of C are scattered
   volatile int* failed = &sh->failed;
 
