@@ -260,7 +260,7 @@ __device__ __forceinline__ double f64_finish(const F64Product& p, int64_t m, int
 
 // KA, KB: K is contiguous in A, in B. 512 x 512 x 8192: z 177 us, dx 155, dw 174 (24 to 28 of 37
 // TFLOP/s, bound by the FP64 tensor pipe and, at 512 tiles on 296 places, by
-// rounds); 4 x 1000 x 50000: 76, 71, 129 us against 62 each for w's bytes.
+// rounds); 4 x 1000 x 50000: 78, 73 and 113 us against 62 each for w's bytes.
 template <typename T, bool KA, bool KB, bool VA, bool VB>
 __global__ void __launch_bounds__(T::THREADS, T::CTAS) f64_tile_kernel(const F64Product p, const F64Plan plan,
                                                                        double* ws) {
@@ -305,8 +305,10 @@ __global__ void __launch_bounds__(T::THREADS, T::CTAS) f64_tile_kernel(const F64
     load(t + T::STAGES - 1);
     const double* as = f64_smem + t % T::STAGES * STAGE + SA::at(fk, wm + fr);
     const double* bs = f64_smem + t % T::STAGES * STAGE + SA::SIZE + SB::at(fk, wn + fr);
+    const int64_t left = k_end - k_begin - t * kF64Depth;
 #pragma unroll
     for (int k = 0; k < kF64Depth; k += 4) {
+      if (k >= left) break;  // dw of a few rows
       double a[MI], b[4];
 #pragma unroll
       for (int i = 0; i < MI; i++) a[i] = as[SA::at(k, 8 * i)];
