@@ -13,15 +13,17 @@
 // not grow with the number of rows. float32 runs on the tensor cores
 // (split_gemm.cu):
 //
-//   operand_top_kernel   largest magnitudes of x and w, the rows that count
+//   row_count_kernel     the rows that count
 //   operand_split_kernel w and the rows of x that count, which are listed: only
-//                        they go through the products, as two float16 planes each
+//                        they go through the products, as two float16 planes each,
+//                        every row with a power of two of its own
 //   per piece of these rows:
 //     split_gemm         z, and per strip of 128 classes of a row its maximum
 //                        and sum of exponentials, from the registers of the
 //                        product; a forward pass alone never writes z
 //     strip_join_kernel  the strips' pairs joined: lse, the rows' losses
-//     grad_planes_kernel z -> n G as two float16 planes, its column sums
+//     grad_planes_kernel z -> n G as two float16 planes, once for dx and once for
+//                        dw, its column sums
 //     split_gemm         dx = G w, dw (+)= G^T x
 //   mean_rows_kernel     the loss
 //
@@ -34,12 +36,13 @@
 
 namespace gt {
 
-// What the kernels of one float32 call share: the operands' largest finite
-// magnitudes (as ordered words), the rows that count, and the products' factors.
+// What the kernels of one float32 call share about the rows that count: how
+// many they are, the smallest up_to with that many <= 2^up_to, and 2^up_to / their number
+// (0 when there is none).
 struct XentMeta {
-  uint32_t x_top, w_top;
   int64_t count;
-  SplitScale logits, dx, dw;
+  int up_to;
+  float share;
 };
 
 __device__ __forceinline__ uint32_t finite_bits(float v) {
@@ -53,81 +56,27 @@ __device__ __forceinline__ uint32_t finite_bits4(float4 v) {
 
 constexpr int kCompactRows = 1024;  // rows per block of the compaction
 
-// The largest magnitudes of w (blocks 0 .. w_blocks - 1) and of the rows of x
-// that count (the next x_blocks, a warp per row), and how many of each 1024 rows
-// count (the others); a label outside [0, V) sets *bad.
-__global__ void __launch_bounds__(256) operand_top_kernel(const float* __restrict__ x, const float* __restrict__ w,
-                                                          const int32_t* __restrict__ labels, int64_t M, int64_t K,
-                                                          int64_t V, int32_t ignore, int w_blocks, int x_blocks,
-                                                          XentMeta* meta, int32_t* counts, int32_t* bad) {
-  __shared__ uint32_t tops[8];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t top = 0;
-  if ((int)blockIdx.x >= w_blocks + x_blocks) {
-    const int64_t b = blockIdx.x - w_blocks - x_blocks;
-    int kept = 0;
-    for (int i = threadIdx.x; i < kCompactRows; i += 256) {
-      const int64_t m = b * kCompactRows + i;
-      kept += __syncthreads_count(m < M && labels[m] != ignore);
-    }
-    if (threadIdx.x == 0) counts[b] = kept;
-    return;
+// How many of each 1024 rows count; a label outside [0, V) sets *bad.
+__global__ void __launch_bounds__(256) row_count_kernel(const int32_t* __restrict__ labels, int64_t M, int64_t V,
+                                                        int32_t ignore, int32_t* counts, int32_t* bad) {
+  int kept = 0;
+  for (int i = threadIdx.x; i < kCompactRows; i += 256) {
+    const int64_t m = (int64_t)blockIdx.x * kCompactRows + i;
+    const int32_t y = m < M ? labels[m] : ignore;
+    if (y != ignore && bad && (y < 0 || y >= V)) *bad = 1;
+    kept += __syncthreads_count(y != ignore);
   }
-  if ((int)blockIdx.x < w_blocks) {
-    const int64_t n = V * K, stride = (int64_t)w_blocks * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t n4 = ((uintptr_t)w & 15) == 0 ? n / 4 : 0;
-    const float4* w4 = reinterpret_cast<const float4*>(w);
-    for (int64_t i = at; i < n4; i += 4 * stride) {  // four loads in flight
-      float4 v[4];
-#pragma unroll
-      for (int u = 0; u < 4; u++) v[u] = i + u * stride < n4 ? w4[i + u * stride] : float4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int u = 0; u < 4; u++) top = max(top, finite_bits4(v[u]));
-    }
-    for (int64_t i = n4 * 4 + at; i < n; i += stride) top = max(top, finite_bits(w[i]));
-  } else {
-    for (int64_t m = (int64_t)(blockIdx.x - w_blocks) * 8 + warp; m < M; m += (int64_t)x_blocks * 8) {
-      const int32_t y = labels[m];
-      if (y == ignore) continue;
-      if (lane == 0 && bad && (y < 0 || y >= V)) *bad = 1;
-      const float* r = x + m * K;
-      const int64_t k4 = ((K & 3) | ((uintptr_t)x & 15)) == 0 ? K / 4 : 0;
-      for (int64_t k = lane; k < k4; k += 128) {
-        float4 v[4];
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-          v[u] = k + 32 * u < k4 ? reinterpret_cast<const float4*>(r)[k + 32 * u] : float4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int u = 0; u < 4; u++) top = max(top, finite_bits4(v[u]));
-      }
-#pragma unroll 4
-      for (int64_t k = 4 * k4 + lane; k < K; k += 32) top = max(top, finite_bits(r[k]));
-    }
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0) tops[warp] = top;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; i++) top = max(top, tops[i]);
-    if (top) atomicMax((int)blockIdx.x < w_blocks ? &meta->w_top : &meta->x_top, top);
-  }
+  if (threadIdx.x == 0) counts[blockIdx.x] = kept;
 }
 
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // The exponent e that puts a largest magnitude at 2^14 .. 2^15 when
-// multiplied by 2^e: -113 .. 163.
+// multiplied by 2^e: -113 .. 126. (2^126 is enough for any: what a plane then
+// loses is below 2^-150, half of the smallest float32.)
 __device__ __forceinline__ int plane_exponent(uint32_t top) {
   if (top == 0) return 0;
-  return 14 - (top < 0x800000u ? 31 - __clz((int)top) - 149 : (int)(top >> 23) - 127);
-}
-
-// 2^-e times f (at most 1), as one factor, or as two halves of the power where one
-// would not be a normal number (beyond 2^-252 nothing is left of an accumulator anyway).
-__device__ __forceinline__ SplitScale undo(int e, float f) {
-  e = min(e, 252);
-  if (e >= -126 && e <= 64) return {__fmul_rn(exp2_int(-e), f), 1.0f};
-  return {exp2_int(-e / 2), __fmul_rn(exp2_int(-e - (-e / 2)), f)};
+  return min(126, 14 - (top < 0x800000u ? 31 - __clz((int)top) - 149 : (int)(top >> 23) - 127));
 }
 
 __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
@@ -136,11 +85,11 @@ __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
   lo = __float2half_rn(isfinite(back) ? __fsub_rn(v, back) : 0.0f);  // an infinity stays one
 }
 
-constexpr int kGradExponent = 15;  // n G lies in [-1, 1]
-
 // w and the rows of x that count, in their order, as planes of pitch Kp, a warp
-// per row: index[j] = the j-th such row, y[j] its label; an ignored row's dx
-// and loss are 0. Behind the last row of x come zeros up to a multiple of 32
+// per row: index[j] = the j-th such row, y[j] its label, xs[j] and ws[v] what the
+// rows' values in the planes are to be multiplied by; an ignored row's dx
+// and loss are 0. The row is read twice, the second time from cache (its
+// largest magnitude is wanted first). Behind the last row of x come zeros up to a multiple of 32
 // rows (dw's products read that far). A row's place is the number of rows that
 // count before it: the counts of the 1024-row blocks before its own, and a
 // ballot over the labels of its own (a kernel of its own for this took 4 us more).
@@ -148,12 +97,11 @@ __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restr
                                                             const int32_t* __restrict__ labels, int64_t M, int64_t K,
                                                             int64_t V, int64_t Kp, int32_t ignore,
                                                             const int32_t* counts, XentMeta* meta, int32_t* index,
-                                                            int32_t* y, __half* __restrict__ xp,
-                                                            __half* __restrict__ wp, float* __restrict__ dx,
-                                                            float* rows) {
+                                                            int32_t* y, float* xs, float* ws,
+                                                            __half* __restrict__ xp, __half* __restrict__ wp,
+                                                            float* __restrict__ dx, float* rows) {
   after_predecessor();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int ex = plane_exponent(meta->x_top), ew = plane_exponent(meta->w_top);
   // the rows that count before row `end`
   auto count_before = [&](int64_t end) {
     const int64_t full = end / kCompactRows;
@@ -168,13 +116,10 @@ __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restr
   if (blockIdx.x == 0 && warp == 0) {
     const int64_t count = count_before(M);
     if (lane == 0) {
-      const float inv = (float)(1.0 / (double)count);
+      const int up_to = count > 1 ? 64 - __clzll(count - 1) : 0;
       meta->count = count;
-      meta->logits = undo(ex + ew, 1.0f);
-      meta->dx = undo(ew + kGradExponent, inv);
-      meta->dw = undo(ex + kGradExponent, inv);
-      if (count == 0)  // no row counts: the gradients are 0
-        meta->dx.c1 = meta->dw.c1 = meta->dx.c2 = meta->dw.c2 = 0.0f;
+      meta->up_to = up_to;
+      meta->share = count ? (float)((double)((int64_t)1 << up_to) / (double)count) : 0.0f;
     }
   }
   for (int64_t i = (int64_t)blockIdx.x * 8 + warp; i < V + M + 32; i += (int64_t)gridDim.x * 8) {
@@ -200,16 +145,33 @@ __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restr
     const float* src = (is_x ? x : w) + row * K;
     __half* hi = (is_x ? xp : wp) + to * Kp;
     __half* lo = hi + (is_x ? M : V) * Kp;
-    const int e = is_x ? ex : ew;
-    const float f1 = exp2_int(e / 2), f2 = exp2_int(e - e / 2);
-    if ((K & 7) == 0 && ((uintptr_t)src & 15) == 0) {
+    const bool vec = (K & 7) == 0 && ((uintptr_t)src & 15) == 0;
+    uint32_t top = 0;
+    if (!keep) {
+    } else if (vec) {
+      for (int64_t k = lane; k < K / 4; k += 128) {  // four loads in flight
+        float4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+          v[u] = k + 32 * u < K / 4 ? reinterpret_cast<const float4*>(src)[k + 32 * u] : float4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < 4; u++) top = max(top, finite_bits4(v[u]));
+      }
+    } else {
+#pragma unroll 8
+      for (int64_t k = lane; k < K; k += 32) top = max(top, finite_bits(src[k]));
+    }
+    const int e = plane_exponent(__reduce_max_sync(0xffffffffu, top));
+    const float f = exp2_int(e);
+    if (lane == 0) (is_x ? xs : ws)[to] = exp2_int(-e);
+    if (vec) {
       for (int64_t k = lane; k < K / 8; k += 32) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
         if (keep) a = reinterpret_cast<const float4*>(src)[2 * k], b = reinterpret_cast<const float4*>(src)[2 * k + 1];
         const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
         __align__(16) __half h[8], l[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) split_half(__fmul_rn(__fmul_rn(v[j], f1), f2), h[j], l[j]);
+        for (int j = 0; j < 8; j++) split_half(__fmul_rn(v[j], f), h[j], l[j]);
         reinterpret_cast<uint4*>(hi)[k] = *reinterpret_cast<uint4*>(h);
         reinterpret_cast<uint4*>(lo)[k] = *reinterpret_cast<uint4*>(l);
       }
@@ -220,7 +182,7 @@ __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restr
         for (int j = 0; j < 8; j++) v[j] = keep && k + 32 * j < K ? src[k + 32 * j] : 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; j++)
-          if (k + 32 * j < K) split_half(__fmul_rn(__fmul_rn(v[j], f1), f2), hi[k + 32 * j], lo[k + 32 * j]);
+          if (k + 32 * j < K) split_half(__fmul_rn(v[j], f), hi[k + 32 * j], lo[k + 32 * j]);
       }
     }
   }
@@ -260,66 +222,184 @@ __global__ void __launch_bounds__(1024) strip_join_kernel(const float2* strips, 
   }
 }
 
-// n G = exp(z - maximum) / sum - [label] for up to 32 rows of 1024 columns (4 per
-// thread), as two float16 planes of n G 2^15 and, for db, summed over the rows.
-constexpr int kGradCols = 1024;
-// Rows per block: 32, or 8 when that leaves SMs idle (15 us against 4 at 128 x 4000).
-static int grad_rows(const gt_ctx* ctx, int64_t rows, int64_t V) {
-  return ceil_div(rows, 32) * ceil_div(V, kGradCols) >= 2 * (int64_t)ctx->sm_count ? 32 : 8;
+// n G = exp(z - maximum) / sum - [label] for 128 rows of 128 columns, as two
+// float16 planes for each of the products that it goes into, and, for db, summed over the rows.
+//
+// dx = G w sums over classes, whose rows of w have scales of their own, and dw = G^T x over
+// rows of x. So the planes for dx hold q 2^T with q = n G ws[v] / (the largest ws of
+// the tile's columns), T of the row and the tile such that the largest |q| lands at 2^14 .. 2^15; those for
+// dw the same with xs of the tile's rows and a T of the column. A class that is far from
+// likely so keeps its digits in dw beside those that are likely, as does a
+// row of small gradients in dx. What undoes it goes to dx_scale and dw_scale, with
+// 2^-up_to, whose rest, share, the products multiply by at the end (no sum
+// exceeds the result's own range so).
+//
+// A block has a tile of 128 x 128 in registers, since a column's T is known
+// only when all its rows are; a warp has every 16th row, a lane four columns. The planes for
+// dx take z's place: a row's 128 columns are as many bytes, and are read before they are written.
+// 2048 x 32000: 158 us, 12 bytes per logit at 5.0 TB/s (one set of planes with one scale for all of G took 87 us).
+constexpr int kGradTile = 128;
+static_assert(kGradTile == kSplitGroup && kGradTile == kStripCols, "a tile is one group of K of either product");
+
+// exp(d) for d <= 0, -infinity and NaN included (0): the exponent's rounding error is put back
+// to first order, so the relative error is that of the hardware's power of two, about 2^-22, whatever d is.
+__device__ __forceinline__ float exp_exact(float d) {
+  constexpr float kLog2e = 1.4426950408889634f, kRest = (float)(1.4426950408889634 - (double)kLog2e);
+  d = fmaxf(d, -200.0f);
+  const float t = __fmul_rn(d, kLog2e);
+  const float r = fmaf(d, kRest, fmaf(d, kLog2e, -t));
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return fmaf(e, __fmul_rn(r, 0.6931471805599453f), e);
 }
-template <bool DB>
-__global__ void __launch_bounds__(256) grad_planes_kernel(const float* z, const float2* stat, const int32_t* y,
-                                                          const XentMeta* meta, int64_t r0, int64_t R, int64_t V,
-                                                          int64_t Vp, int across, int rpb, __half* g, int64_t plane,
-                                                          float* part) {
+
+__device__ __forceinline__ void split_store(__half* hi, __half* lo, const float (&v)[4]) {
+  const __half2 h[2] = {__floats2half2_rn(v[0], v[1]), __floats2half2_rn(v[2], v[3])};
+  const float2 a = __half22float2(h[0]), b = __half22float2(h[1]);
+  const __half2 l[2] = {__floats2half2_rn(__fsub_rn(v[0], a.x), __fsub_rn(v[1], a.y)),
+                        __floats2half2_rn(__fsub_rn(v[2], b.x), __fsub_rn(v[3], b.y))};
+  *reinterpret_cast<uint2*>(hi) = *reinterpret_cast<const uint2*>(h);
+  *reinterpret_cast<uint2*>(lo) = *reinterpret_cast<const uint2*>(l);
+}
+
+// The exponent of a power of two, or of a value's magnitude (a subnormal's as if it were 2^-127).
+__device__ __forceinline__ int exponent_of(float v) { return (int)((__float_as_uint(v) >> 23) & 0xffu) - 127; }
+
+// T for a largest |q| of `top` whose q already lacks a factor 2^base: such that
+// neither 2^T nor 2^-(T - base + up_to) leaves the normal numbers.
+__device__ __forceinline__ int tile_shift(float top, int base, int up_to) {
+  return min(min(14 - exponent_of(top), 127), 126 - up_to + base);
+}
+
+template <bool DX, bool DW, bool DB>
+__global__ void __launch_bounds__(512, 2) grad_planes_kernel(float* z, const float2* stat, const int32_t* y,
+                                                             const float* xs, const float* ws, const XentMeta* meta,
+                                                             int64_t r0, int64_t R, int64_t V, int64_t Vp, int across,
+                                                             __half* g, int64_t plane, float* dx_scale,
+                                                             float* dw_scale, float* part) {
   after_predecessor();
-  __shared__ float2 st[32];
-  __shared__ int32_t ys[32];
+  __shared__ float tops[16][kGradTile], sums[16][kGradTile];
+  __shared__ int shift[kGradTile];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t rb = blockIdx.x / across, cb = blockIdx.x - rb * across;
-  const int64_t m0 = rb * rpb, c = cb * kGradCols + 4 * threadIdx.x, here = rows_here(meta, r0, R);
+  const int64_t m0 = rb * kGradTile, c = cb * kGradTile + 4 * lane, here = rows_here(meta, r0, R);
   // behind the last row come zeros up to a multiple of 32 rows (dw's products read that far)
-  const int n = (int)min((int64_t)rpb, min(R, (here + 31) / 32 * 32) - m0);
-  if (n <= 0) return;
-  if (threadIdx.x < n) {
-    const bool row = m0 + threadIdx.x < here;
-    st[threadIdx.x] = row ? stat[m0 + threadIdx.x] : make_float2(0.0f, 0.0f);
-    ys[threadIdx.x] = row ? y[r0 + m0 + threadIdx.x] : -1;
+  const int64_t end = min(R, (here + 31) / 32 * 32);
+  if (m0 >= end) return;
+  const int up_to = meta->up_to;
+  float p[8][4];
+#pragma unroll
+  for (int u = 0; u < 8; u++) {
+    const int64_t m = m0 + warp + 16 * u;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (m < here) v = *reinterpret_cast<const float4*>(z + m * Vp + c);
+    p[u][0] = v.x, p[u][1] = v.y, p[u][2] = v.z, p[u][3] = v.w;
   }
-  __syncthreads();
-  if (c >= V) return;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int i = 0; i < n; i++) {
-    const float4 v = *reinterpret_cast<const float4*>(z + (m0 + i) * Vp + c);
-    const float2 s = st[i];
-    const int64_t at = (int64_t)ys[i] - c;
-    float p[4] = {v.x, v.y, v.z, v.w};
-    __align__(8) __half hi[4], lo[4];
+  // ws and xs relative to the tile's largest
+  float wf[4] = {0.f, 0.f, 0.f, 0.f};
+  int w_base = 0, x_base = 0;
+  if (DX) {
+    const float4 f = *reinterpret_cast<const float4*>(ws + c);
+    if (c < V) wf[0] = f.x;
+    if (c + 1 < V) wf[1] = f.y;
+    if (c + 2 < V) wf[2] = f.z;
+    if (c + 3 < V) wf[3] = f.w;
+    const float top = fmaxf(fmaxf(wf[0], wf[1]), fmaxf(wf[2], wf[3]));
+    w_base = exponent_of(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
+#pragma unroll
+    for (int j = 0; j < 4; j++) wf[j] *= exp2_int(-w_base);
+  }
+  if (DW) {
+    float top = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+      if (m0 + lane + 32 * u < here) top = fmaxf(top, xs[r0 + m0 + lane + 32 * u]);
+    x_base = exponent_of(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
+  }
+  float top[4] = {0.f, 0.f, 0.f, 0.f}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < 8; u++) {
+    const int64_t m = m0 + warp + 16 * u;
+    if (m >= here) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) p[u][j] = 0.0f;
+      continue;
+    }
+    const float2 s = stat[m];
+    const int64_t at = (int64_t)y[r0 + m] - c;
+#pragma unroll
+    for (int j = 0; j < 4; j++) p[u][j] = exp_exact(p[u][j] - s.x) * s.y;
+    if (at >= 0 && at < 4) {
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (at == j) p[u][j] -= 1.0f;
+    }
+    if (c + 3 >= V) {
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (c + j >= V) p[u][j] = 0.0f;
+    }
+    if (DX) {
+      float q[4], row_top = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; j++) q[j] = p[u][j] * wf[j], row_top = fmaxf(row_top, fabsf(q[j]));
+      row_top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(row_top)));
+      const int t = tile_shift(row_top, w_base, up_to);
+      const float f = exp2_int(t);
+#pragma unroll
+      for (int j = 0; j < 4; j++) q[j] *= f;
+      __half* o = reinterpret_cast<__half*>(z + m * Vp + cb * kGradTile) + 4 * lane;
+      split_store(o, o + kGradTile, q);
+      if (lane == 0) dx_scale[cb * R + m] = exp2_int(-(t - w_base + up_to));
+    }
+    const float xf = DW ? xs[r0 + m] * exp2_int(-x_base) : 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      p[j] = s.y == 0.0f ? 0.0f : expf(p[j] - s.x) * s.y - (at == j ? 1.0f : 0.0f);
-      if (DB) sum[j] += p[j];
-      split_half(p[j] * (float)(1 << kGradExponent), hi[j], lo[j]);
+      if (DB) sum[j] += p[u][j];
+      if (DW) p[u][j] *= xf, top[j] = fmaxf(top[j], fabsf(p[u][j]));
     }
-    __half* o = g + (m0 + i) * Vp + c;
-    *reinterpret_cast<uint2*>(o) = *reinterpret_cast<uint2*>(hi);
-    *reinterpret_cast<uint2*>(o + plane) = *reinterpret_cast<uint2*>(lo);
   }
-  if (DB) {
+  if constexpr (DW || DB) {
+    if (DW) *reinterpret_cast<float4*>(&tops[warp][4 * lane]) = make_float4(top[0], top[1], top[2], top[3]);
+    if (DB) *reinterpret_cast<float4*>(&sums[warp][4 * lane]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    __syncthreads();
+    if (threadIdx.x < kGradTile) {
+      const int64_t col = cb * kGradTile + threadIdx.x;
+      float most = 0.0f, s = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (c + j < V) part[rb * V + c + j] = sum[j];
+      for (int u = 0; u < 16; u++) {
+        if (DW) most = fmaxf(most, tops[u][threadIdx.x]);
+        if (DB) s += sums[u][threadIdx.x];
+      }
+      const int t = tile_shift(most, x_base, up_to);
+      if (DW) shift[threadIdx.x] = t;
+      if (DW && col < V) dw_scale[rb * V + col] = exp2_int(-(t - x_base + up_to));
+      if (DB && col < V) part[rb * V + col] = s;
+    }
+  }
+  if constexpr (DW) {
+    __syncthreads();
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) f[j] = exp2_int(shift[4 * lane + j]);
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const int64_t m = m0 + warp + 16 * u;
+      if (m >= end) break;
+      const float q[4] = {p[u][0] * f[0], p[u][1] * f[1], p[u][2] * f[2], p[u][3] * f[3]};
+      split_store(g + m * Vp + c, g + m * Vp + c + plane, q);
+    }
   }
 }
 
-// db (+)= the column sums of the blocks of rows, / n: 32 columns per block,
+// db (+)= the column sums of the tiles' rows, / n: 32 columns per block,
 // warp w adds the rows w, w + 8, ... in order, then the warps' sums in order.
-__global__ void __launch_bounds__(256) db_kernel(const float* part, int rpb, int64_t r0, int64_t R, int64_t V, const XentMeta* meta,
-                                                 float* db) {
+__global__ void __launch_bounds__(256) db_kernel(const float* part, int64_t r0, int64_t R, int64_t V,
+                                                 const XentMeta* meta, float* db) {
   after_predecessor();
   __shared__ double ws[8][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane, blocks = (rows_here(meta, r0, R) + rpb - 1) / rpb;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane, blocks = (rows_here(meta, r0, R) + kGradTile - 1) / kGradTile;
   double acc = 0.0;
   if (c < V) {
 #pragma unroll 8
@@ -337,19 +417,18 @@ __global__ void __launch_bounds__(256) db_kernel(const float* part, int rpb, int
 static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
   if (few_rows(c.M, c.K, c.V)) return linear_xent_few(ctx, c, held);
   const bool grad = c.dx || c.dw || c.db;
-  const int64_t Kp = ceil_div(c.K, 8) * 8, Vp = ceil_div(c.V, 8) * 8, strips = ceil_div(c.V, kStripCols);
-  // Rows per piece: as many as the workspace holds (z and the two planes of G
-  // take 8 bytes per logit, the strips 8 per 128), in multiples of the tiles'
+  const int64_t Kp = ceil_div(c.K, 8) * 8, Vp = ceil_div(c.V, kGradTile) * kGradTile, groups = Vp / kGradTile;
+  // Rows per piece: as many as the workspace holds (z and dw's planes of G
+  // take 8 bytes per logit, the strips and scales 16 per 128), in multiples of the tiles'
   // 256 rows, and the pieces of equal size.
-  const int64_t per_row = (grad ? 8 * Vp : 0) + 8 * strips;
+  const int64_t per_row = (grad ? 8 * Vp : 0) + 16 * groups;
   int64_t R = std::max<int64_t>(1, c.workspace / per_row / 256) * 256;
   R = std::min(c.M, ceil_div(ceil_div(c.M, ceil_div(c.M, R)), 256) * 256);
-  const int rpb = grad_rows(ctx, R, c.V);
-  const int64_t row_blocks = ceil_div(c.M, kCompactRows);
+  const int64_t row_blocks = ceil_div(c.M, kCompactRows), tiles = ceil_div(R, kGradTile);
   struct {
     XentMeta* meta;
     __half *x, *w, *g;
-    float *z, *losses, *picked, *part;
+    float *xs, *ws, *z, *losses, *picked, *part, *dx_scale, *dw_scale;
     float2 *strips, *stat;
     int32_t *counts, *index, *y;
   } ws;
@@ -357,12 +436,16 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
     ws.meta = k.take<XentMeta>(1);
     ws.x = k.take<__half>(2 * c.M * Kp);
     ws.w = k.take<__half>(2 * c.V * Kp);
-    ws.g = k.take<__half>(grad ? 2 * R * Vp : 0);
+    ws.xs = k.take<float>(c.M);
+    ws.ws = k.take<float>(ceil_div(c.V, 256) * 256);
+    ws.g = k.take<__half>(c.dw ? 2 * R * Vp : 0);
     ws.z = k.take<float>(grad ? R * Vp : 0);
     ws.losses = k.take<float>(c.M);
     ws.picked = k.take<float>(R);
-    ws.part = k.take<float>(c.db ? ceil_div(R, rpb) * c.V : 0);
-    ws.strips = k.take<float2>(strips * R);
+    ws.part = k.take<float>(c.db ? tiles * c.V : 0);
+    ws.dx_scale = k.take<float>(c.dx ? groups * R : 0);
+    ws.dw_scale = k.take<float>(c.dw ? tiles * c.V : 0);
+    ws.strips = k.take<float2>(groups * R);
     ws.stat = k.take<float2>(R);
     ws.counts = k.take<int32_t>(row_blocks);
     ws.index = k.take<int32_t>(c.M);
@@ -374,49 +457,52 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
   Carver at{(char*)held[0]};
   carve(at);
 
-  GT_CUDA(cudaMemsetAsync(ws.meta, 0, sizeof(XentMeta), ctx->stream));
-  const int most = 8 * ctx->sm_count;  // resident blocks: one round each
-  const int wb = std::min(most, grid_for(ctx, c.V * c.K, 256, 16)), xb = std::min(most, grid_for(ctx, c.M * c.K, 256, 16));
-  operand_top_kernel<<<(unsigned)(wb + xb + row_blocks), 256, 0, ctx->stream>>>(
-      c.x, c.w, c.labels, c.M, c.K, c.V, c.ignore, wb, xb, ws.meta, ws.counts, c.bad);
+  row_count_kernel<<<(unsigned)row_blocks, 256, 0, ctx->stream>>>(c.labels, c.M, c.V, c.ignore, ws.counts, c.bad);
   GT_LAUNCH_CHECK();
   const int sb = (int)std::min<int64_t>(ceil_div(c.M + c.V + 32, 8), (int64_t)ctx->sm_count * 32);
   GT_CUDA(launch_overlapped(ctx, operand_split_kernel, sb, 256, 0, c.x, c.w, c.labels, c.M, c.K, c.V, Kp, c.ignore,
-                            ws.counts, ws.meta, ws.index, ws.y, ws.x, ws.w, c.dx, c.rows));
+                            ws.counts, ws.meta, ws.index, ws.y, ws.xs, ws.ws, ws.x, ws.w, c.dx, c.rows));
   const HalfPlanes w{ws.w, c.V, c.K, Kp, c.V * Kp};
   for (int64_t r0 = 0; r0 < c.M; r0 += R) {
     // As many pieces as all rows would need; those behind the rows that count find nothing to do.
     const int64_t r = std::min(R, c.M - r0);
-    const HalfPlanes x{ws.x + r0 * Kp, r, c.K, Kp, c.M * Kp}, g{ws.g, r, c.V, Vp, R * Vp};
+    const HalfPlanes x{ws.x + r0 * Kp, r, c.K, Kp, c.M * Kp};
     SplitGemm f;
     f.M = r, f.N = c.V, f.K = c.K, f.kept = &ws.meta->count, f.kept_from = r0, f.a = x, f.b = w;
-    f.scale = &ws.meta->logits;
+    f.row_scale = ws.xs + r0, f.col_scale = ws.ws;
     f.out = grad ? ws.z : nullptr, f.ldc = Vp, f.bias = c.bias, f.labels = ws.y + r0;
     f.strips = ws.strips, f.strip_rows = R, f.picked = ws.picked;
     GT_TRY(split_gemm(ctx, f));
-    GT_CUDA(launch_overlapped(ctx, strip_join_kernel, (unsigned)ceil_div(r, 32), 1024, 0, ws.strips, R, (int)strips,
-                              ws.y, ws.index, ws.meta, r0, c.V, ws.picked, ws.stat, ws.losses, c.rows));
+    GT_CUDA(launch_overlapped(ctx, strip_join_kernel, (unsigned)ceil_div(r, 32), 1024, 0, ws.strips, R,
+                              (int)ceil_div(c.V, kStripCols), ws.y, ws.index, ws.meta, r0, c.V, ws.picked, ws.stat,
+                              ws.losses, c.rows));
     if (!grad) continue;
-    const int64_t across = ceil_div(c.V, kGradCols);
-    GT_CUDA(launch_overlapped(ctx, c.db ? grad_planes_kernel<true> : grad_planes_kernel<false>,
-                              (unsigned)(across * ceil_div(r, rpb)), 256, 0, ws.z, ws.stat, ws.y, ws.meta, r0, r, c.V,
-                              Vp, (int)across, rpb, ws.g, R * Vp, ws.part));
+    const decltype(&grad_planes_kernel<false, false, true>) planes[8] = {
+        nullptr, grad_planes_kernel<false, false, true>,
+        grad_planes_kernel<false, true, false>, grad_planes_kernel<false, true, true>,
+        grad_planes_kernel<true, false, false>, grad_planes_kernel<true, false, true>,
+        grad_planes_kernel<true, true, false>, grad_planes_kernel<true, true, true>};
+    GT_CUDA(launch_overlapped(ctx, planes[(c.dx ? 4 : 0) + (c.dw ? 2 : 0) + (c.db ? 1 : 0)],
+                              (unsigned)(groups * ceil_div(r, kGradTile)), 512, 0, ws.z, ws.stat, ws.y, ws.xs, ws.ws,
+                              ws.meta, r0, r, c.V, Vp, (int)groups, ws.g, R * Vp, ws.dx_scale, ws.dw_scale, ws.part));
     if (c.dx) {
       SplitGemm d;
-      d.M = r, d.N = c.K, d.K = c.V, d.kept = &ws.meta->count, d.kept_from = r0, d.a = g, d.b = w, d.b_mn = true;
-      d.scale = &ws.meta->dx;
+      d.M = r, d.N = c.K, d.K = c.V, d.kept = &ws.meta->count, d.kept_from = r0, d.b = w, d.b_mn = true;
+      d.a = HalfPlanes{reinterpret_cast<const __half*>(ws.z), r, c.V, 2 * Vp, 0, true};
+      d.scale = &ws.meta->share, d.group_scale = ws.dx_scale, d.group_ld = r;
       d.out = c.dx, d.ldc = c.K, d.row_index = ws.index + r0;
       GT_TRY(split_gemm(ctx, d));
     }
     if (c.dw) {
       SplitGemm d;
-      d.M = c.V, d.N = c.K, d.K = r, d.kept = &ws.meta->count, d.kept_from = r0, d.a = g, d.a_mn = true, d.b = x;
-      d.b_mn = true, d.scale = &ws.meta->dw;
+      d.M = c.V, d.N = c.K, d.K = r, d.kept = &ws.meta->count, d.kept_from = r0, d.a_mn = true, d.b = x;
+      d.a = HalfPlanes{ws.g, r, c.V, Vp, R * Vp}, d.b_mn = true;
+      d.scale = &ws.meta->share, d.group_scale = ws.dw_scale, d.group_ld = c.V;
       d.out = c.dw, d.ldc = c.K, d.accumulate = r0 > 0;
       GT_TRY(split_gemm(ctx, d));
     }
     if (c.db)
-      GT_CUDA(launch_overlapped(ctx, db_kernel, (unsigned)ceil_div(c.V, 32), 256, 0, ws.part, rpb, r0, r, c.V, ws.meta,
+      GT_CUDA(launch_overlapped(ctx, db_kernel, (unsigned)ceil_div(c.V, 32), 256, 0, ws.part, r0, r, c.V, ws.meta,
                                 c.db));
   }
   GT_CUDA(launch_overlapped(ctx, mean_rows_kernel<float>, 1, 1024, 0, ws.losses, c.M, true, &ws.meta->count, c.loss));

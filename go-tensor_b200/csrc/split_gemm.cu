@@ -1,14 +1,20 @@
 // tcgen05 GEMM of float32 operands held as two float16 planes, for sm_100a.
 //
 // Precision. x s = hi + lo with hi = half(x s), lo = half(x s - hi), s a power of
-// two that puts the operand's largest magnitude at 2^14: 22 bits of every
-// value down to 2^-18 of the largest, and nothing worse than 2^-40 of the
-// largest below that. A product is
+// two that puts the largest magnitude that shares it at 2^14 .. 2^15: 22 bits
+// of every value down to 2^-16 of that largest, and an error of at most 2^-39 of
+// it below. What shares a scale is what stands in one sum anyway: a row of x
+// and a row of w in the logits, whose epilogue undoes both; in dx and dw, whose
+// sums run over rows of w and of x with scales of their own, those scales are
+// folded into G, which is scaled again per group of 128 values of K and row of
+// the result, undone as the group's partial sum is added. (One scale per
+// operand cost a product's other rows 2^-39 of the largest row's, and what G had
+// below 2^-39.) A product is
 //   a b ~= hi(a) hi(b) + hi(a) lo(b) + lo(a) hi(b)          (lo lo dropped, 2^-22)
 // the same three products and the same mantissas as 3xTF32 (gemm_tc.cu), but
 // kind::f16 runs at twice the rate of kind::tf32 and a plane takes half the
-// bytes. The range that float16 lacks is in the scale, which the epilogue
-// undoes exactly. The operands arrive split (each is used by two GEMMs), so
+// bytes. The range that float16 lacks is in the scales, which are powers of
+// two. The operands arrive split (each is used by two GEMMs), so
 // no warp splits them here.
 // Tensor-core accumulation truncates, so, as there, the MMAs accumulate 256
 // (or 128) values of K into one of two partial buffers in tensor memory and promoter
@@ -47,8 +53,9 @@ constexpr int SSTAGES = 6;
 // 32000). dw takes 128 too (its error at 1880 x 1118 x 544: 0.67e-6 against 1.01e-6,
 // where plain float32 sums have 0.59e-6) for 276 us against 260, 1.5 % of a
 // whole call. The logits take 256 (284 us against 318).
+constexpr int SGROUP_SCALED = kSplitGroup / SBK;
 template <bool LOGITS>
-constexpr int group_stages() { return LOGITS ? 8 : 4; }
+constexpr int group_stages() { return LOGITS ? 8 : SGROUP_SCALED; }
 constexpr int SGROUP_MAX = 8;
 constexpr int STHREADS = 384;
 constexpr uint32_t PLANE_BYTES = SBM * SBK * 2;  // one plane of one operand, 8 KB
@@ -90,13 +97,14 @@ struct SplitArgs {
   int64_t kept_from;
   int kept_k;  // the rows that there are limit K, not M
   const int32_t* row_index;
-  const SplitScale* scale;
+  const float *scale, *group_scale;
+  int64_t group_ld;
   float* out;
   int64_t ldc;
   int accumulate;
   int vec;     // out's rows are 16-byte aligned
   int m_fast;  // consecutive tiles share their columns of C, else their rows
-  const float* bias;
+  const float *row_scale, *col_scale, *bias;
   const int32_t* labels;
   float2* strips;
   int64_t strip_rows;
@@ -133,7 +141,7 @@ __device__ __forceinline__ SplitSizes actual_sizes(const SplitArgs& s, const Spl
   return z;
 }
 
-// Unit u: tile (mt, nt) over the stages [kb, ke); the split index or -1.
+// Unit u: tile (mt, nt) over the stages [kb, ke), kb at a group's first; the split index or -1.
 __device__ __forceinline__ int split_unit(int u, int m_tiles, int n_tiles, int m_fast, const SplitSizes& su, int num_k,
                                           int& t, int& mt, int& nt, int& kb, int& ke) {
   const int tiles = m_tiles * n_tiles;
@@ -143,8 +151,9 @@ __device__ __forceinline__ int split_unit(int u, int m_tiles, int n_tiles, int m
     const int rest = tiles - su.whole, v = u - su.whole;
     sidx = v / rest;
     t = su.whole + (v - sidx * rest);
-    kb = (int)((int64_t)sidx * num_k / su.splits);
-    ke = (int)((int64_t)(sidx + 1) * num_k / su.splits);
+    const int groups = (num_k + SGROUP_SCALED - 1) / SGROUP_SCALED;
+    kb = min(num_k, (int)((int64_t)sidx * groups / su.splits) * SGROUP_SCALED);
+    ke = min(num_k, (int)((int64_t)(sidx + 1) * groups / su.splits) * SGROUP_SCALED);
   }
   if (m_fast)
     nt = t / m_tiles, mt = t - nt * m_tiles;
@@ -185,11 +194,14 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t tmem_d, uint64_t adesc, ui
       : "memory");
 }
 
-// One operand's stage: both planes. K-major: one box {32, 128, 2}; M/N-major:
-// a box {64, 32, 2} per 64 values.
-template <bool MN>
+// One operand's stage: both planes. K-major: one box {32, 128, 2}, or, grouped,
+// a box {32, 1, 1, 128} per plane; M/N-major: a box {64, 32, 2} per 64 values.
+template <bool MN, bool GROUPED>
 __device__ __forceinline__ void split_load(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int k0) {
-  if (MN) {
+  if (GROUPED) {
+    tma_load_4d(dst, map, bar, k0 % kSplitGroup, 0, k0 / kSplitGroup, row);
+    tma_load_4d(dst + PLANE_BYTES, map, bar, k0 % kSplitGroup, 1, k0 / kSplitGroup, row);
+  } else if (MN) {
     tma_load_3d(dst, map, bar, row, k0, 0);
     tma_load_3d(dst + PLANE_BYTES, map, bar, row + 64, k0, 0);
   } else {
@@ -213,8 +225,6 @@ __device__ __forceinline__ float4* block_chunk(float* xpose, int r, int c) {
 __device__ __forceinline__ float& block_at(float* xpose, int r, int c) {
   return xpose[r * 32 + ((((c >> 2) ^ (r & 7)) << 2) | (c & 3))];
 }
-
-__device__ __forceinline__ float apply(const SplitScale& s, float v) { return __fmul_rn(__fmul_rn(v, s.c1), s.c2); }
 
 // tcgen05.ld of 32 columns without waiting, and the wait for all loads before.
 __device__ __forceinline__ void tmem_issue32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -245,7 +255,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   SplitShared* sh = (SplitShared*)(smem + SBAR_OFFSET);
   constexpr int SGROUP = group_stages<LOGITS>();
-  constexpr bool INDEXED = !A_MN && !LOGITS;  // dx: the rows of C are scattered
+  constexpr bool INDEXED = !A_MN && !LOGITS;  // dx: A is grouped, the rows of C are scattered
   volatile int* failed = &sh->failed;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -305,8 +315,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
             uint64_t* bar = &sh->full[st];
             uint8_t* stage = smem + st * SSTAGE_BYTES;
             mbar_expect_tx(bar, SSTAGE_BYTES);
-            split_load<A_MN>(stage, &tmA, bar, a_row, kt * SBK);
-            split_load<B_MN>(stage + OPER_BYTES, &tmB, bar, b_row, kt * SBK);
+            split_load<A_MN, INDEXED>(stage, &tmA, bar, a_row, kt * SBK);
+            split_load<B_MN, false>(stage + OPER_BYTES, &tmB, bar, b_row, kt * SBK);
           }
           __syncwarp();
           issued_to = it + 1;
@@ -398,7 +408,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
     const int q = warp & 3, h = (warp - 4) >> 2;
     const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16) + 128 * h;
     float* xpose = (float*)(smem + SEPI_OFFSET) + (warp - 4) * 32 * 32;
-    const SplitScale sc = *s.scale;
+    const float sc = LOGITS ? 1.0f : *s.scale;
     int group = 0;
     for (int u = pair; u < units && !__shfl_sync(0xffffffffu, *failed, 0); u += pairs) {
       int t, mt, nt, kb, ke;
@@ -415,7 +425,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
       }
       const int32_t label = LOGITS && lane < rows ? s.labels[m0 + lane] : -1;
       float bias[LOGITS ? 4 : 1];
+      // the row's scale as a factor of at most 1 and one of at least 1, on either side of the
+      // column's, so that no product on the way leaves the range that the last one is in
+      float down = 1.0f, up_again = 1.0f;
       if constexpr (LOGITS) {
+        const float r = lane < rows ? s.row_scale[m0 + lane] : 1.0f;
+        down = fminf(r, 1.0f), up_again = fmaxf(r, 1.0f);
 #pragma unroll
         for (int j = 0; j < 4; j++) bias[j] = s.bias && n0 + 32 * j + lane < s.N ? __ldg(s.bias + n0 + 32 * j + lane) : 0.0f;
       }
@@ -425,6 +440,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
       bool ok = true;
       for (int g = 0; g < groups; g++, group++) {
         const uint32_t buf = (uint32_t)(group & 1);
+        float gs = 1.0f;  // the group's scale of this lane's row, on its way during the wait
+        if constexpr (!LOGITS) {
+          if (lane < rows) gs = s.group_scale[(int64_t)(kb / SGROUP + g) * s.group_ld + m0 + lane];
+        }
         if (!__all_sync(0xffffffffu, mbar_wait(&sh->pfull[buf], (group >> 1) & 1, 7, su.wait_limit_ns))) {
           *failed = 1;
           ok = false;
@@ -439,7 +458,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
           for (int j = 0; j < 4; j++) {  // the next chunk's load runs under this one's adds
             if (j < 3) tmem_issue32(lane_base + buf * 256 + 32 * (j + 1), p[(j + 1) & 1]);
 #pragma unroll
-            for (int i = 0; i < 32; i++) tot[32 * j + i] = __fadd_rn(tot[32 * j + i], __uint_as_float(p[j & 1][i]));
+            for (int i = 0; i < 32; i++) {
+              const float v = __uint_as_float(p[j & 1][i]);
+              tot[32 * j + i] = LOGITS ? __fadd_rn(tot[32 * j + i], v) : __fmaf_rn(v, gs, tot[32 * j + i]);
+            }
             if (j < 3) tmem_wait32(p[(j + 1) & 1]);
           }
         }
@@ -467,9 +489,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
           default: split_chunk<3>(z, tot); break;
         }
         const int nb = n0 + 32 * j, cols = part ? 32 : max(0, min(32, (int)s.N - nb));
-        if (!part) {
+        if constexpr (LOGITS) {
+          const float4* cs = reinterpret_cast<const float4*>(s.col_scale + nb);  // the same for all lanes
 #pragma unroll
-          for (int i = 0; i < 32; i++) z[i] = apply(sc, z[i]);
+          for (int c = 0; c < 8; c++) {
+            const float4 f = cs[c];
+            z[4 * c] = __fmul_rn(__fmul_rn(__fmul_rn(z[4 * c], down), f.x), up_again);
+            z[4 * c + 1] = __fmul_rn(__fmul_rn(__fmul_rn(z[4 * c + 1], down), f.y), up_again);
+            z[4 * c + 2] = __fmul_rn(__fmul_rn(__fmul_rn(z[4 * c + 2], down), f.z), up_again);
+            z[4 * c + 3] = __fmul_rn(__fmul_rn(__fmul_rn(z[4 * c + 3], down), f.w), up_again);
+          }
+        } else if (!part) {
+#pragma unroll
+          for (int i = 0; i < 32; i++) z[i] = __fmul_rn(z[i], sc);
         }
         if constexpr (LOGITS) {
           if (s.bias) {
@@ -577,7 +609,7 @@ __global__ void split_reduce_kernel(SplitUnits su, SplitArgs s) {
   const int m_tiles = (sz.M + STILE - 1) / STILE, n_tiles = (int)((s.N + STILE - 1) / STILE);
   const int rest = m_tiles * n_tiles - sz.whole;
   const int64_t total = (int64_t)rest * STILE_ELEMS;
-  const SplitScale sc = *s.scale;
+  const float sc = *s.scale;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int r = (int)(i / STILE_ELEMS), e = (int)(i - (int64_t)r * STILE_ELEMS), t = sz.whole + r;
     const int mt = s.m_fast ? t % m_tiles : t / n_tiles, nt = s.m_fast ? t / m_tiles : t % n_tiles;
@@ -586,7 +618,7 @@ __global__ void split_reduce_kernel(SplitUnits su, SplitArgs s) {
     float acc = su.ws[i];
     for (int k = 1; k < sz.splits; k++) acc = __fadd_rn(acc, su.ws[(int64_t)k * total + i]);
     float* o = s.out + (s.row_index ? (int64_t)s.row_index[m] : m) * s.ldc + n;
-    acc = apply(sc, acc);
+    acc = __fmul_rn(acc, sc);
     *o = s.accumulate ? __fadd_rn(*o, acc) : acc;
   }
 }
@@ -594,6 +626,16 @@ __global__ void split_reduce_kernel(SplitUnits su, SplitArgs s) {
 static char* split_map(gt_ctx* ctx, CUtensorMap* map, const HalfPlanes& p, bool mn) {
   auto encode = (EncodeTiledFn)ctx->encode_tiled;
   if (!encode) return errorf("split_gemm: cuTensorMapEncodeTiled is unavailable");
+  if (p.grouped) {
+    cuuint64_t dims[4] = {kSplitGroup, 2, (cuuint64_t)(p.pitch / (2 * kSplitGroup)), (cuuint64_t)p.rows};
+    cuuint64_t strides[3] = {kSplitGroup * 2, kSplitGroup * 4, (cuuint64_t)p.pitch * 2};
+    cuuint32_t box[4] = {(cuuint32_t)SBK, 1, 1, (cuuint32_t)SBM}, estr[4] = {1, 1, 1, 1};
+    CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, (void*)p.base, dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return errorf("split_gemm: cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return nullptr;
+  }
   cuuint64_t dims[3] = {(cuuint64_t)p.cols, (cuuint64_t)p.rows, 2};
   cuuint64_t strides[2] = {(cuuint64_t)p.pitch * 2, (cuuint64_t)p.plane_elems * 2};
   cuuint32_t box[3] = {mn ? 64u : (cuuint32_t)SBK, mn ? (cuuint32_t)SBK : (cuuint32_t)SBM, 2};
@@ -656,8 +698,9 @@ static char* split_launch(gt_ctx* ctx, const SplitGemm& g) {
   su.wait_limit_ns = tc_wait_limit_ns();
   su.withhold = tc_take_withhold();
   const int vec = (((uintptr_t)g.out & 15) | (g.ldc & 3)) == 0;
-  SplitArgs s{g.M,   g.N,          g.K, g.kept,      g.kept_from, A_MN,     g.row_index, g.scale,      g.out,
-              g.ldc, g.accumulate, vec, g.N > g.M,   g.bias,      g.labels, g.strips,    g.strip_rows, g.picked};
+  SplitArgs s{g.M,    g.N,        g.K,     g.kept,      g.kept_from, A_MN,        g.row_index, g.scale,  g.group_scale,
+              g.group_ld, g.out,  g.ldc,   g.accumulate, vec,        g.N > g.M,   g.row_scale, g.col_scale, g.bias,
+              g.labels, g.strips, g.strip_rows, g.picked};
   void* ws = nullptr;
   if (su.splits > 1) {
     // (with fewer rows than planned, the tiles split in the last round may be up to one per pair)
@@ -684,11 +727,14 @@ char* split_gemm(gt_ctx* ctx, const SplitGemm& g) {
   if (ctx->sm_count < 2) return errorf("split_gemm: needs a pair of SMs");
   g_split_used = true;
   if (g.strips) {
-    if (g.a_mn || g.b_mn) return errorf("split_gemm: the logits' operands are K-major");
+    if (g.a_mn || g.b_mn || g.a.grouped) return errorf("split_gemm: the logits' operands are K-major");
+    if (!g.row_scale || !g.col_scale) return errorf("split_gemm: the logits' scales are missing");
     return tc::split_launch<false, false, true>(ctx, g);
   }
   if (g.a_mn ? g.row_index != nullptr : !g.row_index || g.accumulate)
     return errorf("split_gemm: an index of rows goes with K-major A and no accumulation");
+  if (g.a_mn == g.a.grouped || !g.scale || !g.group_scale)
+    return errorf("split_gemm: K-major A comes in groups, and every group has its scales");
   if (!g.a_mn && g.b_mn) return tc::split_launch<false, true, false>(ctx, g);
   if (g.a_mn && g.b_mn) return tc::split_launch<true, true, false>(ctx, g);
   return errorf("split_gemm: layout not built");

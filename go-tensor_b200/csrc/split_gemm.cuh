@@ -8,23 +8,25 @@
 namespace gt {
 
 // A float32 matrix (rows x cols) as two float16 planes, hi = half(x s) and
-// lo = half(x s - hi) with s a power of two: base[plane * plane_elems + row *
-// pitch + col]. pitch and plane_elems are multiples of 8 and the base is
-// 16-byte aligned (TMA).
+// lo = half(x s - hi) with s a power of two per row (or, for G, per row or
+// column of a group): base[plane * plane_elems + row * pitch + col]. pitch and
+// plane_elems are multiples of 8 and the base is 16-byte aligned (TMA).
+// grouped: 128 columns of a row lie together, hi before lo: base[row * pitch +
+// col / 128 * 256 + plane * 128 + col % 128]; the pitch is a multiple of 256 and
+// what lies behind cols in the last group is zero.
 struct HalfPlanes {
   const __half* base = nullptr;
   int64_t rows = 0, cols = 0, pitch = 0, plane_elems = 0;
+  bool grouped = false;
 };
 
-// The two factors that an accumulator is multiplied by, in order: c2 is 1
-// unless one power of two cannot hold the scale.
-struct SplitScale {
-  float c1, c2;
-};
+// Values of K that share a scale of A in dx and dw, and classes per strip.
+constexpr int kSplitGroup = 128;
 
 // C (M x N) = A (M x K) B (K x N). A is stored with rows M and columns K, or
 // with rows K and columns M (a_mn); B with rows N and columns K, or with rows
-// K and columns N (b_mn).
+// K and columns N (b_mn). The logits: both K-major; dx: A K-major and grouped, B
+// N-major; dw: both M/N-major.
 struct SplitGemm {
   int64_t M = 0, N = 0, K = 0;
   // The rows (a_mn: the K) that there really are, known on the device only:
@@ -35,14 +37,20 @@ struct SplitGemm {
   const int32_t* row_index = nullptr;  // row m of C goes to row row_index[m] of out
   HalfPlanes a, b;
   bool a_mn = false, b_mn = false;
-  const SplitScale* scale = nullptr;  // device
+  // dx, dw: C = scale * sum over the groups of kSplitGroup values of K of group_scale[group *
+  // group_ld + row] * (the group's products). Both on the device.
+  const float* scale = nullptr;
+  const float* group_scale = nullptr;
+  int64_t group_ld = 0;
   float* out = nullptr;               // row-major, pitch ldc; logits: may be NULL
   int64_t ldc = 0;
   bool accumulate = false;  // out += instead of out =
-  // The logits' epilogue (strips set): out = C + bias, and for every row and
+  // The logits (strips set): C = row_scale[row] * col_scale[col] * products
+  // (powers of two; col_scale has room for a multiple of 256), out = C + bias, and for every row and
   // strip of kStripCols columns the maximum of C + bias and the sum of exp(. -
   // maximum), at strips[strip * strip_rows + row]; the label's logit goes to
   // picked[row].
+  const float *row_scale = nullptr, *col_scale = nullptr;
   const float* bias = nullptr;
   const int32_t* labels = nullptr;
   float2* strips = nullptr;

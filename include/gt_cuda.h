@@ -352,6 +352,12 @@ GT_API char* gt_xent_fwd_bwd_noalloc(gt_ctx* ctx, int dtype, const void* logits,
  * dx, and the loss, dw and db of the call are NaN. Infinities and NaN in a row
  * of x that counts, or in w, may turn any output that depends on them into
  * NaN.
+ * float32: with few rows (at most 8, or at most 64 with M K V at most 2^27)
+ * plain float32 sums; else each value of x and w keeps 22 bits down to 2^-16 of
+ * its row's largest magnitude and is off by at most 2^-39 of that below, and
+ * g is held to the same measure beside the up to 128 values of a row (dx) or
+ * of a class (dw) that it is summed with, each weighted with the largest
+ * magnitude of the row of w or x that it multiplies. Sums are float32.
  * The logits exist only in pieces of rows whose workspace stays within
  * workspace_bytes (0: 2 GiB; one piece of 256 rows is used whatever it says;
  * float32 also keeps x and w as split planes, 4 bytes per value). No output may overlap an input or another output. The result does
