@@ -16,8 +16,8 @@
 // bytes. The range that float16 lacks is in the scales, which are powers of
 // two. The operands arrive split (each is used by two GEMMs), so
 // no warp splits them here.
-// Tensor-core accumulation truncates, so, as there, the MMAs accumulate 256
-// (or 128) values of K into one of two partial buffers in tensor memory and promoter
+// Tensor-core accumulation truncates, so, as there, the MMAs accumulate 128
+// values of K into one of two partial buffers in tensor memory and promoter
 // warps add each partial to a total in registers with rounded adds.
 //
 // Work split. A CTA pair (cta_group::2) computes 256 x 256 outputs: each CTA
@@ -44,19 +44,16 @@ namespace tc {
 constexpr int SBM = 128;                         // rows of A and of B per CTA
 constexpr int SBK = 32;                          // K per stage
 constexpr int SSTAGES = 6;
-// Stages per promotion. The sum of a partial is truncated at every MMA, by up
-// to 2^-23 of what it holds by then, so short groups are more exact and long
-// ones leave the epilogue more time under the next tile's first two groups.
-// dx, whose rows of G hold one value near -1 among small ones, takes 128 of K
-// (its error at V = 517: 0.6e-6 of the result against 1.3e-6 with 256), which
-// its long K and few epilogues hide (277 us either way at 2048 x 1024 x
-// 32000). dw takes 128 too (its error at 1880 x 1118 x 544: 0.67e-6 against 1.01e-6,
-// where plain float32 sums have 0.59e-6) for 276 us against 260, 1.5 % of a
-// whole call. The logits take 256 (284 us against 318).
-constexpr int SGROUP_SCALED = kSplitGroup / SBK;
-template <bool LOGITS>
-constexpr int group_stages() { return LOGITS ? 8 : SGROUP_SCALED; }
-constexpr int SGROUP_MAX = 8;
+// Stages per promotion: 128 of K, the values that share a scale in dx and dw.
+// The sum of a partial is truncated at every MMA, by up to 2^-23 of what it holds
+// by then, always towards zero, so short groups are more exact and long ones leave the
+// epilogue more time under the next tile's first two groups. With 256, sums of positive
+// products came out 13.7 * 2^-23 too small on average, with 128 half of that;
+// dx at V = 517 was off by 1.3e-6 of the result (0.6e-6), dw at 1880 x 1118 x 544 by
+// 1.01e-6 (0.67e-6, where plain float32 sums have 0.59e-6). At 2048 x 1024 x 32000: logits 318 us
+// against 284 with 256, dw 276 against 260, dx 277 either way.
+constexpr int SGROUP = kSplitGroup / SBK;
+constexpr int SMIN_SPLIT = 16;                   // stages that a K-split has at least
 constexpr int STHREADS = 384;
 constexpr uint32_t PLANE_BYTES = SBM * SBK * 2;  // one plane of one operand, 8 KB
 constexpr uint32_t OPER_BYTES = 2 * PLANE_BYTES;
@@ -135,7 +132,7 @@ __device__ __forceinline__ SplitSizes actual_sizes(const SplitArgs& s, const Spl
   if (su.splits > 1 && su.whole > 0) {
     z.whole = tiles / su.pairs * su.pairs;
     const int rest = tiles - z.whole;
-    z.splits = rest ? max(1, min(min(su.pairs / rest, 64), (z.K + SBK - 1) / SBK / (2 * SGROUP_MAX))) : 1;
+    z.splits = rest ? max(1, min(min(su.pairs / rest, 64), (z.K + SBK - 1) / SBK / SMIN_SPLIT)) : 1;
   }
   if (z.splits == 1) z.whole = tiles;
   return z;
@@ -151,9 +148,9 @@ __device__ __forceinline__ int split_unit(int u, int m_tiles, int n_tiles, int m
     const int rest = tiles - su.whole, v = u - su.whole;
     sidx = v / rest;
     t = su.whole + (v - sidx * rest);
-    const int groups = (num_k + SGROUP_SCALED - 1) / SGROUP_SCALED;
-    kb = min(num_k, (int)((int64_t)sidx * groups / su.splits) * SGROUP_SCALED);
-    ke = min(num_k, (int)((int64_t)(sidx + 1) * groups / su.splits) * SGROUP_SCALED);
+    const int groups = (num_k + SGROUP - 1) / SGROUP;
+    kb = min(num_k, (int)((int64_t)sidx * groups / su.splits) * SGROUP);
+    ke = min(num_k, (int)((int64_t)(sidx + 1) * groups / su.splits) * SGROUP);
   }
   if (m_fast)
     nt = t / m_tiles, mt = t - nt * m_tiles;
@@ -254,7 +251,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   SplitShared* sh = (SplitShared*)(smem + SBAR_OFFSET);
-  constexpr int SGROUP = group_stages<LOGITS>();
   constexpr bool INDEXED = !A_MN && !LOGITS;  // dx: A is grouped, the rows of C are scattered
   volatile int* failed = &sh->failed;
 
@@ -659,7 +655,7 @@ static SplitUnits split_plan(int64_t tiles, int64_t pairs, int64_t num_k) {
   auto traffic = [&](int64_t t, int S) { return (S + 1) * (double)t * STILE_ELEMS * 4.0 / 5e6 / 0.42; };
   const double base = rounds(tiles) * (num_k + kOverhead);
   double cost = base;
-  for (int S = 2; S <= 64 && num_k / S >= 2 * SGROUP_MAX; S++) {
+  for (int S = 2; S <= 64 && num_k / S >= SMIN_SPLIT; S++) {
     const double per = std::ceil((double)num_k / S) + kOverhead;
     if ((double)S * tiles * STILE_ELEMS * 4 <= (double)(1 << 30)) {
       const double c = rounds(tiles * S) * per + traffic(tiles, S);

@@ -132,3 +132,18 @@ def test_far_apart_in_several_pieces(workspace):
     x, w, b, y = inputs(900, 130, 1500, 6, 0, gain=10.0, ignored=0.3)
     x[::50] *= np.float32(100)
     compare(Head(x, w, b, y, 0, workspace_bytes=workspace).call().host(), *reference(x, w, b, y))
+
+
+@pytest.mark.parametrize("K", [512, 1000, 2048])
+def test_truncated_sums_stay_short(K):
+    """Sums of positive products, where truncation adds up: a label of weight 0 makes a row's loss the other class'
+    logit. Of 24 additions within 128 terms, the s-th truncates a sum that is s / 24 of the partial one by half a unit of
+    2^-23 at most on average: 6.25 * 2^-23 of the logit in all, and 2^-22 for the dropped products; the roundings are as
+    often up as down (2^-24 / 10 for the mean of 300 rows)."""
+    rng = np.random.default_rng(8)
+    x, w = rng.uniform(1, 2, (300, K)).astype(np.float32), rng.uniform(1, 2, (2, K)).astype(np.float32)
+    w[0] = 0
+    got = Head(x, w, None, np.zeros(300, np.int64), 0, outputs=("rows",)).call().host()["rows"]
+    z = x.astype(np.float64) @ w[1].astype(np.float64)
+    off = float(((got - z) / z).mean())
+    assert abs(off) <= 6.25 * 2.0 ** -23 + 2.0 ** -22 + 2.0 ** -24 / 10
