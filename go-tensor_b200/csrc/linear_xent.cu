@@ -88,7 +88,7 @@ __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
 // w and the rows of x that count, in their order, as planes of pitch Kp, a warp
 // per row: index[j] = the j-th such row, y[j] its label, xs[j] and ws[v] what the
 // rows' values in the planes are to be multiplied by; an ignored row's dx
-// and loss are 0. The row is read twice, the second time from cache (its
+// and loss are 0. The row's first 1024 values stay in registers, the rest is read twice, the second time from cache (the row's
 // largest magnitude is wanted first). Behind the last row of x come zeros up to a multiple of 32
 // rows (dw's products read that far). A row's place is the number of rows that
 // count before it: the counts of the 1024-row blocks before its own, and a
@@ -146,43 +146,76 @@ __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restr
     __half* hi = (is_x ? xp : wp) + to * Kp;
     __half* lo = hi + (is_x ? M : V) * Kp;
     const bool vec = (K & 7) == 0 && ((uintptr_t)src & 15) == 0;
+    auto load8 = [&](int64_t k, float (&v)[8]) {
+      const float4 a = reinterpret_cast<const float4*>(src)[2 * k], b = reinterpret_cast<const float4*>(src)[2 * k + 1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    };
+    float held[4][8];  // the row's first 1024 values
     uint32_t top = 0;
-    if (!keep) {
-    } else if (vec) {
-      for (int64_t k = lane; k < K / 4; k += 128) {  // four loads in flight
-        float4 v[4];
+    if (vec) {
 #pragma unroll
-        for (int u = 0; u < 4; u++)
-          v[u] = k + 32 * u < K / 4 ? reinterpret_cast<const float4*>(src)[k + 32 * u] : float4{0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < 4; u++) {
 #pragma unroll
-        for (int u = 0; u < 4; u++) top = max(top, finite_bits4(v[u]));
+        for (int j = 0; j < 8; j++) held[u][j] = 0.0f;
+        if (keep && lane + 32 * u < K / 8) load8(lane + 32 * u, held[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = max(top, finite_bits(held[u][j]));
+      if (keep) {
+#pragma unroll 4
+        for (int64_t k = 256 + lane; k < K / 4; k += 32) top = max(top, finite_bits4(reinterpret_cast<const float4*>(src)[k]));
       }
     } else {
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const int64_t k = lane + 32 * (8 * u + j);
+          held[u][j] = keep && k < K ? src[k] : 0.0f;
+        }
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = max(top, finite_bits(held[u][j]));
+      if (keep) {
 #pragma unroll 8
-      for (int64_t k = lane; k < K; k += 32) top = max(top, finite_bits(src[k]));
+        for (int64_t k = 1024 + lane; k < K; k += 32) top = max(top, finite_bits(src[k]));
+      }
     }
     const int e = plane_exponent(__reduce_max_sync(0xffffffffu, top));
     const float f = exp2_int(e);
     if (lane == 0) (is_x ? xs : ws)[to] = exp2_int(-e);
     if (vec) {
-      for (int64_t k = lane; k < K / 8; k += 32) {
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-        if (keep) a = reinterpret_cast<const float4*>(src)[2 * k], b = reinterpret_cast<const float4*>(src)[2 * k + 1];
-        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      auto store8 = [&](int64_t k, const float (&v)[8]) {
         __align__(16) __half h[8], l[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) split_half(__fmul_rn(v[j], f), h[j], l[j]);
         reinterpret_cast<uint4*>(hi)[k] = *reinterpret_cast<uint4*>(h);
         reinterpret_cast<uint4*>(lo)[k] = *reinterpret_cast<uint4*>(l);
+      };
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+        if (lane + 32 * u < K / 8) store8(lane + 32 * u, held[u]);
+      for (int64_t k = 128 + lane; k < K / 8; k += 32) {
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (keep) load8(k, v);
+        store8(k, v);
       }
     } else {
-      for (int64_t k = lane; k < K; k += 256) {  // eight loads in flight
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = keep && k + 32 * j < K ? src[k + 32 * j] : 0.0f;
+      auto store1 = [&](int64_t k, const float (&v)[8]) {  // values k, k + 32, ...
 #pragma unroll
         for (int j = 0; j < 8; j++)
           if (k + 32 * j < K) split_half(__fmul_rn(v[j], f), hi[k + 32 * j], lo[k + 32 * j]);
+      };
+#pragma unroll
+      for (int u = 0; u < 4; u++) store1(lane + 256 * u, held[u]);
+      for (int64_t k = 1024 + lane; k < K; k += 256) {  // eight loads in flight
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = keep && k + 32 * j < K ? src[k + 32 * j] : 0.0f;
+        store1(k, v);
       }
     }
   }

@@ -206,13 +206,6 @@ __device__ __forceinline__ void split_load(uint8_t* dst, const CUtensorMap* map,
   }
 }
 
-// The promoters' 32-column chunk J of the running total.
-template <int J>
-__device__ __forceinline__ void split_chunk(float (&z)[32], const float (&tot)[128]) {
-#pragma unroll
-  for (int i = 0; i < 32; i++) z[i] = tot[32 * J + i];
-}
-
 // A 32 x 32 block in a warp's transpose buffer: 16-byte chunk c of row r at
 // chunk c ^ (r % 8), so that 8 rows' same chunk and one row's 8 chunks are both
 // free of bank conflicts.
@@ -420,12 +413,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
         if (sidx < 0 && lane < rows) my_row = s.row_index[m0 + lane] - m0;
       }
       const int32_t label = LOGITS && lane < rows ? s.labels[m0 + lane] : -1;
-      float bias[LOGITS ? 4 : 1];
+      float bias[4];
       // the row's scale as a factor of at most 1 and one of at least 1, on either side of the
       // column's, so that no product on the way leaves the range that the last one is in
       float down = 1.0f, up_again = 1.0f;
       if constexpr (LOGITS) {
         const float r = lane < rows ? s.row_scale[m0 + lane] : 1.0f;
+        if (lane < 4) asm volatile("prefetch.global.L1 [%0];" ::"l"(s.col_scale + n0 + 32 * lane));
         down = fminf(r, 1.0f), up_again = fmaxf(r, 1.0f);
 #pragma unroll
         for (int j = 0; j < 4; j++) bias[j] = s.bias && n0 + 32 * j + lane < s.N ? __ldg(s.bias + n0 + 32 * j + lane) : 0.0f;
@@ -473,17 +467,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
       const int64_t ld = part ? STILE : s.ldc;
       const bool vec = part || s.vec;
       float top = -INFINITY, sum = 0.0f;  // LOGITS: this lane's row over the strip
-      // 32 x 32 blocks through the per-warp buffer (the switch keeps the
-      // register indices static in a loop that is not unrolled).
-#pragma unroll 1
+      // 32 x 32 blocks, what is stored through the per-warp buffer
+#pragma unroll
       for (int j = 0; j < 4; j++) {
         float z[32];
-        switch (j) {
-          case 0: split_chunk<0>(z, tot); break;
-          case 1: split_chunk<1>(z, tot); break;
-          case 2: split_chunk<2>(z, tot); break;
-          default: split_chunk<3>(z, tot); break;
-        }
+#pragma unroll
+        for (int i = 0; i < 32; i++) z[i] = tot[32 * j + i];
         const int nb = n0 + 32 * j, cols = part ? 32 : max(0, min(32, (int)s.N - nb));
         if constexpr (LOGITS) {
           const float4* cs = reinterpret_cast<const float4*>(s.col_scale + nb);  // the same for all lanes
@@ -501,20 +490,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
         }
         if constexpr (LOGITS) {
           if (s.bias) {
-            const float my_bias = j == 0 ? bias[0] : j == 1 ? bias[1] : j == 2 ? bias[2] : bias[3];
 #pragma unroll
-            for (int i = 0; i < 32; i++) z[i] = __fadd_rn(z[i], __shfl_sync(0xffffffffu, my_bias, i));
+            for (int i = 0; i < 32; i++) z[i] = __fadd_rn(z[i], __shfl_sync(0xffffffffu, bias[j], i));
           }
           if (cols < 32) {
 #pragma unroll
             for (int i = 0; i < 32; i++) z[i] = i < cols ? z[i] : -INFINITY;
           }
         }
-#pragma unroll
-        for (int c = 0; c < 8; c++)
-          *block_chunk(xpose, lane, c) = make_float4(z[4 * c], z[4 * c + 1], z[4 * c + 2], z[4 * c + 3]);
-        __syncwarp();
         if (dst) {
+#pragma unroll
+          for (int c = 0; c < 8; c++)
+            *block_chunk(xpose, lane, c) = make_float4(z[4 * c], z[4 * c + 1], z[4 * c + 2], z[4 * c + 3]);
+          __syncwarp();
           if (vec && cols == 32) {  // 4 rows x 128 bytes per access
             const int r0 = lane >> 3, c = lane & 7;
             float* o = dst + (INDEXED ? 0 : (int64_t)r0 * ld) + 32 * j + 4 * c;
@@ -579,7 +567,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
           for (int i = 0; i < 32; i++) add[i & 3] += exp_below(z[i] - from);
           sum = sum * exp_below(top - from) + ((add[0] + add[1]) + (add[2] + add[3]));
           top = up;
-          if (label >= nb && label < nb + cols) s.picked[m0 + lane] = block_at(xpose, lane, label - nb);
+          if (label >= nb && label < nb + cols) {
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+              if (label - nb == i) s.picked[m0 + lane] = z[i];
+          }
         }
         __syncwarp();
       }
