@@ -15,8 +15,8 @@
 //   few_dx_kernel      the partial dx of the runs, added up
 // (few8_logits_kernel and few8_grad_kernel for at most 8 rows)
 //
-// Sums are float32 in runs of at most 256 (logits) or 1024 (dx) terms that are
-// then added up, so they stay as exact as the tensor-core path's.
+// Sums are float32 in runs of at most 256 (logits) or 1024 (dx) terms of a thread
+// that are then added up, so they stay as exact as the tensor-core path's.
 //
 // Measured (the tensor-core path in brackets): 7 x 96 x 517 17 us (62), 64 x 128 x
 // 1000 39 us (82), 64 x 512 x 5000 105 us (103), 8 x 2048 x 50000 395 us (600; w read
@@ -47,6 +47,7 @@ struct FewMeta {
 constexpr int kEight = 8;
 constexpr int kEightStrip = 32;    // classes per block
 constexpr int kEightChunk = 1024;  // K per stage of x
+constexpr int kEightRun = 8;       // stages per run: 256 terms of a lane
 __global__ void __launch_bounds__(256, 2) few8_logits_kernel(const float* __restrict__ x, const float* __restrict__ w,
                                                              const float* __restrict__ bias,
                                                              const int32_t* __restrict__ labels, int M, int64_t K,
@@ -80,7 +81,7 @@ __global__ void __launch_bounds__(256, 2) few8_logits_kernel(const float* __rest
       }
     }
   };
-  float acc[32];  // [class][row]
+  float acc[32], total = 0.0f;  // [class][row]; the sums of earlier runs
 #pragma unroll
   for (int i = 0; i < 32; i++) acc[i] = 0.0f;
   fetch(0);
@@ -111,21 +112,25 @@ __global__ void __launch_bounds__(256, 2) few8_logits_kernel(const float* __rest
               fmaf(a[c].w, b.w, fmaf(a[c].z, b.z, fmaf(a[c].y, b.y, fmaf(a[c].x, b.x, acc[c * kEight + m]))));
       }
     }
-  }
-  // The 32 sums over the lanes by halving exchanges: lane l ends with sum l.
+    if (k0 / kEightChunk % kEightRun != kEightRun - 1 && k0 + kEightChunk < K) continue;
+    // The 32 sums over the lanes by halving exchanges: lane l ends with sum l.
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    const bool up = lane & off;
+    for (int off = 16; off > 0; off >>= 1) {
+      const bool up = lane & off;
 #pragma unroll
-    for (int j = 0; j < off; j++) {
-      const float keep_v = up ? acc[j + off] : acc[j], send = up ? acc[j] : acc[j + off];
-      acc[j] = keep_v + __shfl_xor_sync(0xffffffffu, send, off);
+      for (int j = 0; j < off; j++) {
+        const float keep_v = up ? acc[j + off] : acc[j], send = up ? acc[j] : acc[j + off];
+        acc[j] = keep_v + __shfl_xor_sync(0xffffffffu, send, off);
+      }
     }
+    total += acc[0];
+#pragma unroll
+    for (int i = 0; i < 32; i++) acc[i] = 0.0f;
   }
   {
     const int c = lane / kEight, m = lane % kEight;
     const int64_t v = mine + c;
-    zs[m][4 * warp + c] = v < V ? acc[0] + (bias ? __ldg(bias + v) : 0.0f) : -INFINITY;
+    zs[m][4 * warp + c] = v < V ? total + (bias ? __ldg(bias + v) : 0.0f) : -INFINITY;
   }
   __syncthreads();
   if (warp < M) {

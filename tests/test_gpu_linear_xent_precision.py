@@ -147,3 +147,20 @@ def test_truncated_sums_stay_short(K):
     z = x.astype(np.float64) @ w[1].astype(np.float64)
     off = float(((got - z) / z).mean())
     assert abs(off) <= 6.25 * 2.0 ** -23 + 2.0 ** -22 + 2.0 ** -24 / 10
+
+
+@pytest.mark.parametrize("M", [1, 5, 8])
+@pytest.mark.parametrize("K", [40000, 131072])
+def test_long_sums_of_few_rows(M, K):
+    """At most 8 rows: 32 lanes share a sum. Runs of at most 256 terms per lane, each rounded (2^-24 of what it holds by
+    then: half the run's sum on average for positive products, 128 * 2^-24 at most of it in all), 5 joins of the lanes, and
+    one addition per run."""
+    rng = np.random.default_rng(9)
+    x, w = rng.uniform(1, 2, (M, K)).astype(np.float32), rng.uniform(1, 2, (2, K)).astype(np.float32)
+    x[:] = np.float32(1.9) + np.float32(2.0 ** -20)  # equal terms: the roundings of a run go the same way
+    w[1] = np.float32(1.7) + np.float32(2.0 ** -21)
+    w[0] = 0
+    got = Head(x, w, None, np.zeros(M, np.int64), 0, outputs=("rows",)).call().host()["rows"]
+    z = x.astype(np.float64) @ w[1].astype(np.float64)
+    runs = -(-K // 8192)
+    assert (np.abs((got - z) / z) <= (128 + 5 + runs + 1) * U).all()
