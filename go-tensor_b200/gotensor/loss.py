@@ -13,12 +13,17 @@ from ._lib import FLOAT32, check
 from .backend import Context, CudaStorage
 
 
-def address(buf, n=None, dt=None, what="buffer"):
-    """The device address of a storage (checked for length and dtype) or of an address, None for None."""
+def address(buf, ctx, n=None, dt=None, what="buffer", size=None):
+    """The device address of a storage or of an address, None for None. A storage has to be on ctx's device and is
+    checked for n elements of dtype dt, or, with a size, for n values of that many bytes whatever its own dtype."""
     if buf is None:
         return None
     if isinstance(buf, CudaStorage):
-        if n is not None and buf.n < n:
+        if buf.ctx is not ctx:
+            raise TypeError(f"{what}: the storage is not on cuda:{ctx.index}")
+        if size is not None and buf.nbytes < n * size:
+            raise ValueError(f"{what}: {n * size} bytes wanted, the storage has {buf.nbytes}")
+        if size is None and n is not None and buf.n < n:
             raise ValueError(f"{what}: {n} elements wanted, the storage has {buf.n}")
         if dt is not None and buf.dt != dt:
             raise TypeError(f"{what}: mixed dtypes")
@@ -32,8 +37,12 @@ def linear_cross_entropy(x, w, bias, labels, M, K, V, *, loss, rows=None, dx=Non
     the gradients in ``dx`` (M, K), ``dw`` (V, K) and ``db`` (V); each of the four may be None. ``labels`` and
     ``bad_label`` are addresses of int32 on the device. Rows labelled ``ignore_label`` take no part."""
     ctx = Context.get(device)
+
+    def at(buf, n, what):
+        return address(buf, ctx, n, dtype, what)
+
     check(ctx.lib.gt_linear_xent_fwd_bwd(
-        ctx.ptr, dtype, address(x, M * K, dtype, "x"), address(w, V * K, dtype, "w"), address(bias, V, dtype, "bias"),
-        address(labels), M, K, V, ignore_label, workspace_bytes, address(loss, 1, dtype, "loss"),
-        address(rows, M, dtype, "rows"), address(dx, M * K, dtype, "dx"), address(dw, V * K, dtype, "dw"),
-        address(db, V, dtype, "db"), address(bad_label)))
+        ctx.ptr, dtype, at(x, M * K, "x"), at(w, V * K, "w"), at(bias, V, "bias"),
+        address(labels, ctx, M, None, "labels", size=4), M, K, V, ignore_label, workspace_bytes, at(loss, 1, "loss"),
+        at(rows, M, "rows"), at(dx, M * K, "dx"), at(dw, V * K, "dw"), at(db, V, "db"),
+        address(bad_label, ctx, 1, None, "bad_label", size=4)))

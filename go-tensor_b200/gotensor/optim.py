@@ -37,24 +37,28 @@ class AdamW:
         self.ctx = Context.get(device)
         self.lib = self.ctx.lib
         self.cfg = AdamCfg(lr, beta1, beta2, eps, weight_decay)
-        held = None if state == STATE_E4M3 else dtype
         self.tensors = list(tensors)  # keeps the storages alive
         arr = (AdamwTensor * max(1, len(self.tensors)))()
         for a, t in zip(arr, self.tensors):
-            a.p, a.g = address(t.p, t.n, dtype, "p"), address(t.g, t.n, dtype, "g")
-            a.m = address(t.m, t.n if held is not None else None, held, "m")
-            a.v = address(t.v, t.n if held is not None else None, held, "v")
-            a.m_scale = address(t.m_scale, -(-t.n // BLOCK), FLOAT32, "m_scale")
-            a.v_scale = address(t.v_scale, -(-t.n // BLOCK), FLOAT32, "v_scale")
+            a.p, a.g = self._at(t.p, t.n, dtype, "p"), self._at(t.g, t.n, dtype, "g")
+            if state == STATE_E4M3:  # codes: a byte each, in a storage of any dtype
+                a.m, a.v = self._at(t.m, t.n, None, "m", size=1), self._at(t.v, t.n, None, "v", size=1)
+            else:
+                a.m, a.v = self._at(t.m, t.n, dtype, "m"), self._at(t.v, t.n, dtype, "v")
+            a.m_scale = self._at(t.m_scale, -(-t.n // BLOCK), FLOAT32, "m_scale")
+            a.v_scale = self._at(t.v_scale, -(-t.n // BLOCK), FLOAT32, "v_scale")
             a.n, a.lr_mul, a.wd_mul = t.n, t.lr_mul, t.wd_mul
         self._step = step
         self.dtype = dtype
         self._clip = None
         self.ptr = None
         p = ctypes.c_void_p()
-        check(self.lib.gt_adamw_new(self.ctx.ptr, dtype, state, arr, len(self.tensors), address(step), seed,
-                                    ctypes.byref(p)))
+        check(self.lib.gt_adamw_new(self.ctx.ptr, dtype, state, arr, len(self.tensors),
+                                    self._at(step, 1, None, "step", size=8), seed, ctypes.byref(p)))
         self.ptr = p
+
+    def _at(self, buf, n, dt, what, size=None):
+        return address(buf, self.ctx, n, dt, what, size)
 
     def close(self):
         """Frees the handle (not while the stream is captured)."""
@@ -74,7 +78,7 @@ class AdamW:
         if len(grads) != len(self.tensors):
             raise ValueError(f"{len(grads)} gradients for {len(self.tensors)} tensors")
         arr = (ctypes.c_void_p * max(1, len(grads)))(
-            *[address(g, t.n, self.dtype, "g") for g, t in zip(grads, self.tensors)])
+            *[self._at(g, t.n, self.dtype, "g") for g, t in zip(grads, self.tensors)])
         check(self.lib.gt_adamw_set_grads(self.ptr, arr, len(grads)))
         for t, g in zip(self.tensors, grads):
             t.g = g
@@ -82,7 +86,7 @@ class AdamW:
     def clip_grad_norm(self, max_norm, out):
         """Writes the gradients' global norm and the coefficient min(1, max_norm / norm) to the two doubles at the
         device address ``out``; the next ``step`` multiplies the gradients by it."""
-        out = address(out)
+        out = self._at(out, 2, _lib.FLOAT64, "out")
         check(self.lib.gt_adamw_clip(self.ptr, max_norm, out))
         self._clip = out
 
@@ -92,4 +96,5 @@ class AdamW:
         if lr is not None:
             self.cfg.lr = lr
         clip, self._clip = self._clip, None
-        check(self.lib.gt_adamw_step(self.ptr, ctypes.byref(self.cfg), clip, address(lr_device)))
+        check(self.lib.gt_adamw_step(self.ptr, ctypes.byref(self.cfg), clip,
+                                     self._at(lr_device, 1, _lib.FLOAT64, "lr_device")))
