@@ -34,6 +34,7 @@ class AdamW:
 
     def __init__(self, tensors, *, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,
                  state=STATE_NATIVE, seed=0, dtype=FLOAT32, device=0):
+        self.ptr = None
         self.ctx = Context.get(device)
         self.lib = self.ctx.lib
         self.cfg = AdamCfg(lr, beta1, beta2, eps, weight_decay)
@@ -51,7 +52,6 @@ class AdamW:
         self._step = step
         self.dtype = dtype
         self._clip = None
-        self.ptr = None
         p = ctypes.c_void_p()
         check(self.lib.gt_adamw_new(self.ctx.ptr, dtype, state, arr, len(self.tensors),
                                     self._at(step, 1, None, "step", size=8), seed, ctypes.byref(p)))
@@ -62,9 +62,9 @@ class AdamW:
 
     def close(self):
         """Frees the handle (not while the stream is captured)."""
-        p, self.ptr = self.ptr, None
-        if p:
-            check(self.lib.gt_adamw_free(p))
+        if self.ptr:
+            check(self.lib.gt_adamw_free(self.ptr))
+            self.ptr = None
 
     def __del__(self):
         try:
@@ -86,15 +86,16 @@ class AdamW:
     def clip_grad_norm(self, max_norm, out):
         """Writes the gradients' global norm and the coefficient min(1, max_norm / norm) to the two doubles at the
         device address ``out``; the next ``step`` multiplies the gradients by it."""
-        out = self._at(out, 2, _lib.FLOAT64, "out")
-        check(self.lib.gt_adamw_clip(self.ptr, max_norm, out))
-        self._clip = out
+        check(self.lib.gt_adamw_clip(self.ptr, max_norm, self._at(out, 2, _lib.FLOAT64, "out")))
+        self._clip = out  # (a storage stays alive until the step)
 
     def step(self, lr=None, lr_device=None):
         """One update; ``lr`` replaces the learning rate from here on, ``lr_device`` is a device double that
-        replaces it for this call (and for the replays of a graph that captured it)."""
+        replaces it for this call (and for the replays of a graph that captured it). A refused call changes
+        nothing: the clipping before it goes to the next."""
+        cfg = self.cfg
         if lr is not None:
-            self.cfg.lr = lr
-        clip, self._clip = self._clip, None
-        check(self.lib.gt_adamw_step(self.ptr, ctypes.byref(self.cfg), clip,
+            cfg = AdamCfg(lr, cfg.beta1, cfg.beta2, cfg.eps, cfg.weight_decay)
+        check(self.lib.gt_adamw_step(self.ptr, ctypes.byref(cfg), self._at(self._clip, 2, _lib.FLOAT64, "out"),
                                      self._at(lr_device, 1, _lib.FLOAT64, "lr_device")))
+        self.cfg, self._clip = cfg, None

@@ -87,3 +87,43 @@ def test_adamw_storages_of_another_device(place, name):
     other = place(300, FLOAT32, device=1)
     with pytest.raises(TypeError, match="not on cuda:0"):
         adamw(place, **{name: other})
+
+
+class Calls:
+    """A library that refuses what `refuse` names and counts the rest."""
+
+    def __init__(self):
+        self.refuse, self.seen = set(), []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.seen.append((name, args))
+            if name not in self.refuse:
+                return None
+            lib = _lib.cuda_lib()
+            return lib.gt_adamw_free(None) or lib.gt_adamw_clip(None, 1.0, 16)
+        return call
+
+
+def test_a_refused_call_changes_nothing(place, contexts):
+    contexts[0].lib = lib = Calls()
+    t = optim.Tensor(p=place(300), g=place(300), m=place(300), v=place(300), n=300)
+    opt = optim.AdamW([t], step=0x8000, lr=0.5)
+    opt.ptr = 7
+    clip = place(2, FLOAT64)
+    opt.clip_grad_norm(1.0, clip)
+    lib.refuse = {"gt_adamw_step"}
+    with pytest.raises(GTError):
+        opt.step(lr=0.25)
+    lib.refuse = set()
+    opt.step()
+    name, args = lib.seen[-1]
+    assert name == "gt_adamw_step" and args[2] == clip.ptr and args[1]._obj.lr == 0.5
+    opt.step(lr=0.125)
+    assert lib.seen[-1][1][2] is None and lib.seen[-1][1][1]._obj.lr == 0.125
+    lib.refuse = {"gt_adamw_free"}
+    with pytest.raises(GTError):
+        opt.close()
+    lib.refuse = set()
+    opt.close()
+    assert lib.seen[-1] == ("gt_adamw_free", (7,)) and opt.ptr is None
