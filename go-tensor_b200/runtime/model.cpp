@@ -454,6 +454,7 @@ void Model::set_fused_head(bool on, int32_t ignore_label) {
   if (on) {
     for (auto& buf : acts_)
       if (buf.get() == last.out) buf.reset();
+    logits_.reset();  // of an evaluation, or where the head was switched off
     last.out = nullptr;
   } else if (!last.out) {
     logits_ = DevBuf(ctx_, (size_t)batch_ * classes_ * es_);
