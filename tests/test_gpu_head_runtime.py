@@ -30,3 +30,50 @@ def test_switching_the_head_on_releases_the_logits():
         m.fused_head()
         assert used() <= lean + (1 << 20)
 
+
+def net(kind, dt):
+    """Layers before the head of 50 classes, for a batch of 70: (layers, input shape)."""
+    layers, shape = {
+        "flatten": ([gm.Flatten(), gm.Linear(3 * 4 * 5, 50)], [70, 3, 4, 5]),
+        "activation": ([gm.Linear(20, 30), gm.Flatten(), gm.Tanh(), gm.Linear(30, 50)], [70, 20]),
+        "activation only": ([gm.ReLU(), gm.Linear(20, 50)], [70, 20]),
+        "two linears": ([gm.Linear(20, 30), gm.Linear(30, 50)], [70, 20]),
+        "conv": ([gm.Conv2d(2, 5, 3), gm.ReLU(), gm.Flatten(), gm.Linear(5 * 6 * 6, 50)], [70, 2, 8, 8]),
+        "pool": ([gm.Conv2d(2, 5, 3), gm.ReLU(), gm.MaxPool2d(2), gm.Flatten(), gm.Linear(5 * 3 * 3, 50)], [70, 2, 8, 8]),
+        "two convs": ([gm.Conv2d(2, 5, 3, padding=1), gm.ReLU(), gm.MaxPool2d(2), gm.Conv2d(5, 7, 3), gm.ReLU(),
+                       gm.MaxPool2d(2), gm.Flatten(), gm.Linear(7, 50)], [70, 2, 8, 8]),
+        "pool without relu": ([gm.Conv2d(2, 5, 3), gm.MaxPool2d(3, 1), gm.Flatten(), gm.Linear(5 * 4 * 4, 50)],
+                              [70, 2, 8, 8]),
+    }[kind]
+    m = gm.Model(layers, shape, dtype=dt)
+    t = [np.float32, np.float64][dt]
+    m.set_flat_params((np.random.default_rng(1).standard_normal(m.num_params) * 0.3).astype(t))
+    return m, shape, t
+
+
+@pytest.mark.parametrize("dt,tol", [(0, 1e-4), (1, 1e-10)])
+@pytest.mark.parametrize("kind", ["flatten", "activation", "activation only", "two linears", "conv", "pool", "two convs",
+                                  "pool without relu"])
+def test_layers_before_the_head(kind, dt, tol):
+    """The framework's tolerances between its own paths: 1e-4 and 1e-10 of max(1, value); steps, evaluation between."""
+    m, shape, t = net(kind, dt)
+    rng = np.random.default_rng(2)
+    x, y = rng.standard_normal(shape).astype(t), rng.integers(0, 50, shape[0])
+    m.set_batch(x, y)
+    m.forward_backward()
+    want, loss, logits = m.grads(), m.loss(), m.forward()
+    m.fused_head()
+    m.forward_backward()
+    assert abs(m.loss() - loss) <= tol * max(1, abs(loss))
+    for k, v in m.grads().items():
+        assert (np.abs(v - want[k]) <= tol * np.maximum(1, np.abs(want[k]))).all(), k
+        assert np.abs(want[k]).max() > 1e-4, k
+    assert np.array_equal(m.forward(), logits)
+    before = m.flat_params()
+    m.adamw(lr=1e-3, max_norm=1.0)
+    m.enable_graph(True)
+    losses = []
+    for _ in range(6):
+        m.train_step()
+        losses.append(m.loss())
+    assert np.isfinite(losses).all() and (m.flat_params() != before).any()
