@@ -36,11 +36,12 @@
 
 namespace gt {
 
-// What the kernels of one float32 call share about the rows that count: how
-// many they are, the smallest up_to with that many <= 2^up_to, and 2^up_to / their number
-// (0 when there is none).
+// What the kernels of one float32 call share: how many rows count, n (their
+// number, or what the caller gave), the smallest up_to >= 0 with n <= 2^up_to (at
+// most 31), and 2^up_to / n (0 when no row counts).
 struct XentMeta {
   int64_t count;
+  double n;
   int up_to;
   float share;
 };
@@ -99,7 +100,8 @@ __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restr
                                                             const int32_t* counts, XentMeta* meta, int32_t* index,
                                                             int32_t* y, float* xs, float* ws,
                                                             __half* __restrict__ xp, __half* __restrict__ wp,
-                                                            float* __restrict__ dx, float* rows) {
+                                                            float* __restrict__ dx, float* rows,
+                                                            const double* over) {
   after_predecessor();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // the rows that count before row `end`
@@ -116,10 +118,13 @@ __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restr
   if (blockIdx.x == 0 && warp == 0) {
     const int64_t count = count_before(M);
     if (lane == 0) {
-      const int up_to = count > 1 ? 64 - __clzll(count - 1) : 0;
+      const double n = over ? *over : (double)count;
+      int up_to = 0;
+      while (up_to < 31 && n > (double)((int64_t)1 << up_to)) up_to++;
       meta->count = count;
+      meta->n = n;
       meta->up_to = up_to;
-      meta->share = count ? (float)((double)((int64_t)1 << up_to) / (double)count) : 0.0f;
+      meta->share = count ? (float)((double)((int64_t)1 << up_to) / n) : 0.0f;
     }
   }
   for (int64_t i = (int64_t)blockIdx.x * 8 + warp; i < V + M + 32; i += (int64_t)gridDim.x * 8) {
@@ -442,7 +447,7 @@ __global__ void __launch_bounds__(256) db_kernel(const float* part, int64_t r0, 
   __syncthreads();
   if (warp != 0 || c >= V) return;
   for (int i = 1; i < 8; i++) acc += ws[i][lane];
-  const float d = (float)(meta->count ? acc / (double)meta->count : 0.0);
+  const float d = (float)(meta->count ? acc / meta->n : 0.0);
   db[c] = r0 == 0 ? d : db[c] + d;
 }
 
@@ -494,7 +499,7 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
   GT_LAUNCH_CHECK();
   const int sb = (int)std::min<int64_t>(ceil_div(c.M + c.V + 32, 8), (int64_t)ctx->sm_count * 32);
   GT_CUDA(launch_overlapped(ctx, operand_split_kernel, sb, 256, 0, c.x, c.w, c.labels, c.M, c.K, c.V, Kp, c.ignore,
-                            ws.counts, ws.meta, ws.index, ws.y, ws.xs, ws.ws, ws.x, ws.w, c.dx, c.rows));
+                            ws.counts, ws.meta, ws.index, ws.y, ws.xs, ws.ws, ws.x, ws.w, c.dx, c.rows, c.over));
   const HalfPlanes w{ws.w, c.V, c.K, Kp, c.V * Kp};
   for (int64_t r0 = 0; r0 < c.M; r0 += R) {
     // As many pieces as all rows would need; those behind the rows that count find nothing to do.
@@ -538,7 +543,8 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
       GT_CUDA(launch_overlapped(ctx, db_kernel, (unsigned)ceil_div(c.V, 32), 256, 0, ws.part, r0, r, c.V, ws.meta,
                                 c.db));
   }
-  GT_CUDA(launch_overlapped(ctx, mean_rows_kernel<float>, 1, 1024, 0, ws.losses, c.M, true, &ws.meta->count, c.loss));
+  GT_CUDA(launch_overlapped(ctx, mean_rows_kernel<float>, 1, 1024, 0, ws.losses, c.M, &ws.meta->count, &ws.meta->n,
+                            c.loss));
   return nullptr;
 }
 
@@ -556,29 +562,31 @@ static bool overlap(const Range& a, const Range& b) {
 
 using namespace gt;
 
-extern "C" char* gt_linear_xent_fwd_bwd(gt_ctx* ctx, int dtype, const void* x, const void* w, const void* bias,
+static char* head_call(const char* who, gt_ctx* ctx, int dtype, const void* x, const void* w, const void* bias,
                                         const int32_t* labels, int64_t M, int64_t K, int64_t V, int32_t ignore_label,
                                         int64_t workspace_bytes, void* loss, void* row_loss, void* dx, void* dw,
-                                        void* db, int32_t* bad_label) {
+                                        void* db, int32_t* bad_label,
+                       const double* over) {
   GT_CHECK_DTYPE(dtype);
-  if (!x || !w || !labels || !loss) return errorf("gt_linear_xent_fwd_bwd: null argument");
-  if (M <= 0 || K <= 0 || V <= 0) return errorf("gt_linear_xent_fwd_bwd: M, K and V must be positive");
+  if (!x || !w || !labels || !loss) return errorf("%s: null argument", who);
+  if (M <= 0 || K <= 0 || V <= 0) return errorf("%s: M, K and V must be positive", who);
   if (M > INT32_MAX / 2 || K > INT32_MAX / 2 || V > INT32_MAX / 2)
-    return errorf("gt_linear_xent_fwd_bwd: M, K and V must stay below 2^30");
+    return errorf("%s: M, K and V must stay below 2^30", who);
   if ((double)M * (double)K > 0x1p56 || (double)V * (double)K > 0x1p56)
-    return errorf("gt_linear_xent_fwd_bwd: x and w must stay below 2^56 elements");
-  if (workspace_bytes < 0) return errorf("gt_linear_xent_fwd_bwd: negative workspace");
+    return errorf("%s: x and w must stay below 2^56 elements", who);
+  if (workspace_bytes < 0) return errorf("%s: negative workspace", who);
   const int64_t es = dtype == GT_FLOAT64 ? 8 : 4;
   if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)bias | (uintptr_t)loss | (uintptr_t)row_loss | (uintptr_t)dx |
-        (uintptr_t)dw | (uintptr_t)db) & (es - 1)) || (((uintptr_t)labels | (uintptr_t)bad_label) & 3))
-    return errorf("gt_linear_xent_fwd_bwd: a pointer is not aligned to its elements");
-  const Range in[] = {{x, M * K * es}, {w, V * K * es}, {bias, V * es}, {labels, M * 4}};
+        (uintptr_t)dw | (uintptr_t)db) & (es - 1)) || (((uintptr_t)labels | (uintptr_t)bad_label) & 3) ||
+      ((uintptr_t)over & 7))
+    return errorf("%s: a pointer is not aligned to its elements", who);
+  const Range in[] = {{x, M * K * es}, {w, V * K * es}, {bias, V * es}, {labels, M * 4}, {over, 8}};
   const Range out[] = {{loss, es}, {row_loss, M * es}, {dx, M * K * es}, {dw, V * K * es}, {db, V * es}, {bad_label, 4}};
   for (const Range& o : out) {
     for (const Range& i : in)
-      if (overlap(o, i)) return errorf("gt_linear_xent_fwd_bwd: an output overlaps an input");
+      if (overlap(o, i)) return errorf("%s: an output overlaps an input", who);
     for (const Range& p : out)
-      if (&p != &o && overlap(o, p)) return errorf("gt_linear_xent_fwd_bwd: two outputs overlap");
+      if (&p != &o && overlap(o, p)) return errorf("%s: two outputs overlap", who);
   }
   GT_ENTER(ctx);
   if (workspace_bytes == 0) workspace_bytes = (int64_t)2 << 30;
@@ -586,9 +594,57 @@ extern "C" char* gt_linear_xent_fwd_bwd(gt_ctx* ctx, int dtype, const void* x, c
   char* err = nullptr;
   GT_DISPATCH(dtype, {
     const XentCall<T> c{(const T*)x, (const T*)w, (const T*)bias, labels, M, K, V, ignore_label, workspace_bytes,
-                        (T*)loss, (T*)row_loss, (T*)dx, (T*)dw, (T*)db, bad_label};
+                        (T*)loss, (T*)row_loss, (T*)dx, (T*)dw, (T*)db, bad_label, over};
     err = linear_xent(ctx, c, held);
   });
   for (void* h : held) release(ctx, h);
   return err;
 }
+
+// The number of labels that are not ignore, one block.
+__global__ void __launch_bounds__(1024) count_labels_kernel(const int32_t* __restrict__ labels, int64_t n,
+                                                            int32_t ignore, double* count) {
+  __shared__ int64_t ws[32];
+  int64_t kept = 0;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) kept += labels[i] != ignore;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) kept += __shfl_xor_sync(0xffffffffu, kept, off);
+  if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = kept;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 32; w++) kept += ws[w];
+    *count = (double)kept;
+  }
+}
+
+extern "C" {
+
+char* gt_linear_xent_fwd_bwd(gt_ctx* ctx, int dtype, const void* x, const void* w, const void* bias,
+                             const int32_t* labels, int64_t M, int64_t K, int64_t V, int32_t ignore_label,
+                             int64_t workspace_bytes, void* loss, void* row_loss, void* dx, void* dw, void* db,
+                             int32_t* bad_label) {
+  return head_call("gt_linear_xent_fwd_bwd", ctx, dtype, x, w, bias, labels, M, K, V, ignore_label, workspace_bytes,
+                   loss, row_loss, dx, dw, db, bad_label, nullptr);
+}
+
+char* gt_linear_xent_fwd_bwd_over(gt_ctx* ctx, int dtype, const void* x, const void* w, const void* bias,
+                                  const int32_t* labels, int64_t M, int64_t K, int64_t V, int32_t ignore_label,
+                                  int64_t workspace_bytes, const double* over, void* loss, void* row_loss, void* dx,
+                                  void* dw, void* db, int32_t* bad_label) {
+  if (!over) return errorf("gt_linear_xent_fwd_bwd_over: null argument");
+  return head_call("gt_linear_xent_fwd_bwd_over", ctx, dtype, x, w, bias, labels, M, K, V, ignore_label,
+                   workspace_bytes, loss, row_loss, dx, dw, db, bad_label, over);
+}
+
+char* gt_count_labels(gt_ctx* ctx, const int32_t* labels, int64_t n, int32_t ignore_label, double* count) {
+  if (!labels || !count) return errorf("gt_count_labels: null argument");
+  if (n < 0) return errorf("gt_count_labels: negative length");
+  if (((uintptr_t)labels & 3) || ((uintptr_t)count & 7))
+    return errorf("gt_count_labels: a pointer is not aligned to its elements");
+  GT_ENTER(ctx);
+  count_labels_kernel<<<1, 1024, 0, ctx->stream>>>(labels, n, ignore_label, count);
+  GT_LAUNCH_CHECK();
+  return nullptr;
+}
+
+}  // extern "C"

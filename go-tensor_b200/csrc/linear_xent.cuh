@@ -14,6 +14,7 @@ struct XentCall {
   int64_t workspace;
   T *loss, *rows, *dx, *dw, *db;
   int32_t* bad;
+  const double* over;  // what the sums are divided by; NULL: the number of rows that count
 };
 
 // The pointers of one workspace block.
@@ -71,14 +72,15 @@ __device__ __forceinline__ void join(float2& a, const float2 b) {
   a.x = top;
 }
 
-// loss = sum of the rows' losses / n, in float64, one block, a fixed order.
+// loss = sum of the rows' losses / *n, in float64, one block, a fixed order; listed: only
+// that many rows are there.
 template <typename T>
-__global__ void __launch_bounds__(1024) mean_rows_kernel(const T* rows, int64_t M, bool compact,
-                                                         const int64_t* counts, T* loss) {
+__global__ void __launch_bounds__(1024) mean_rows_kernel(const T* rows, int64_t M, const int64_t* listed,
+                                                         const double* n, T* loss) {
   after_predecessor();
   __shared__ double part[32];
   double acc = 0.0;
-  if (compact) M = counts[0];  // only the rows that count are listed
+  if (listed) M = *listed;
   for (int64_t i = threadIdx.x; i < M; i += blockDim.x) acc += (double)rows[i];
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
@@ -87,7 +89,7 @@ __global__ void __launch_bounds__(1024) mean_rows_kernel(const T* rows, int64_t 
   if (threadIdx.x == 0) {
     acc = 0.0;
     for (int w = 0; w < 32; w++) acc += part[w];
-    *loss = (T)(acc / (double)counts[0]);
+    *loss = (T)(acc / *n);
   }
 }
 

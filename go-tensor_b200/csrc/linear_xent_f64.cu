@@ -22,9 +22,10 @@
 
 namespace gt {
 
-// counts[0] = rows that count (label != ignore); a label outside [0, V) sets *bad.
+// *divisor = rows that count (label != ignore), or *over; a label outside [0, V) sets *bad.
 __global__ void __launch_bounds__(1024) label_count_kernel(const int32_t* __restrict__ labels, int64_t M, int64_t V,
-                                                           int32_t ignore, int64_t* counts, int32_t* bad) {
+                                                           int32_t ignore, const double* over, double* divisor,
+                                                           int32_t* bad) {
   __shared__ int64_t ws[32];
   int64_t n = 0;
   bool outside = false;
@@ -43,7 +44,7 @@ __global__ void __launch_bounds__(1024) label_count_kernel(const int32_t* __rest
   if (threadIdx.x == 0) {
     n = 0;
     for (int w = 0; w < 32; w++) n += ws[w];
-    counts[0] = n;
+    *divisor = over ? *over : (double)n;
   }
 }
 
@@ -88,7 +89,7 @@ __device__ __forceinline__ double block_reduce(double v, double* ws, bool sum) {
 constexpr int kSegment = 4096;
 __global__ void __launch_bounds__(256) xent_segment_kernel(double* z, const int32_t* __restrict__ labels, int64_t V,
                                                            int64_t Vp, int64_t segments, int32_t ignore,
-                                                           const int64_t* counts, double2* pairs, double* picked,
+                                                           const double* divisor, double2* pairs, double* picked,
                                                            double* row_loss, bool grad) {
   after_predecessor();
   __shared__ double ws[8];
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(256) xent_segment_kernel(double* z, const int3
     }
   } else {
     if (threadIdx.x == 0) row_loss[i] = log(s) + (m - label_z);
-    const double inv = 1.0 / (double)counts[0], f = inv / s;
+    const double inv = 1.0 / *divisor, f = inv / s;
 #pragma unroll
     for (int j = 0; j < 16; j++) {
       const int c = 2 * (threadIdx.x + 256 * (j >> 1)) + (j & 1);
@@ -157,7 +158,7 @@ __global__ void __launch_bounds__(256) xent_segment_kernel(double* z, const int3
 // row's loss, and e -> G.
 __global__ void __launch_bounds__(256) xent_scale_kernel(double* z, const int32_t* __restrict__ labels, int64_t V,
                                                          int64_t Vp, int64_t segments, int64_t blocks, int32_t ignore,
-                                                         const int64_t* counts, const double2* pairs,
+                                                         const double* divisor, const double2* pairs,
                                                          const double* picked, double* row_loss, bool grad) {
   after_predecessor();
   __shared__ double ws[8];
@@ -175,7 +176,7 @@ __global__ void __launch_bounds__(256) xent_scale_kernel(double* z, const int32_
   s = block_reduce(s, ws, true);
   if (seg == 0 && threadIdx.x == 0) row_loss[i] = y < 0 || y >= V ? (double)NAN : log(s) + (m - picked[i]);
   if (!grad) return;
-  const double inv = 1.0 / (double)counts[0];
+  const double inv = 1.0 / *divisor;
   const double f = exp(pairs[i * segments + seg].x - from) * (inv / s);
   const int64_t n = min((int64_t)kSegment, V - seg * kSegment), at = (int64_t)y - seg * kSegment;
   double* zr = z + i * Vp + seg * kSegment;
@@ -474,8 +475,7 @@ char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
   int64_t R = std::max<int64_t>(1, c.workspace / (Vp * (int64_t)sizeof(double)));
   R = std::min(c.M, R >= 128 ? R / 128 * 128 : 128);
   struct {
-    int64_t* counts;
-    double *z, *x, *rows, *parts, *picked;
+    double *divisor, *z, *x, *rows, *parts, *picked;
     double2* pairs;
   } ws{};
   // The products of the piece of r rows at r0, one kind at a time.
@@ -502,7 +502,7 @@ char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
     if (c.dw) GT_TRY(dw(0, r, &need));
   }
   auto carve = [&](Carver& k) {
-    ws.counts = k.take<int64_t>(1);
+    ws.divisor = k.take<double>(1);
     ws.z = k.take<double>(R * Vp);
     ws.x = k.take<double>(R * Kp);
     ws.rows = k.take<double>(c.rows ? 0 : c.M);
@@ -516,7 +516,7 @@ char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
   Carver at{(char*)held[0]};
   carve(at);
   double* rows = c.rows ? c.rows : ws.rows;
-  label_count_kernel<<<1, 1024, 0, ctx->stream>>>(c.labels, c.M, c.V, c.ignore, ws.counts, c.bad);
+  label_count_kernel<<<1, 1024, 0, ctx->stream>>>(c.labels, c.M, c.V, c.ignore, c.over, ws.divisor, c.bad);
   GT_LAUNCH_CHECK();
   for (int64_t r0 = 0; r0 < c.M; r0 += R) {
     const int64_t r = std::min(R, c.M - r0);
@@ -525,11 +525,11 @@ char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
                               c.ignore, ws.x));
     GT_TRY(logits(r, nullptr));
     GT_CUDA(launch_overlapped(ctx, xent_segment_kernel, (unsigned)(r * segments), 256, 0, ws.z, labels, c.V, Vp, segments,
-                              c.ignore, ws.counts, ws.pairs, ws.picked, rows + r0, grad));
+                              c.ignore, ws.divisor, ws.pairs, ws.picked, rows + r0, grad));
     if (segments > 1) {
       const int64_t blocks = grad ? segments : 1;
       GT_CUDA(launch_overlapped(ctx, xent_scale_kernel, (unsigned)(r * blocks), 256, 0, ws.z, labels, c.V, Vp, segments,
-                                blocks, c.ignore, ws.counts, ws.pairs, ws.picked, rows + r0, grad));
+                                blocks, c.ignore, ws.divisor, ws.pairs, ws.picked, rows + r0, grad));
     }
     if (c.dx) GT_TRY(dx(r0, r, nullptr));
     if (c.dw) GT_TRY(dw(r0, r, nullptr));
@@ -537,7 +537,7 @@ char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
       GT_CUDA(launch_overlapped(ctx, piece_columns_kernel, (unsigned)ceil_div(c.V, 32), 1024, 0, ws.z, r, c.V, Vp,
                                 r0 == 0, c.db));
   }
-  GT_CUDA(launch_overlapped(ctx, mean_rows_kernel<double>, 1, 1024, 0, rows, c.M, false, ws.counts, c.loss));
+  GT_CUDA(launch_overlapped(ctx, mean_rows_kernel<double>, 1, 1024, 0, rows, c.M, nullptr, ws.divisor, c.loss));
   return nullptr;
 }
 

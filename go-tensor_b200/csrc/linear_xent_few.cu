@@ -254,7 +254,7 @@ template <int MT>
 __global__ void __launch_bounds__(1024) few_join_kernel(const float2* strips, int n, int M,
                                                         const int32_t* __restrict__ labels, int64_t V, int32_t ignore,
                                                         const float* picked, float2* stat,
-                                                        float* rows, float* loss,
+                                                        float* rows, float* loss, const double* over,
                                                         FewMeta* meta, int32_t* bad) {
   after_predecessor();
   constexpr int PARTS = MT >= 32 ? 1 : 32 / MT;
@@ -292,8 +292,9 @@ __global__ void __launch_bounds__(1024) few_join_kernel(const float2* strips, in
   if (threadIdx.x == 0) {
     double sum = 0.0;
     for (int i = 0; i < M; i++) sum += (double)row_loss[i];
-    *loss = (float)(sum / (double)count);
-    meta->inv_n = count ? (float)(1.0 / (double)count) : 0.0f;
+    const double n = over ? *over : (double)count;
+    *loss = (float)(sum / n);
+    meta->inv_n = count ? (float)(1.0 / n) : 0.0f;
   }
 }
 
@@ -601,7 +602,7 @@ static char* few_run(gt_ctx* ctx, const XentCall<float>& c, void** held) {
                                                                        ws.picked);
   GT_LAUNCH_CHECK();
   GT_CUDA(launch_overlapped(ctx, few_join_kernel<MT>, 1, 1024, 0, ws.strips, (int)strips, (int)c.M, c.labels, c.V,
-                            c.ignore, ws.picked, ws.stat, c.rows, c.loss, ws.meta, c.bad));
+                            c.ignore, ws.picked, ws.stat, c.rows, c.loss, c.over, ws.meta, c.bad));
   if (!grad) return nullptr;
   const dim3 grid((unsigned)kb, (unsigned)runs);
   if constexpr (eight) {

@@ -123,6 +123,9 @@ CUDA_API = {
     "gt_adam_step_dev": ("err", [_P, _INT, _P, _P, _P, _P, _I64, ctypes.POINTER(AdamCfg), _P]),
     "gt_linear_xent_fwd_bwd": ("err", [_P, _INT, _P, _P, _P, _P, _I64, _I64, _I64, ctypes.c_int32, _I64, _P, _P, _P,
                                        _P, _P, _P]),
+    "gt_linear_xent_fwd_bwd_over": ("err", [_P, _INT, _P, _P, _P, _P, _I64, _I64, _I64, ctypes.c_int32, _I64, _P, _P,
+                                            _P, _P, _P, _P, _P]),
+    "gt_count_labels": ("err", [_P, _P, _I64, ctypes.c_int32, _P]),
     "gt_adamw_new": ("err", [_P, _INT, _INT, ctypes.POINTER(AdamwTensor), _I64, _P, ctypes.c_uint64,
                              ctypes.POINTER(_P)]),
     "gt_adamw_free": ("err", [_P]),

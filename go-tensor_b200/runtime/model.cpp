@@ -451,6 +451,7 @@ void Model::set_fused_head(bool on, int32_t ignore_label) {
     elems = std::max(elems, numel(ops_[i].in_shape));
   }
   DevBuf a(ctx_, elems * es_), b(ctx_, elems * es_);
+  if (!counted_.get()) counted_ = DevBuf(ctx_, sizeof(double));  // (here: a step may be captured)
   if (on) {
     for (auto& buf : acts_)
       if (buf.get() == last.out) buf.reset();
@@ -475,6 +476,13 @@ void Model::forward(bool train) {
   if (fused_head_ && !train && !ops_.back().out) {  // an evaluation keeps the logits
     logits_ = DevBuf(ctx_, (size_t)batch_ * classes_ * es_);
     ops_.back().out = logits_.get();
+  }
+  if (fused_head_ && train && world_ > 1) {
+    // The ranks' rows that count, averaged while the forward pass runs: the
+    // head divides by it, so that the average of the ranks' losses and
+    // gradients is the mean over the whole batch's.
+    check(gt_count_labels(ctx_, labels_device(), batch_, ignore_label_, (double*)counted_.get()));
+    check(gt_allreduce_avg_async(ctx_, GT_FLOAT64, counted_.get(), 1));
   }
   for (auto& op : ops_) {
     if (fused_head_ && train && &op == &ops_.back()) break;  // with its loss, in backward()
@@ -537,9 +545,17 @@ void Model::backward(bool join) {
   int top = (int)ops_.size() - 1;
   if (fused_head_) {  // the last Linear, the loss and their gradients in one call
     Op& op = ops_.back();
-    check(gt_linear_xent_fwd_bwd(ctx_, dtype_, op.in, p + op.w_off * es_, p + op.b_off * es_, labels_device(), op.M, op.K,
-                                 op.N, ignore_label_, 0, loss_.get(), nullptr, op.needs_dx ? g : nullptr,
-                                 gr + op.w_off * es_, gr + op.b_off * es_, nullptr));
+    void* dx = op.needs_dx ? g : nullptr;
+    if (world_ > 1) {
+      check(gt_comm_wait(ctx_));  // counted_ (nothing else is on its way yet)
+      check(gt_linear_xent_fwd_bwd_over(ctx_, dtype_, op.in, p + op.w_off * es_, p + op.b_off * es_, labels_device(),
+                                        op.M, op.K, op.N, ignore_label_, 0, (const double*)counted_.get(), loss_.get(),
+                                        nullptr, dx, gr + op.w_off * es_, gr + op.b_off * es_, nullptr));
+    } else {
+      check(gt_linear_xent_fwd_bwd(ctx_, dtype_, op.in, p + op.w_off * es_, p + op.b_off * es_, labels_device(), op.M,
+                                   op.K, op.N, ignore_label_, 0, loss_.get(), nullptr, dx, gr + op.w_off * es_,
+                                   gr + op.b_off * es_, nullptr));
+    }
     top--;
   } else if (ops_.back().db_upstream)  // the last Linear's bias gradient in the same pass
     check(gt_xent_fwd_bwd_db(ctx_, dtype_, ops_.back().out, labels_device(), batch_, classes_, loss_.get(), g,

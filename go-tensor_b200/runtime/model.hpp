@@ -201,6 +201,7 @@ class Model {
   double max_norm_ = 0;       // 0: no clipping
   bool fused_head_ = false;
   int32_t ignore_label_ = -1;
+  DevBuf counted_;  // with the fused head and several ranks: the mean of their rows that count
   DevBuf logits_;  // with the fused head: the logits of an evaluation, allocated on first use
   gt_sgd_cfg sgd_{};
   gt_adam_cfg adam_{};

@@ -370,6 +370,18 @@ GT_API char* gt_linear_xent_fwd_bwd(gt_ctx* ctx, int dtype, const void* x, const
                                     int64_t workspace_bytes, void* loss, void* row_loss, void* dx, void* dw, void* db,
                                     int32_t* bad_label);
 
+/* The same with *over (device, above 0) in place of n, for a batch whose rows
+ * are spread over several calls or ranks: with the mean over the ranks of
+ * their counts, the means over the ranks of loss, dw and db are those of the
+ * whole batch, however unevenly its ignored rows lie. A call none of whose
+ * rows counts has the loss 0 / *over and gradients of 0. */
+GT_API char* gt_linear_xent_fwd_bwd_over(gt_ctx* ctx, int dtype, const void* x, const void* w, const void* bias,
+                                         const int32_t* labels, int64_t M, int64_t K, int64_t V, int32_t ignore_label,
+                                         int64_t workspace_bytes, const double* over, void* loss, void* row_loss,
+                                         void* dx, void* dw, void* db, int32_t* bad_label);
+/* *count (device) = how many of the n labels are not ignore_label. */
+GT_API char* gt_count_labels(gt_ctx* ctx, const int32_t* labels, int64_t n, int32_t ignore_label, double* count);
+
 /* Optimizer hyperparameters (optim.SGDConfig / optim.AdamConfig,
  * optim/optim.go:22-27, 74-80). */
 typedef struct {

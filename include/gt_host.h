@@ -87,7 +87,10 @@ GT_API char* gth_grad_norm(gth_model* m, double* out);
  * gradient are then never kept (their buffers are released; an evaluation
  * allocates the logits again). Rows labelled ignore_label take no part in the
  * loss (a value outside the classes to pass over none). The model must end in
- * a Linear. The gradients are those of the separate calls within rounding. */
+ * a Linear. The gradients are those of the separate calls within rounding.
+ * With several ranks (gth_dp_init), every one has to have it on or off alike:
+ * loss and gradients are the mean over all ranks' rows that count, however
+ * many each has. */
 GT_API char* gth_set_fused_head(gth_model* m, int on, int32_t ignore_label);
 
 /* Device buffers the next step reads: the input batch (input_shape, model

@@ -77,3 +77,36 @@ def test_layers_before_the_head(kind, dt, tol):
         m.train_step()
         losses.append(m.loss())
     assert np.isfinite(losses).all() and (m.flat_params() != before).any()
+
+
+@pytest.mark.parametrize("dt", [0, 1])
+@pytest.mark.parametrize("M,K,V", [(10, 40, 333), (30, 40, 333), (300, 40, 333), (300, 33, 9000)])
+@pytest.mark.parametrize("ignored", [(0.0, 0.9, 0.3), (0.2, 1.0, 0.0), (1.0, 1.0, 0.5)])
+def test_shares_of_a_batch(dt, M, K, V, ignored):
+    """Three shards with unequal padding, one call each over the mean of their counts (what three ranks compute): the
+    means of loss, dw and db are those of the whole batch, dx is three times its rows. The shards' bounds add up to the
+    whole's; 8 roundings of the results come on top."""
+    from gotensor.loss import count_labels
+    from test_gpu_adamw import Raw
+    from test_gpu_linear_xent import IGN, Head, Ints, compare, inputs, reference
+    x, w, b, y = inputs(3 * M, K, V, 6, dt)
+    drop = np.concatenate([np.random.default_rng(i).random(M) < p for i, p in enumerate(ignored)])
+    y = np.where(drop, IGN, y)
+    counts = []
+    for i in range(3):
+        n = Raw(np.full(1, -1.0))
+        count_labels(Ints(y[i * M:(i + 1) * M]).ptr, M, count=n.ptr)
+        cuda_backend().Sync()
+        counts.append(n.host()[0])
+        assert counts[-1] == (~drop[i * M:(i + 1) * M]).sum()
+    over = Raw(np.array([np.mean(counts)]))
+    got = [Head(x[i * M:(i + 1) * M], w, b, y[i * M:(i + 1) * M], dt, over=over.ptr).call().host() for i in range(3)]
+    want, tol = reference(x, w, b, y, dt)
+    u = 2.0 ** -53 if dt else 2.0 ** -24
+    mean = {k: np.mean([g[k].astype(np.float64) for g in got], axis=0) for k in ("loss", "dw", "db")}
+    mean["dx"] = np.concatenate([g["dx"].astype(np.float64) / 3 for g in got])
+    mean["rows"] = np.concatenate([g["rows"] for g in got])
+    compare(mean, want, {k: t + 8 * u * np.abs(want[k]) for k, t in tol.items()})
+    for g, n in zip(got, counts):
+        if n == 0:
+            assert g["loss"][0] == 0 and not g["dx"].any() and not g["dw"].any() and not g["db"].any()

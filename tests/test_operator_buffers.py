@@ -127,3 +127,35 @@ def test_a_refused_call_changes_nothing(place, contexts):
     lib.refuse = set()
     opt.close()
     assert lib.seen[-1] == ("gt_adamw_free", (7,)) and opt.ptr is None
+
+
+X, W, B, Y, LOSS, ROWS, DX, DW, DB, BAD, OVER = (0x10000000 * (i + 1) for i in range(11))
+
+
+@pytest.mark.parametrize("kw,message", [
+    ({}, "null context"), ({"over": None}, "over: null"), ({"over": OVER + 4}, "over: a pointer is not aligned"),
+    ({"over": LOSS}, "over: an output overlaps an input"), ({"over": DW + 8}, "overlaps an input"),
+    ({"x": None}, "over: null"), ({"M": 0}, "over: M, K and V")])
+def test_head_over_refuses(kw, message):
+    a = dict(x=X, M=4, over=OVER)
+    a.update(kw)
+    with pytest.raises(GTError, match=message):
+        _lib.check(_lib.cuda_lib().gt_linear_xent_fwd_bwd_over(None, 0, a["x"], W, B, Y, a["M"], 8, 16, -100, 0,
+                                                               a["over"], LOSS, ROWS, DX, DW, DB, BAD))
+
+
+@pytest.mark.parametrize("labels,n,count,message", [(Y, 4, LOSS, "null context"), (None, 4, LOSS, "null"),
+                                                    (Y, 4, None, "null"), (Y, -1, LOSS, "negative"),
+                                                    (Y + 2, 4, LOSS, "aligned"), (Y, 4, LOSS + 4, "aligned")])
+def test_count_labels_refuses(labels, n, count, message):
+    with pytest.raises(GTError, match=message):
+        _lib.check(_lib.cuda_lib().gt_count_labels(None, labels, n, -100, count))
+
+
+def test_over_has_to_be_a_double_of_this_device(place):
+    with pytest.raises(TypeError, match="over"):
+        head(place, over=place(1, FLOAT32))
+    with pytest.raises(TypeError, match="not on"):
+        head(place, over=place(1, FLOAT64, device=1))
+    with pytest.raises(GTError, match="null context"):
+        head(place, over=place(1, FLOAT64))
