@@ -456,12 +456,14 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
   if (few_rows(c.M, c.K, c.V)) return linear_xent_few(ctx, c, held);
   const bool grad = c.dx || c.dw || c.db;
   const int64_t Kp = ceil_div(c.K, 8) * 8, Vp = ceil_div(c.V, kGradTile) * kGradTile, groups = Vp / kGradTile;
-  // Rows per piece: as many as the workspace holds (z and dw's planes of G
-  // take 8 bytes per logit, the strips and scales 16 per 128), in multiples of the tiles'
-  // 256 rows, and the pieces of equal size.
-  const int64_t per_row = (grad ? 8 * Vp : 0) + 16 * groups;
-  int64_t R = std::max<int64_t>(1, c.workspace / per_row / 256) * 256;
+  // Rows per piece: as many as the workspace holds beside the products' partial sums, in multiples of the tiles'
+  // 256 rows, and the pieces of equal size. A row takes 4 bytes per logit for z and 4 for dw's
+  // planes of G, and per 128 logits its strip and the scales and sums of G.
+  const int64_t per_row = (grad ? 4 * Vp : 0) + (c.dw ? 4 * Vp : 0) + 24 * groups + 12;
+  const int64_t rest = c.workspace - std::min(c.workspace / 16, kPartialBytes);
+  int64_t R = std::max<int64_t>(1, rest / per_row / 256) * 256;
   R = std::min(c.M, ceil_div(ceil_div(c.M, ceil_div(c.M, R)), 256) * 256);
+  const int64_t partial_bytes = std::min(kPartialBytes, std::max<int64_t>(0, c.workspace - R * per_row));
   const int64_t row_blocks = ceil_div(c.M, kCompactRows), tiles = ceil_div(R, kGradTile);
   struct {
     XentMeta* meta;
@@ -528,7 +530,7 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
       d.M = r, d.N = c.K, d.K = c.V, d.kept = &ws.meta->count, d.kept_from = r0, d.b = w, d.b_mn = true;
       d.a = HalfPlanes{reinterpret_cast<const __half*>(ws.z), r, c.V, 2 * Vp, 0, true};
       d.scale = &ws.meta->share, d.group_scale = ws.dx_scale, d.group_ld = r;
-      d.out = c.dx, d.ldc = c.K, d.row_index = ws.index + r0;
+      d.out = c.dx, d.ldc = c.K, d.row_index = ws.index + r0, d.partial_bytes = partial_bytes;
       GT_TRY(split_gemm(ctx, d));
     }
     if (c.dw) {
@@ -536,7 +538,7 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
       d.M = c.V, d.N = c.K, d.K = r, d.kept = &ws.meta->count, d.kept_from = r0, d.a_mn = true, d.b = x;
       d.a = HalfPlanes{ws.g, r, c.V, Vp, R * Vp}, d.b_mn = true;
       d.scale = &ws.meta->share, d.group_scale = ws.dw_scale, d.group_ld = c.V;
-      d.out = c.dw, d.ldc = c.K, d.accumulate = r0 > 0;
+      d.out = c.dw, d.ldc = c.K, d.accumulate = r0 > 0, d.partial_bytes = partial_bytes;
       GT_TRY(split_gemm(ctx, d));
     }
     if (c.db)

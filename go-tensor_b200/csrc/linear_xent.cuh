@@ -17,6 +17,10 @@ struct XentCall {
   const double* over;  // what the sums are divided by; NULL: the number of rows that count
 };
 
+// The most that the partial sums of a product's K-splits take. They have a sixteenth of the workspace
+// (at most this), and what the pieces leave of it.
+constexpr int64_t kPartialBytes = (int64_t)128 << 20;
+
 // The pointers of one workspace block.
 struct Carver {
   char* base;

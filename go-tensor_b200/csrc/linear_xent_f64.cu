@@ -205,6 +205,7 @@ struct F64Product {
   const int32_t* labels = nullptr;
   int32_t ignore = 0;
   bool accumulate = false;
+  int64_t partial_bytes = 0;  // the most that the partial sums of K-splits may take
 };
 
 // Units 0 .. whole - 1 are tiles; each further tile is `splits` units over
@@ -400,6 +401,7 @@ static F64Plan f64_plan(const gt_ctx* ctx, const F64Product& p) {
   double least = cost(p.K, 1);
   for (int64_t s = 2; s <= 256 && p.K / s >= 64 && rest * s <= 4 * slots; s++) {
     const int64_t k_per = ceil_div(ceil_div(p.K, s), kF64Depth) * kF64Depth, splits = ceil_div(p.K, k_per);
+    if (rest * splits * T::BM * T::BN * 8 > p.partial_bytes) break;
     const double c = cost(k_per, splits);
     if (c < 0.97 * least) least = c, best.k_per = k_per, best.splits = splits, best.whole = best.tiles - rest;
   }
@@ -472,8 +474,12 @@ __global__ void __launch_bounds__(1024) piece_columns_kernel(const double* g, in
 char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
   const bool grad = c.dx || c.dw || c.db;
   const int64_t Kp = ceil_div(c.K, 2) * 2, Vp = ceil_div(c.V, 2) * 2;  // even: 16-byte copies
-  int64_t R = std::max<int64_t>(1, c.workspace / (Vp * (int64_t)sizeof(double)));
+  const int64_t segments = ceil_div(c.V, kSegment);
+  // Rows per piece: as many as the workspace holds beside the products' partial sums.
+  const int64_t per_row = 8 * Vp + 8 * Kp + (segments > 1 ? 16 * segments + 8 : 0);
+  int64_t R = (c.workspace - std::min(c.workspace / 16, kPartialBytes)) / per_row;
   R = std::min(c.M, R >= 128 ? R / 128 * 128 : 128);
+  const int64_t partial_bytes = std::min(kPartialBytes, std::max<int64_t>(0, c.workspace - R * per_row));
   struct {
     double *divisor, *z, *x, *rows, *parts, *picked;
     double2* pairs;
@@ -481,20 +487,19 @@ char* linear_xent(gt_ctx* ctx, const XentCall<double>& c, void** held) {
   // The products of the piece of r rows at r0, one kind at a time.
   auto logits = [&](int64_t r, int64_t* need) {
     F64Product p{r, c.V, c.K, ws.x, Kp, c.w, c.K, ws.z, Vp};
-    p.bias = c.bias;
+    p.bias = c.bias, p.partial_bytes = partial_bytes;
     return f64_product<true, true>(ctx, p, ws.parts, need);
   };
   auto dx = [&](int64_t r0, int64_t r, int64_t* need) {
     F64Product p{r, c.K, c.V, ws.z, Vp, c.w, c.K, c.dx + r0 * c.K, c.K};
-    p.labels = c.labels + r0, p.ignore = c.ignore;
+    p.labels = c.labels + r0, p.ignore = c.ignore, p.partial_bytes = partial_bytes;
     return f64_product<true, false>(ctx, p, ws.parts, need);
   };
   auto dw = [&](int64_t r0, int64_t r, int64_t* need) {
     F64Product p{c.V, c.K, r, ws.z, Vp, ws.x, Kp, c.dw, c.K};
-    p.accumulate = r0 > 0;
+    p.accumulate = r0 > 0, p.partial_bytes = partial_bytes;
     return f64_product<false, false>(ctx, p, ws.parts, need);
   };
-  const int64_t segments = ceil_div(c.V, kSegment);
   int64_t need = 0;
   for (const int64_t r : {R, c.M - (c.M - 1) / R * R}) {  // a full piece, the last one
     GT_TRY(logits(r, &need));

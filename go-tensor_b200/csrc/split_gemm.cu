@@ -638,8 +638,9 @@ static char* split_map(gt_ctx* ctx, CUtensorMap* map, const HalfPlanes& p, bool 
 // K-splits: whole tiles, every tile split S ways, or only the tiles of the
 // last round, whichever the cost model finds cheapest. In units of a stage on
 // a pair (768 clocks of MMA, 0.42 us): rounds of (stages + a fixed overhead per
-// unit), plus the partials' trip through memory at about 5 TB/s.
-static SplitUnits split_plan(int64_t tiles, int64_t pairs, int64_t num_k) {
+// unit), plus the partials' trip through memory at about 5 TB/s. The partials
+// stay within max_bytes (the last round's may be up to one per pair, see actual_sizes).
+static SplitUnits split_plan(int64_t tiles, int64_t pairs, int64_t num_k, int64_t max_bytes) {
   constexpr double kOverhead = 12.0;
   SplitUnits best;
   best.whole = (int)tiles;
@@ -649,12 +650,12 @@ static SplitUnits split_plan(int64_t tiles, int64_t pairs, int64_t num_k) {
   double cost = base;
   for (int S = 2; S <= 64 && num_k / S >= SMIN_SPLIT; S++) {
     const double per = std::ceil((double)num_k / S) + kOverhead;
-    if ((double)S * tiles * STILE_ELEMS * 4 <= (double)(1 << 30)) {
+    if ((double)S * tiles * STILE_ELEMS * 4 <= (double)max_bytes) {
       const double c = rounds(tiles * S) * per + traffic(tiles, S);
       if (c < cost) cost = c, best.whole = 0, best.splits = S;
     }
     const int64_t full = tiles / pairs * pairs, rest = tiles - full;
-    if (full > 0 && rest > 0 && rest * S <= pairs) {
+    if (full > 0 && rest > 0 && rest * S <= pairs && pairs * STILE_ELEMS * 4 <= max_bytes) {
       const double c = (double)(tiles / pairs) * (num_k + kOverhead) + per + traffic(rest, S);
       if (c < cost) cost = c, best.whole = (int)full, best.splits = S;
     }
@@ -681,7 +682,7 @@ static char* split_launch(gt_ctx* ctx, const SplitGemm& g) {
   if (LOGITS)  // its epilogue needs whole rows of a tile
     su.whole = (int)tiles;
   else
-    su = split_plan(tiles, avail, ceil_div(g.K, SBK));
+    su = split_plan(tiles, avail, ceil_div(g.K, SBK), g.partial_bytes);
   su.pairs = (int)avail;
   su.wait_limit_ns = tc_wait_limit_ns();
   su.withhold = tc_take_withhold();
@@ -692,7 +693,7 @@ static char* split_launch(gt_ctx* ctx, const SplitGemm& g) {
   void* ws = nullptr;
   if (su.splits > 1) {
     // (with fewer rows than planned, the tiles split in the last round may be up to one per pair)
-    const int64_t parts = su.whole > 0 ? std::max(avail, su.splits * (tiles - su.whole)) : su.splits * tiles;
+    const int64_t parts = su.whole > 0 ? avail : su.splits * tiles;
     GT_TRY(scratch(ctx, (size_t)parts * STILE_ELEMS * sizeof(float), &ws));
     su.ws = (float*)ws;
   }

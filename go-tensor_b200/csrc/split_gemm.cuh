@@ -45,6 +45,7 @@ struct SplitGemm {
   float* out = nullptr;               // row-major, pitch ldc; logits: may be NULL
   int64_t ldc = 0;
   bool accumulate = false;  // out += instead of out =
+  int64_t partial_bytes = 0;  // the most that the partial sums of K-splits may take
   // The logits (strips set): C = row_scale[row] * col_scale[col] * products
   // (powers of two; col_scale has room for a multiple of 256), out = C + bias, and for every row and
   // strip of kStripCols columns the maximum of C + bias and the sum of exp(. -

@@ -358,9 +358,14 @@ GT_API char* gt_xent_fwd_bwd_noalloc(gt_ctx* ctx, int dtype, const void* logits,
  * g is held to the same measure beside the up to 128 values of a row (dx) or
  * of a class (dw) that it is summed with, each weighted with the largest
  * magnitude of the row of w or x that it multiplies. Sums are float32.
- * The logits exist only in pieces of rows whose workspace stays within
- * workspace_bytes (0: 2 GiB; one piece of 256 rows is used whatever it says;
- * float32 also keeps x and w as split planes, 4 bytes per value). No output may overlap an input or another output. The result does
+ * The logits exist only in pieces of rows. These, what is kept per logit, and the
+ * products' partial sums stay within workspace_bytes (0: 2 GiB), or are one
+ * piece of 256 rows (float64: 128), about 8 bytes per logit, if that is more.
+ * Beside it float32 keeps x and w as split planes, 4 bytes per value with
+ * rows rounded up to 8 values, 24 bytes per row and 4 per class; float64 8
+ * bytes per row. With few rows (above) a call takes about 5 M V bytes, a
+ * sixteenth of w's and 20 MB whatever workspace_bytes says.
+ * No output may overlap an input or another output. The result does
  * not depend on timing: the same call gives the same bits. Replaces Linear
  * followed by CrossEntropyLoss (nn/module.go:51-53, nn/loss.go:12-14) and
  * their backward for vocabularies whose logits are too large to keep; there
