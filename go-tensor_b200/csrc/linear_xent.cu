@@ -88,17 +88,18 @@ __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
 
 // w and the rows of x that count, in their order, as planes of pitch Kp, a warp
 // per row: index[j] = the j-th such row, y[j] its label, xs[j] and ws[v] what the
-// rows' values in the planes are to be multiplied by; an ignored row's dx
-// and loss are 0. The row's first 1024 values stay in registers, the rest is read twice, the second time from cache (the row's
+// rows' values in the planes are to be multiplied by, wb[v] the class' bias; an
+// ignored row's dx and loss are 0. The row's first 1024 values stay in registers, the rest is read twice, the second time from cache (the row's
 // largest magnitude is wanted first). Behind the last row of x come zeros up to a multiple of 32
 // rows (dw's products read that far). A row's place is the number of rows that
 // count before it: the counts of the 1024-row blocks before its own, and a
 // ballot over the labels of its own (a kernel of its own for this took 4 us more).
 __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restrict__ x, const float* __restrict__ w,
+                                                            const float* __restrict__ bias,
                                                             const int32_t* __restrict__ labels, int64_t M, int64_t K,
                                                             int64_t V, int64_t Kp, int32_t ignore,
                                                             const int32_t* counts, XentMeta* meta, int32_t* index,
-                                                            int32_t* y, float* xs, float* ws,
+                                                            int32_t* y, float* xs, float* ws, float* wb,
                                                             __half* __restrict__ xp, __half* __restrict__ wp,
                                                             float* __restrict__ dx, float* rows,
                                                             const double* over) {
@@ -127,6 +128,8 @@ __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restr
       meta->share = count ? (float)((double)((int64_t)1 << up_to) / n) : 0.0f;
     }
   }
+  for (int64_t v = V + (int64_t)blockIdx.x * 256 + threadIdx.x; v < (V + 255) / 256 * 256; v += (int64_t)gridDim.x * 256)
+    ws[v] = 1.0f, wb[v] = -INFINITY;
   for (int64_t i = (int64_t)blockIdx.x * 8 + warp; i < V + M + 32; i += (int64_t)gridDim.x * 8) {
     const bool is_x = i >= V;
     bool keep = true;
@@ -192,6 +195,7 @@ __global__ void __launch_bounds__(256) operand_split_kernel(const float* __restr
     const int e = plane_exponent(__reduce_max_sync(0xffffffffu, top));
     const float f = exp2_int(e);
     if (lane == 0) (is_x ? xs : ws)[to] = exp2_int(-e);
+    if (lane == 0 && !is_x) wb[to] = bias ? bias[to] : 0.0f;
     if (vec) {
       auto store8 = [&](int64_t k, const float (&v)[8]) {
         __align__(16) __half h[8], l[8];
@@ -468,7 +472,7 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
   struct {
     XentMeta* meta;
     __half *x, *w, *g;
-    float *xs, *ws, *z, *losses, *picked, *part, *dx_scale, *dw_scale;
+    float *xs, *ws, *wb, *z, *losses, *picked, *part, *dx_scale, *dw_scale;
     float2 *strips, *stat;
     int32_t *counts, *index, *y;
   } ws;
@@ -478,6 +482,7 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
     ws.w = k.take<__half>(2 * c.V * Kp);
     ws.xs = k.take<float>(c.M);
     ws.ws = k.take<float>(ceil_div(c.V, 256) * 256);
+    ws.wb = k.take<float>(ceil_div(c.V, 256) * 256);
     ws.g = k.take<__half>(c.dw ? 2 * R * Vp : 0);
     ws.z = k.take<float>(grad ? R * Vp : 0);
     ws.losses = k.take<float>(c.M);
@@ -500,8 +505,8 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
   row_count_kernel<<<(unsigned)row_blocks, 256, 0, ctx->stream>>>(c.labels, c.M, c.V, c.ignore, ws.counts, c.bad);
   GT_LAUNCH_CHECK();
   const int sb = (int)std::min<int64_t>(ceil_div(c.M + c.V + 32, 8), (int64_t)ctx->sm_count * 32);
-  GT_CUDA(launch_overlapped(ctx, operand_split_kernel, sb, 256, 0, c.x, c.w, c.labels, c.M, c.K, c.V, Kp, c.ignore,
-                            ws.counts, ws.meta, ws.index, ws.y, ws.xs, ws.ws, ws.x, ws.w, c.dx, c.rows, c.over));
+  GT_CUDA(launch_overlapped(ctx, operand_split_kernel, sb, 256, 0, c.x, c.w, c.bias, c.labels, c.M, c.K, c.V, Kp,
+                            c.ignore, ws.counts, ws.meta, ws.index, ws.y, ws.xs, ws.ws, ws.wb, ws.x, ws.w, c.dx, c.rows, c.over));
   const HalfPlanes w{ws.w, c.V, c.K, Kp, c.V * Kp};
   for (int64_t r0 = 0; r0 < c.M; r0 += R) {
     // As many pieces as all rows would need; those behind the rows that count find nothing to do.
@@ -510,7 +515,7 @@ static char* linear_xent(gt_ctx* ctx, const XentCall<float>& c, void** held) {
     SplitGemm f;
     f.M = r, f.N = c.V, f.K = c.K, f.kept = &ws.meta->count, f.kept_from = r0, f.a = x, f.b = w;
     f.row_scale = ws.xs + r0, f.col_scale = ws.ws;
-    f.out = grad ? ws.z : nullptr, f.ldc = Vp, f.bias = c.bias, f.labels = ws.y + r0;
+    f.out = grad ? ws.z : nullptr, f.ldc = Vp, f.bias = ws.wb, f.labels = ws.y + r0;
     f.strips = ws.strips, f.strip_rows = R, f.picked = ws.picked;
     GT_TRY(split_gemm(ctx, f));
     GT_CUDA(launch_overlapped(ctx, strip_join_kernel, (unsigned)ceil_div(r, 32), 1024, 0, ws.strips, R,

@@ -407,22 +407,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
       const int rows = max(0, min(32, sz.M - m0));
       // What the epilogue reads besides, fetched while the products run: row m0 +
       // r of C in out (lane r holds it; without an index, and in the
-      // workspace, the r-th), the row's label, the columns' biases.
+      // workspace, the r-th), the row's label, the columns' scales and biases.
       int32_t my_row = lane;
       if constexpr (INDEXED) {
         if (sidx < 0 && lane < rows) my_row = s.row_index[m0 + lane] - m0;
       }
       const int32_t label = LOGITS && lane < rows ? s.labels[m0 + lane] : -1;
-      float bias[4];
       // the row's scale as a factor of at most 1 and one of at least 1, on either side of the
       // column's, so that no product on the way leaves the range that the last one is in
       float down = 1.0f, up_again = 1.0f;
       if constexpr (LOGITS) {
         const float r = lane < rows ? s.row_scale[m0 + lane] : 1.0f;
-        if (lane < 4) asm volatile("prefetch.global.L1 [%0];" ::"l"(s.col_scale + n0 + 32 * lane));
         down = fminf(r, 1.0f), up_again = fmaxf(r, 1.0f);
-#pragma unroll
-        for (int j = 0; j < 4; j++) bias[j] = s.bias && n0 + 32 * j + lane < s.N ? __ldg(s.bias + n0 + 32 * j + lane) : 0.0f;
+        if (lane < 8) asm volatile("prefetch.global.L1 [%0];" ::"l"((lane < 4 ? s.col_scale : s.bias) + n0 + 32 * (lane & 3)));
       }
       float tot[128];
 #pragma unroll
@@ -475,28 +472,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
         for (int i = 0; i < 32; i++) z[i] = tot[32 * j + i];
         const int nb = n0 + 32 * j, cols = part ? 32 : max(0, min(32, (int)s.N - nb));
         if constexpr (LOGITS) {
-          const float4* cs = reinterpret_cast<const float4*>(s.col_scale + nb);  // the same for all lanes
+          // (the same addresses for all lanes; the scales' products are exact, so one rounding, the bias')
+          const float4 *cs = reinterpret_cast<const float4*>(s.col_scale + nb),
+                       *cb = reinterpret_cast<const float4*>(s.bias + nb);
 #pragma unroll
           for (int c = 0; c < 8; c++) {
-            const float4 f = cs[c];
-            z[4 * c] = __fmul_rn(__fmul_rn(__fmul_rn(z[4 * c], down), f.x), up_again);
-            z[4 * c + 1] = __fmul_rn(__fmul_rn(__fmul_rn(z[4 * c + 1], down), f.y), up_again);
-            z[4 * c + 2] = __fmul_rn(__fmul_rn(__fmul_rn(z[4 * c + 2], down), f.z), up_again);
-            z[4 * c + 3] = __fmul_rn(__fmul_rn(__fmul_rn(z[4 * c + 3], down), f.w), up_again);
+            const float4 f = cs[c], b = cb[c];
+            z[4 * c] = __fmaf_rn(__fmul_rn(__fmul_rn(z[4 * c], down), f.x), up_again, b.x);
+            z[4 * c + 1] = __fmaf_rn(__fmul_rn(__fmul_rn(z[4 * c + 1], down), f.y), up_again, b.y);
+            z[4 * c + 2] = __fmaf_rn(__fmul_rn(__fmul_rn(z[4 * c + 2], down), f.z), up_again, b.z);
+            z[4 * c + 3] = __fmaf_rn(__fmul_rn(__fmul_rn(z[4 * c + 3], down), f.w), up_again, b.w);
           }
         } else if (!part) {
 #pragma unroll
           for (int i = 0; i < 32; i++) z[i] = __fmul_rn(z[i], sc);
-        }
-        if constexpr (LOGITS) {
-          if (s.bias) {
-#pragma unroll
-            for (int i = 0; i < 32; i++) z[i] = __fadd_rn(z[i], __shfl_sync(0xffffffffu, bias[j], i));
-          }
-          if (cols < 32) {
-#pragma unroll
-            for (int i = 0; i < 32; i++) z[i] = i < cols ? z[i] : -INFINITY;
-          }
         }
         if (dst) {
 #pragma unroll
@@ -717,7 +706,7 @@ char* split_gemm(gt_ctx* ctx, const SplitGemm& g) {
   g_split_used = true;
   if (g.strips) {
     if (g.a_mn || g.b_mn || g.a.grouped) return errorf("split_gemm: the logits' operands are K-major");
-    if (!g.row_scale || !g.col_scale) return errorf("split_gemm: the logits' scales are missing");
+    if (!g.row_scale || !g.col_scale || !g.bias) return errorf("split_gemm: the logits' scales or biases are missing");
     return tc::split_launch<false, false, true>(ctx, g);
   }
   if (g.a_mn ? g.row_index != nullptr : !g.row_index || g.accumulate)

@@ -47,12 +47,12 @@ struct SplitGemm {
   bool accumulate = false;  // out += instead of out =
   int64_t partial_bytes = 0;  // the most that the partial sums of K-splits may take
   // The logits (strips set): C = row_scale[row] * col_scale[col] * products
-  // (powers of two; col_scale has room for a multiple of 256), out = C + bias, and for every row and
+  // (powers of two), out = C + bias, and for every row and
   // strip of kStripCols columns the maximum of C + bias and the sum of exp(. -
   // maximum), at strips[strip * strip_rows + row]; the label's logit goes to
   // picked[row].
-  const float *row_scale = nullptr, *col_scale = nullptr;
-  const float* bias = nullptr;
+  // Up to a multiple of 256 columns, col_scale is 1 and bias -infinity behind the last.
+  const float *row_scale = nullptr, *col_scale = nullptr, *bias = nullptr;
   const int32_t* labels = nullptr;
   float2* strips = nullptr;
   int64_t strip_rows = 0;

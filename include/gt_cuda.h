@@ -362,7 +362,7 @@ GT_API char* gt_xent_fwd_bwd_noalloc(gt_ctx* ctx, int dtype, const void* logits,
  * products' partial sums stay within workspace_bytes (0: 2 GiB), or are one
  * piece of 256 rows (float64: 128), about 8 bytes per logit, if that is more.
  * Beside it float32 keeps x and w as split planes, 4 bytes per value with
- * rows rounded up to 8 values, 24 bytes per row and 4 per class; float64 8
+ * rows rounded up to 8 values, 24 bytes per row and 8 per class; float64 8
  * bytes per row. With few rows (above) a call takes about 5 M V bytes, a
  * sixteenth of w's and 20 MB whatever workspace_bytes says.
  * No output may overlap an input or another output. The result does

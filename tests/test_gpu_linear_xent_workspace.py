@@ -43,7 +43,7 @@ def bound(M, K, V, dt, workspace):
     """include/gt_cuda.h: what is kept whatever workspace_bytes says, and the larger of it and the smallest piece."""
     if dt:
         return 8 * M + max(workspace, min(M, 128) * (8 * up(V, 2) + 8 * up(K, 2) + 16 * (V // 4096 + 1) + 8)) + SMALL
-    fixed = 4 * (M + V) * up(K, 8) + 24 * M + 4 * up(V, 256)
+    fixed = 4 * (M + V) * up(K, 8) + 24 * M + 8 * up(V, 256)
     per_row = 8 * up(V, 128) + up(V, 128) // 128 * 24 + 12
     return fixed + max(workspace, min(M, 256) * per_row) + SMALL
 
