@@ -50,8 +50,9 @@ constexpr int SSTAGES = 6;
 // epilogue more time under the next tile's first two groups. With 256, sums of positive
 // products came out 13.7 * 2^-23 too small on average, with 128 half of that;
 // dx at V = 517 was off by 1.3e-6 of the result (0.6e-6), dw at 1880 x 1118 x 544 by
-// 1.01e-6 (0.67e-6, where plain float32 sums have 0.59e-6). At 2048 x 1024 x 32000: logits 318 us
-// against 284 with 256, dw 276 against 260, dx 277 either way.
+// 1.01e-6 (0.67e-6, where plain float32 sums have 0.59e-6), the loss at 4096 x 1024 x 65536 by 2.7e-7
+// (1.4e-7; plain 1.0e-7). At 2048 x 1024 x 32000 with z stored through registers: logits 329 us
+// against 299 with 256, dw 276 against 260, dx 277 either way.
 constexpr int SGROUP = kSplitGroup / SBK;
 constexpr int SMIN_SPLIT = 16;                   // stages that a K-split has at least
 constexpr int STHREADS = 384;
@@ -60,9 +61,9 @@ constexpr uint32_t OPER_BYTES = 2 * PLANE_BYTES;
 constexpr uint32_t SSTAGE_BYTES = 2 * OPER_BYTES;
 constexpr int SPROMOTERS = 8;                    // warps
 constexpr int STILE = 256;
-constexpr uint32_t SBAR_OFFSET = SSTAGES * SSTAGE_BYTES;
-constexpr uint32_t SEPI_OFFSET = SBAR_OFFSET + 512;
-constexpr uint32_t SSMEM_BYTES = SEPI_OFFSET + SPROMOTERS * 32 * 32 * 4 + 1024;
+constexpr uint32_t SEPI_OFFSET = SSTAGES * SSTAGE_BYTES;  // (1024-byte aligned: the 128-byte swizzle)
+constexpr uint32_t SBAR_OFFSET = SEPI_OFFSET + SPROMOTERS * 32 * 32 * 4;
+constexpr uint32_t SSMEM_BYTES = SBAR_OFFSET + 512 + 1024;
 static_assert(SSMEM_BYTES <= 232448, "shared memory budget");
 constexpr int64_t STILE_ELEMS = (int64_t)STILE * STILE;
 // The launch gives every thread 65536 / 384 = 170, rounded down to 168: 4
@@ -240,7 +241,7 @@ __device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
 template <bool A_MN, bool B_MN, bool LOGITS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
     split_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                      const SplitArgs s, const SplitUnits su) {
+                      const __grid_constant__ CUtensorMap tmOut, const SplitArgs s, const SplitUnits su) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   SplitShared* sh = (SplitShared*)(smem + SBAR_OFFSET);
@@ -488,11 +489,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
           for (int i = 0; i < 32; i++) z[i] = __fmul_rn(z[i], sc);
         }
         if (dst) {
+          if constexpr (LOGITS) {  // the buffer's last copy has been read
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+          }
 #pragma unroll
           for (int c = 0; c < 8; c++)
             *block_chunk(xpose, lane, c) = make_float4(z[4 * c], z[4 * c + 1], z[4 * c + 2], z[4 * c + 3]);
-          __syncwarp();
-          if (vec && cols == 32) {  // 4 rows x 128 bytes per access
+          if constexpr (LOGITS) {
+            // z goes out by TMA, which leaves these warps to the statistics (its pitch is a multiple of 32); through
+            // registers, 4 rows x 128 bytes at a time, 2048 x 1024 x 32000 took 333 us instead of 302
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0 && rows > 0 && nb < s.ldc) {
+              tma_store_2d(&tmOut, xpose, nb, m0);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+          } else {
+            __syncwarp();
+          }
+          if constexpr (LOGITS) {
+          } else if (vec && cols == 32) {  // 4 rows x 128 bytes per access
             const int r0 = lane >> 3, c = lane & 7;
             float* o = dst + (INDEXED ? 0 : (int64_t)r0 * ld) + 32 * j + 4 * c;
             if (A_MN && s.accumulate && !part) {
@@ -569,6 +586,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
           s.strips[(int64_t)(n0 / kStripCols) * s.strip_rows + m0 + lane] = make_float2(top, sum);
       }
     }
+    if (LOGITS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   tc_fence_before();
@@ -598,6 +616,19 @@ __global__ void split_reduce_kernel(SplitUnits su, SplitArgs s) {
     acc = __fmul_rn(acc, sc);
     *o = s.accumulate ? __fadd_rn(*o, acc) : acc;
   }
+}
+
+// float32 rows x cols of pitch `ld`, stored from 32 x 32 blocks in the 128-byte swizzle (block_chunk).
+static char* out_map(gt_ctx* ctx, CUtensorMap* map, float* out, int64_t rows, int64_t ld) {
+  auto encode = (EncodeTiledFn)ctx->encode_tiled;
+  if (!encode) return errorf("split_gemm: cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[2] = {(cuuint64_t)ld, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 4};
+  cuuint32_t box[2] = {32, 32}, estr[2] = {1, 1};
+  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, (void*)out, dims, strides, box, estr,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return errorf("split_gemm: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return nullptr;
 }
 
 static char* split_map(gt_ctx* ctx, CUtensorMap* map, const HalfPlanes& p, bool mn) {
@@ -661,9 +692,10 @@ static char* split_launch(gt_ctx* ctx, const SplitGemm& g) {
     GT_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SSMEM_BYTES));
     if (ctx->device >= 0 && ctx->device < 64) configured[ctx->device] = true;
   }
-  CUtensorMap ta, tb;
+  CUtensorMap ta, tb, tout{};
   GT_TRY(split_map(ctx, &ta, g.a, A_MN));
   GT_TRY(split_map(ctx, &tb, g.b, B_MN));
+  if (LOGITS && g.out) GT_TRY(out_map(ctx, &tout, g.out, g.M, g.ldc));
   const int64_t m_tiles = ceil_div(g.M, STILE), n_tiles = ceil_div(g.N, STILE), tiles = m_tiles * n_tiles;
   if (tiles > INT32_MAX / 64) return errorf("split_gemm: too many tiles");
   const int64_t free_sms = (int64_t)ctx->sm_count - ctx->gemm_sm_reserve, avail = free_sms >= 2 ? free_sms / 2 : 1;
@@ -687,8 +719,8 @@ static char* split_launch(gt_ctx* ctx, const SplitGemm& g) {
     su.ws = (float*)ws;
   }
   const int64_t units = su.whole + (tiles - su.whole) * su.splits;
-  cudaError_t e = launch_overlapped(ctx, kern, (unsigned)(2 * std::min(units, avail)), STHREADS, SSMEM_BYTES, ta, tb, s,
-                                    su);
+  cudaError_t e = launch_overlapped(ctx, kern, (unsigned)(2 * std::min(units, avail)), STHREADS, SSMEM_BYTES, ta, tb, tout,
+                                    s, su);
   if (e == cudaSuccess && su.splits > 1)
     e = launch_overlapped(ctx, split_reduce_kernel, grid_for(ctx, (tiles - su.whole) * STILE_ELEMS, 256), 256, 0, su, s);
   if (e == cudaSuccess) e = cudaGetLastError();
@@ -706,6 +738,7 @@ char* split_gemm(gt_ctx* ctx, const SplitGemm& g) {
   g_split_used = true;
   if (g.strips) {
     if (g.a_mn || g.b_mn || g.a.grouped) return errorf("split_gemm: the logits' operands are K-major");
+    if (g.ldc % 32 || ((uintptr_t)g.out & 15)) return errorf("split_gemm: the logits' rows come in blocks of 32");
     if (!g.row_scale || !g.col_scale || !g.bias) return errorf("split_gemm: the logits' scales or biases are missing");
     return tc::split_launch<false, false, true>(ctx, g);
   }
