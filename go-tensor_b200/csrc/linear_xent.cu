@@ -94,7 +94,7 @@ __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
 // rows (dw's products read that far). A row's place is the number of rows that
 // count before it: the counts of the 1024-row blocks before its own, and a
 // ballot over the labels of its own (a kernel of its own for this took 4 us more).
-__global__ void __launch_bounds__(256) operand_split_kernel(const float* __restrict__ x, const float* __restrict__ w,
+__global__ void __launch_bounds__(256, 4) operand_split_kernel(const float* __restrict__ x, const float* __restrict__ w,
                                                             const float* __restrict__ bias,
                                                             const int32_t* __restrict__ labels, int64_t M, int64_t K,
                                                             int64_t V, int64_t Kp, int32_t ignore,
@@ -321,6 +321,7 @@ __global__ void __launch_bounds__(512, 2) grad_planes_kernel(float* z, const flo
                                                              float* dw_scale, float* part) {
   after_predecessor();
   __shared__ float tops[16][kGradTile], sums[16][kGradTile];
+  __shared__ float4 about[kGradTile];  // per row: maximum, 1 / sum, xs, and the label's place in the tile
   __shared__ int shift[kGradTile];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t rb = blockIdx.x / across, cb = blockIdx.x - rb * across;
@@ -328,25 +329,36 @@ __global__ void __launch_bounds__(512, 2) grad_planes_kernel(float* z, const flo
   // behind the last row come zeros up to a multiple of 32 rows (dw's products read that far)
   const int64_t end = min(R, (here + 31) / 32 * 32);
   if (m0 >= end) return;
+  const int rows = (int)max((int64_t)0, min((int64_t)kGradTile, here - m0)), zeroed = (int)min((int64_t)kGradTile, end - m0);
+  const int cols = (int)min((int64_t)4, max((int64_t)0, V - c));  // of this lane's four
   const int up_to = meta->up_to;
+  float* zr = z + (m0 + warp) * Vp + c;
   float p[8][4];
 #pragma unroll
   for (int u = 0; u < 8; u++) {
-    const int64_t m = m0 + warp + 16 * u;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (m < here) v = *reinterpret_cast<const float4*>(z + m * Vp + c);
+    if (warp + 16 * u < rows) v = *reinterpret_cast<const float4*>(zr + (int64_t)(16 * u) * Vp);
     p[u][0] = v.x, p[u][1] = v.y, p[u][2] = v.z, p[u][3] = v.w;
   }
+  if (threadIdx.x < rows) {
+    const int64_t m = m0 + threadIdx.x;
+    const float2 s = stat[m];
+    const int64_t at = (int64_t)y[r0 + m] - cb * kGradTile;
+    about[threadIdx.x] = make_float4(s.x, s.y, xs[r0 + m], __int_as_float(at >= 0 && at < kGradTile ? (int)at : -4));
+  }
+  __syncthreads();
   // ws and xs relative to the tile's largest
   float wf[4] = {0.f, 0.f, 0.f, 0.f};
   int w_base = 0, x_base = 0;
   if (DX) {
     const float4 f = *reinterpret_cast<const float4*>(ws + c);
-    if (c < V) wf[0] = f.x;
-    if (c + 1 < V) wf[1] = f.y;
-    if (c + 2 < V) wf[2] = f.z;
-    if (c + 3 < V) wf[3] = f.w;
-    const float top = fmaxf(fmaxf(wf[0], wf[1]), fmaxf(wf[2], wf[3]));
+    wf[0] = f.x, wf[1] = f.y, wf[2] = f.z, wf[3] = f.w;
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if (j >= cols) wf[j] = 0.0f;
+      top = fmaxf(top, wf[j]);
+    }
     w_base = exponent_of(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
 #pragma unroll
     for (int j = 0; j < 4; j++) wf[j] *= exp2_int(-w_base);
@@ -355,31 +367,32 @@ __global__ void __launch_bounds__(512, 2) grad_planes_kernel(float* z, const flo
     float top = 0.0f;
 #pragma unroll
     for (int u = 0; u < 4; u++)
-      if (m0 + lane + 32 * u < here) top = fmaxf(top, xs[r0 + m0 + lane + 32 * u]);
+      if (lane + 32 * u < rows) top = fmaxf(top, about[lane + 32 * u].z);
     x_base = exponent_of(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
   }
+  const float x_unit = exp2_int(-x_base);
   float top[4] = {0.f, 0.f, 0.f, 0.f}, sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int u = 0; u < 8; u++) {
-    const int64_t m = m0 + warp + 16 * u;
-    if (m >= here) {
+    const int row = warp + 16 * u;
+    if (row >= rows) {
 #pragma unroll
       for (int j = 0; j < 4; j++) p[u][j] = 0.0f;
       continue;
     }
-    const float2 s = stat[m];
-    const int64_t at = (int64_t)y[r0 + m] - c;
+    const float4 s = about[row];
 #pragma unroll
     for (int j = 0; j < 4; j++) p[u][j] = exp_exact(p[u][j] - s.x) * s.y;
-    if (at >= 0 && at < 4) {
+    const int at = __float_as_int(s.w) - 4 * lane;
+    if ((unsigned)at < 4u) {
 #pragma unroll
       for (int j = 0; j < 4; j++)
         if (at == j) p[u][j] -= 1.0f;
     }
-    if (c + 3 >= V) {
+    if (cols < 4) {
 #pragma unroll
       for (int j = 0; j < 4; j++)
-        if (c + j >= V) p[u][j] = 0.0f;
+        if (j >= cols) p[u][j] = 0.0f;
     }
     if (DX) {
       float q[4], row_top = 0.0f;
@@ -390,11 +403,11 @@ __global__ void __launch_bounds__(512, 2) grad_planes_kernel(float* z, const flo
       const float f = exp2_int(t);
 #pragma unroll
       for (int j = 0; j < 4; j++) q[j] *= f;
-      __half* o = reinterpret_cast<__half*>(z + m * Vp + cb * kGradTile) + 4 * lane;
+      __half* o = reinterpret_cast<__half*>(zr + (int64_t)(16 * u) * Vp - 4 * lane) + 4 * lane;
       split_store(o, o + kGradTile, q);
-      if (lane == 0) dx_scale[cb * R + m] = exp2_int(-(t - w_base + up_to));
+      if (lane == 0) dx_scale[cb * R + m0 + row] = exp2_int(-(t - w_base + up_to));
     }
-    const float xf = DW ? xs[r0 + m] * exp2_int(-x_base) : 0.0f;
+    const float xf = s.z * x_unit;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       if (DB) sum[j] += p[u][j];
@@ -424,12 +437,12 @@ __global__ void __launch_bounds__(512, 2) grad_planes_kernel(float* z, const flo
     float f[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) f[j] = exp2_int(shift[4 * lane + j]);
+    __half* o = g + (m0 + warp) * Vp + c;
 #pragma unroll
     for (int u = 0; u < 8; u++) {
-      const int64_t m = m0 + warp + 16 * u;
-      if (m >= end) break;
+      if (warp + 16 * u >= zeroed) break;
       const float q[4] = {p[u][0] * f[0], p[u][1] * f[1], p[u][2] * f[2], p[u][3] * f[3]};
-      split_store(g + m * Vp + c, g + m * Vp + c + plane, q);
+      split_store(o + (int64_t)(16 * u) * Vp, o + (int64_t)(16 * u) * Vp + plane, q);
     }
   }
 }
