@@ -180,6 +180,7 @@ HOST_API = {
     "gth_set_sgd": ("err", [_P, ctypes.POINTER(SgdCfg)]),
     "gth_set_adam": ("err", [_P, ctypes.POINTER(AdamCfg)]),
     "gth_set_adamw": ("err", [_P, ctypes.POINTER(AdamCfg), _INT, _D, _INT, ctypes.c_uint64]),
+    "gth_set_adamw_lr": ("err", [_P, _D]),
     "gth_grad_norm": ("err", [_P, ctypes.POINTER(_D)]),
     "gth_set_fused_head": ("err", [_P, _INT, ctypes.c_int32]),
     "gth_input_device": (_P, [_P]),

@@ -153,6 +153,10 @@ class Model:
         check(self.lib.gth_set_adamw(self.ptr, ctypes.byref(AdamCfg(lr, beta1, beta2, eps, weight_decay)), state,
                                      max_norm, int(decay_vectors), seed))
 
+    def adamw_lr(self, lr):
+        """AdamW's learning rate from the next step on, the moments kept (a schedule, captured steps included)."""
+        check(self.lib.gth_set_adamw_lr(self.ptr, lr))
+
     def grad_norm(self) -> float:
         """The gradients' norm at the last clipped AdamW step."""
         out = ctypes.c_double()

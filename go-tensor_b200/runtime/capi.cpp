@@ -99,6 +99,9 @@ GT_API char* gth_set_adamw(gth_model* m, const gt_adam_cfg* cfg, int state, doub
     m->m->set_adamw(*cfg, state, max_norm, decay_vectors != 0, seed);
   });
 }
+GT_API char* gth_set_adamw_lr(gth_model* m, double lr) {
+  return guard([&] { m->m->set_adamw_lr(lr); });
+}
 GT_API char* gth_grad_norm(gth_model* m, double* out) {
   return guard([&] {
     if (!out) throw Error("gth_grad_norm: null output");

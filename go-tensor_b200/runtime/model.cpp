@@ -18,6 +18,7 @@
 #include "model.hpp"
 
 #include <algorithm>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 
@@ -400,6 +401,8 @@ void Model::set_adamw(const gt_adam_cfg& cfg, int state, double max_norm, bool d
   opt_b_ = DevBuf(ctx_, dev_params_ * held);  // v
   opt_scales_ = DevBuf(ctx_, state == GT_STATE_E4M3 ? 2 * blocks * sizeof(float) : 16);
   clip_ = DevBuf(ctx_, 2 * sizeof(double));
+  lr_ = DevBuf(ctx_, sizeof(double));
+  check(gt_upload(ctx_, lr_.get(), &cfg.lr, sizeof(double)));
   check(gt_zero(ctx_, opt_a_.get(), dev_params_ * held));
   check(gt_zero(ctx_, opt_b_.get(), dev_params_ * held));
   check(gt_zero(ctx_, opt_scales_.get(), opt_scales_.bytes()));
@@ -428,6 +431,14 @@ void Model::set_adamw(const gt_adam_cfg& cfg, int state, double max_norm, bool d
   adam_ = cfg;
   max_norm_ = max_norm;
   opt_steps_ = 0;
+}
+
+// The steps read the rate on the device, captured ones included.
+void Model::set_adamw_lr(double lr) {
+  if (opt_ != OPT_ADAMW) throw Error("gth_set_adamw_lr: needs AdamW (gth_set_adamw)");
+  if (!std::isfinite(lr)) throw Error("gth_set_adamw_lr: the learning rate must be finite");
+  check(gt_upload(ctx_, lr_.get(), &lr, sizeof lr));
+  adam_.lr = lr;
 }
 
 double Model::grad_norm() {
@@ -694,7 +705,7 @@ void Model::optimizer_step() {
     if (world_ > 1) check(gt_comm_wait(ctx_));
     double* clip = max_norm_ > 0 ? (double*)clip_.get() : nullptr;
     if (clip) check(gt_adamw_clip(adamw_, max_norm_, clip));
-    check(gt_adamw_step(adamw_, &adam_, clip, nullptr));
+    check(gt_adamw_step(adamw_, &adam_, clip, (const double*)lr_.get()));
   } else {
     if (world_ > 1) check(gt_comm_wait(ctx_));
     check(gt_adam_step_dev(ctx_, dtype_, pbuf_.get(), gbuf_.get(), opt_a_.get(), opt_b_.get(), dev_params_, &adam_,

@@ -118,6 +118,7 @@ class Model {
   void set_sgd(const gt_sgd_cfg& cfg);
   void set_adam(const gt_adam_cfg& cfg);
   void set_adamw(const gt_adam_cfg& cfg, int state, double max_norm, bool decay_vectors, uint64_t seed);
+  void set_adamw_lr(double lr);
   double grad_norm();  // of the last clipped AdamW step
   // The last Linear and the loss as one call over pieces of the logits.
   void set_fused_head(bool on, int32_t ignore_label);
@@ -197,7 +198,8 @@ class Model {
 
   enum { OPT_NONE, OPT_SGD, OPT_ADAM, OPT_ADAMW } opt_ = OPT_NONE;
   gt_adamw* adamw_ = nullptr;
-  DevBuf opt_scales_, clip_;  // AdamW: scales of 8-bit states; the norm and the clipping coefficient
+  // AdamW: scales of 8-bit states; the norm and the clipping coefficient; the learning rate
+  DevBuf opt_scales_, clip_, lr_;
   double max_norm_ = 0;       // 0: no clipping
   bool fused_head_ = false;
   int32_t ignore_label_ = -1;

@@ -79,6 +79,9 @@ GT_API char* gth_set_adam(gth_model* m, const gt_adam_cfg* cfg);
  * reference. */
 GT_API char* gth_set_adamw(gth_model* m, const gt_adam_cfg* cfg, int state, double max_norm, int decay_vectors,
                            uint64_t seed);
+/* AdamW's learning rate from the next step on, states and step counter kept
+ * (a schedule; steps replayed as a graph follow it). */
+GT_API char* gth_set_adamw_lr(gth_model* m, double lr);
 /* The gradients' norm at the last clipped AdamW step (synchronizes). */
 GT_API char* gth_grad_norm(gth_model* m, double* out);
 /* With on != 0, training runs the last Linear, the softmax cross-entropy and

@@ -110,3 +110,40 @@ def test_shares_of_a_batch(dt, M, K, V, ignored):
     for g, n in zip(got, counts):
         if n == 0:
             assert g["loss"][0] == 0 and not g["dx"].any() and not g["dw"].any() and not g["db"].any()
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("state", [0, 1])
+def test_learning_rate_schedule(state, graph):
+    """The rate of each step, moments kept: bit for bit the operator's steps with that rate, also when the captured step
+    is replayed."""
+    from gpu_common import assert_bits
+    from test_gpu_head_step import ADAM, ByHand, batches, make
+    m = make()
+    m.fused_head()
+    m.adamw(state=state, max_norm=0.3, seed=11, **ADAM)
+    m.enable_graph(graph)
+    hand = ByHand(m, state, 0.3)
+    x, y = batches(1)[0]
+    m.set_batch(x, y)
+    for i, lr in enumerate([None, 1e-3, 4e-3, 4e-3, 0.0, 2e-4]):
+        if lr is not None:
+            m.adamw_lr(lr)
+            hand.opt.cfg.lr = lr
+        before = m.flat_params()
+        m.train_step()
+        hand.step(x, y)
+        for k, v in m.state_dict().items():
+            assert_bits(v.reshape(-1), hand.p[k].host().reshape(-1), (i, k))
+        assert (m.flat_params() != before).any() == (lr != 0.0)
+
+
+def test_learning_rate_refusals():
+    from gotensor._lib import GTError
+    m = gm.Model([gm.Linear(4, 4)], [2, 4])
+    with pytest.raises(GTError, match="needs AdamW"):
+        m.adamw_lr(1e-3)
+    m.adamw()
+    for lr in (float("nan"), float("inf")):
+        with pytest.raises(GTError, match="finite"):
+            m.adamw_lr(lr)
