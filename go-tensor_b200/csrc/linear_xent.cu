@@ -74,9 +74,10 @@ __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint3
 
 // The exponent e that puts a largest magnitude at 2^14 .. 2^15 when
 // multiplied by 2^e: -113 .. 126. (2^126 is enough for any: what a plane then
-// loses is below 2^-150, half of the smallest float32.)
+// loses is below 2^-150, half of the smallest float32.) A row of zeros has 126
+// too, so that G weighted with 2^-e counts it for nothing beside others.
 __device__ __forceinline__ int plane_exponent(uint32_t top) {
-  if (top == 0) return 0;
+  if (top == 0) return 126;
   return min(126, 14 - (top < 0x800000u ? 31 - __clz((int)top) - 149 : (int)(top >> 23) - 127));
 }
 
@@ -268,9 +269,10 @@ __global__ void __launch_bounds__(1024) strip_join_kernel(const float2* strips, 
 // float16 planes for each of the products that it goes into, and, for db, summed over the rows.
 //
 // dx = G w sums over classes, whose rows of w have scales of their own, and dw = G^T x over
-// rows of x. So the planes for dx hold q 2^T with q = n G ws[v] / (the largest ws of
-// the tile's columns), T of the row and the tile such that the largest |q| lands at 2^14 .. 2^15; those for
-// dw the same with xs of the tile's rows and a T of the column. A class that is far from
+// rows of x. So the planes for dx hold q 2^T with q = n G ws[v] (and, where the tile's largest ws
+// is below 1, a factor 2^-base that makes it 1: q stays a normal number), T of the row and
+// the tile such that the largest |q| lands at 2^14 .. 2^15; those for dw the same with xs of
+// the tile's rows and a T of the column. A class that is far from
 // likely so keeps its digits in dw beside those that are likely, as does a
 // row of small gradients in dx. What undoes it goes to dx_scale and dw_scale, with
 // 2^-up_to, whose rest, share, the products multiply by at the end (no sum
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(512, 2) grad_planes_kernel(float* z, const flo
     about[threadIdx.x] = make_float4(s.x, s.y, xs[r0 + m], __int_as_float(at >= 0 && at < kGradTile ? (int)at : -4));
   }
   __syncthreads();
-  // ws and xs relative to the tile's largest
+  // ws and xs relative to the tile's largest where that is below 1
   float wf[4] = {0.f, 0.f, 0.f, 0.f};
   int w_base = 0, x_base = 0;
   if (DX) {
@@ -359,7 +361,7 @@ __global__ void __launch_bounds__(512, 2) grad_planes_kernel(float* z, const flo
       if (j >= cols) wf[j] = 0.0f;
       top = fmaxf(top, wf[j]);
     }
-    w_base = exponent_of(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
+    w_base = min(0, exponent_of(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)))));
 #pragma unroll
     for (int j = 0; j < 4; j++) wf[j] *= exp2_int(-w_base);
   }
@@ -368,7 +370,7 @@ __global__ void __launch_bounds__(512, 2) grad_planes_kernel(float* z, const flo
 #pragma unroll
     for (int u = 0; u < 4; u++)
       if (lane + 32 * u < rows) top = fmaxf(top, about[lane + 32 * u].z);
-    x_base = exponent_of(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
+    x_base = min(0, exponent_of(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)))));
   }
   const float x_unit = exp2_int(-x_base);
   float top[4] = {0.f, 0.f, 0.f, 0.f}, sum[4] = {0.f, 0.f, 0.f, 0.f};

@@ -164,3 +164,40 @@ def test_long_sums_of_few_rows(M, K):
     z = x.astype(np.float64) @ w[1].astype(np.float64)
     runs = -(-K // 8192)
     assert (np.abs((got - z) / z) <= (128 + 5 + runs + 1) * U).all()
+
+
+@pytest.mark.parametrize("what", ["x", "w"])
+@pytest.mark.parametrize("M", [140, 300])
+def test_rows_of_zeros(M, what):
+    """Every other row of x, or of w, is zero: they add nothing to dw, or dx, so what they carry of G may not cost the
+    others' digits. The rows that are not zero are sure of their labels (their G is 2^-20 and below); those that are see
+    equal logits, or the classes of zeros are the likely ones."""
+    x, w, b, y = inputs(M, 64, 600, 10, 0, gain=12.0)
+    if what == "x":
+        z = x.astype(np.float64) @ w.astype(np.float64).T + b
+        y = np.where(np.arange(M) % 2 == 0, z.argmax(1), y)
+        for i in range(0, M, 2):  # far ahead of the second
+            w[y[i]] += 0.5 * x[i]
+        z = x.astype(np.float64) @ w.astype(np.float64).T + b
+        y = np.where(np.arange(M) % 2 == 0, z.argmax(1), y)
+        x[1::2] = 0
+    else:
+        w[1::2] = 0
+        b[1::2] = 40
+        b[0::2] -= 20
+        y = y // 2 * 2 + 1
+    compare(Head(x, w, b, y, 0).call().host(), *reference(x, w, b, y))
+
+
+@pytest.mark.parametrize("factor", [1e20, 1e30, 1e36])
+def test_unlikely_classes_beside_large_masked_ones(factor):
+    """Far larger weights of a masked class in each group of 128; the classes that are left are 2^-20 to 2^-60 likely but
+    for one in the first group, and its row of w is zero: dx is what they add."""
+    x, w, b, y = inputs(200, 64, 1000, 11, 0, gain=3.0)
+    w[5] = 0
+    y[:] = 5
+    b[:] -= 40
+    b[5] = 0
+    b[64::128] = -np.inf
+    w[64::128] *= np.float32(factor)
+    compare(Head(x, w, b, y, 0).call().host(), *reference(x, w, b, y))
