@@ -3,7 +3,7 @@
 //
 // With so few rows the call is bound by latency when w is small, by reading w
 // twice and writing dw once when it is large; splitting w into planes first, as the
-// tensor-core path does, moves 12 more bytes per value, and its 256-row tiles
+// tensor-core path does, moves 8 more bytes per value, and its 256-row tiles
 // are mostly empty. So the products run on the FP32 pipe from w as it is:
 //
 //   few_logits_kernel  a block per strip of classes: z for all rows, the strip's
@@ -18,9 +18,9 @@
 // Sums are float32 in runs of at most 256 (logits) or 1024 (dx) terms of a thread
 // that are then added up, so they stay as exact as the tensor-core path's.
 //
-// Measured (the tensor-core path in brackets): 7 x 96 x 517 17 us (62), 64 x 128 x
-// 1000 39 us (82), 64 x 512 x 5000 105 us (103), 8 x 2048 x 50000 395 us (600; w read
-// twice and dw written once take 190 at HBM rate), 16 x 2048 x 50000 674 us (583): it
+// Measured (the tensor-core path in brackets): 7 x 96 x 517 17 us (54), 64 x 128 x
+// 1000 37 us (65), 64 x 512 x 5000 94 us (73), 8 x 2048 x 50000 393 us (503; w read
+// twice and dw written once take 190 at HBM rate), 16 x 2048 x 50000 660 us (494): it
 // is bound by shared-memory reads there, so the choice goes by the products'
 // size (few_rows).
 #include <algorithm>
