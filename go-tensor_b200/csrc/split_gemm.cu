@@ -420,7 +420,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(STHREADS, 1)
       if constexpr (LOGITS) {
         const float r = lane < rows ? s.row_scale[m0 + lane] : 1.0f;
         down = fminf(r, 1.0f), up_again = fmaxf(r, 1.0f);
-        if (lane < 8) asm volatile("prefetch.global.L1 [%0];" ::"l"((lane < 4 ? s.col_scale : s.bias) + n0 + 32 * (lane & 3)));
+        if (lane < 8)
+          asm volatile("prefetch.global.L1 [%0];" ::"l"((lane < 4 ? s.col_scale : s.bias) + n0 + 32 * (lane & 3)));
       }
       float tot[128];
 #pragma unroll
