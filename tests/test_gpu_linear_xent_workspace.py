@@ -1,11 +1,11 @@
 """The head loss' memory: what a call takes from the pool at its highest, beside the documented bound."""
 import ctypes
+import gc
 
-import numpy as np
 import pytest
 
 from gpu_common import cuda_backend
-from test_gpu_linear_xent import IGN, Head, compare, inputs, reference
+from test_gpu_linear_xent import Head, compare, inputs, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -26,13 +26,18 @@ class Pool:
 
     def taken(self, call):
         """The bytes that call() had from the pool at once."""
-        cuda_backend().Sync()
-        zero = ctypes.c_uint64(0)
-        assert self.cu.cuMemPoolSetAttribute(self.pool, USED_HIGH, ctypes.byref(zero)) == 0
-        before = self.get(USED_CURRENT)
-        call()
-        cuda_backend().Sync()
-        return self.get(USED_HIGH) - before
+        gc.collect()
+        gc.disable()  # storages that go while this looks would count as the call's
+        try:
+            cuda_backend().Sync()
+            zero = ctypes.c_uint64(0)
+            assert self.cu.cuMemPoolSetAttribute(self.pool, USED_HIGH, ctypes.byref(zero)) == 0
+            before = self.get(USED_CURRENT)
+            call()
+            cuda_backend().Sync()
+            return self.get(USED_HIGH) - before
+        finally:
+            gc.enable()
 
 
 def up(n, to):
